@@ -1,4 +1,4 @@
-"""ctypes binding of libjeeves_fp8.so (the C ABI in include/jeeves_fp8.h).
+"""ctypes binding of libjeeves_fp8.so (the C ABI in include/*.h).
 
 The library is loaded from this package's directory only: the FP8 path has no
 CPU or PyTorch fallback, so a missing or unloadable library raises.
@@ -15,7 +15,7 @@ LIB_PATH = Path(__file__).resolve().with_name("libjeeves_fp8.so")
 
 JV_OK, JV_ERR_VALUE, JV_ERR_RUNTIME, JV_ERR_HIP = 0, 1, 2, 3
 
-# name -> (restype, argtypes); mirrors include/jeeves_fp8.h
+# name -> (restype, argtypes); mirrors include/jeeves_fp8.h and include/jeeves_attention.h
 SIGNATURES: dict[str, tuple] = {
     "jv_fp8_last_error": (c_char_p, []),
     "jv_device_cu_count": (c_int, [c_int]),
@@ -51,6 +51,16 @@ SIGNATURES: dict[str, tuple] = {
     "jv_fp8_counters_needed": (c_int64, [c_int64, c_int64, c_int64, c_int]),
     "jv_fp8_quantizes_in_gemm": (c_int, [c_int64, c_int64, c_int64, c_int, c_int, c_int]),
     "jv_fp8_launch_shape": (c_int, [c_int64, c_int64, c_int64, c_int, POINTER(c_int32)]),
+    # include/jeeves_attention.h
+    "jv_norm_rope": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int,
+                             c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]),
+    "jv_append_kv": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_int64,
+                             c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p, c_float, c_void_p, c_int64, c_int64,
+                             c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]),
+    "jv_paged_attention_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int]),
+    "jv_paged_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                   c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_float, c_void_p, c_int64, c_int64, c_int64,
+                                   c_int64, c_int, c_void_p, c_int64, c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,945 @@
+// Attention over the paged cache for a ragged batch, each sequence's queries
+// before the keys it owns (causal, the last query at the last key) and, where
+// the batch shares a prefix, all of the prefix's keys.
+//
+// For a query row q: o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m) over the
+// keys it sees, s_j = scale q.k_j, in one pass over the keys with a running
+// reference r in place of m: weights 2^(s_j scale log2(e) - r), and sums and
+// outputs scaled by 2^(r - r') when r moves to r'. r only has to stay within
+// 2^8 of the largest weight, so it moves when a score exceeds it by 8, not at
+// every new maximum; until then a step needs no exchange between lanes and no
+// rescaling. Each row's reference moves by its own scores alone, so a row's
+// bits do not depend on the rows beside it. Scores, weights' sums and outputs are fp32; the weights are
+// rounded to the 16-bit type for the product with V (a relative 2^-9 or 2^-12
+// at most for bf16 and fp16, of mixed signs); their sum is that of the unrounded
+// ones. fp16 weights are 2^7 larger, up to 2^15, so that those that many keys
+// share stay normal numbers.
+//
+// Both products run on MFMA with the keys on the A side: S^T = K Q^T leaves
+// each lane the scores of one query row, and the score tile's registers are,
+// with no move between lanes, the B operand of O^T = V^T P^T, if V^T's k slots
+// take the keys in the same order; ds_read_b64_tr_b16 reads V that way from
+// row-major tiles. So a row's reference, sum and rescaling are one lane's.
+//
+// K and V tiles go from global memory to LDS directly (16 bytes a lane), with
+// their 16-byte chunks XOR-swizzled so that both kinds of reads meet 256
+// bytes of distinct banks.
+#include "attention.h"
+
+namespace jv {
+
+constexpr float kRescaleAt = 8.0f;
+
+__device__ __forceinline__ void load_lds16(const uint8_t* src, uint8_t* dst_wave_base) {
+  typedef __attribute__((address_space(3))) void lds_void;
+  typedef __attribute__((address_space(1))) void global_void;
+  __builtin_amdgcn_global_load_lds((global_void*)(src), (lds_void*)(dst_wave_base), 16, 0, 0);
+}
+
+// s_waitcnt with only the vector-memory counter constrained (vmcnt in bits 3:0
+// and 15:14; expcnt and lgkmcnt left at their maxima).
+template <int N>
+__device__ __forceinline__ void wait_vmem_below() {
+  static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+__device__ __forceinline__ i32x4 lds_read16(const uint8_t* p) { return *reinterpret_cast<const i32x4*>(p); }
+
+// Four 16-bit values of one column: of the 4 x 16 block that 16 consecutive
+// lanes address (8 bytes a lane, four lanes a row), lane i gets column i.
+__device__ __forceinline__ s16x4 lds_read_tr(const uint8_t* p) {
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
+}
+
+// The same for four addresses, each at OFF and at OFF + STEP bytes: the four
+// 8-value operands that the pairs make. As one block with its wait, because
+// before the builtin the compiler waits for every copy to LDS in flight, the
+// next tile's too; the block waits for the LDS reads alone.
+template <int OFF, int STEP>
+__device__ __forceinline__ void lds_read_tr4(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, i32x4* out) {
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  i32x2 x[8];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%c12\n"
+      "ds_read_b64_tr_b16 %1, %8 offset:%c13\n"
+      "ds_read_b64_tr_b16 %2, %9 offset:%c12\n"
+      "ds_read_b64_tr_b16 %3, %9 offset:%c13\n"
+      "ds_read_b64_tr_b16 %4, %10 offset:%c12\n"
+      "ds_read_b64_tr_b16 %5, %10 offset:%c13\n"
+      "ds_read_b64_tr_b16 %6, %11 offset:%c12\n"
+      "ds_read_b64_tr_b16 %7, %11 offset:%c13\n"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+      : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(OFF), "n"(OFF + STEP)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = i32x4{x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y};
+}
+
+// LDS byte address of a pointer into a __shared__ array.
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  typedef __attribute__((address_space(3))) const uint8_t lds_u8;
+  return (uint32_t)(uintptr_t)(lds_u8*)p;
+}
+
+__device__ __forceinline__ i32x4 cat_tr(s16x4 a, s16x4 b) {
+  return __builtin_bit_cast(i32x4, s16x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w});
+}
+
+// A tile's rows are D / 8 chunks of 16 bytes; what XORs a row's chunk index.
+// LDS serves 256 bytes (64 banks) at a time. K is read 16 rows at one chunk:
+// the row within the rows that start at bank 0 separates them. V is read by
+// 32 lanes, 4 rows x 4 chunks or 8 rows x 2: bits 2 and 1 from the row.
+template <int D>
+__device__ __forceinline__ int k_swizzle(int row) {
+  return D == 64 ? (row >> 1) & 7 : row & 15;
+}
+template <int D>
+__device__ __forceinline__ int v_swizzle(int row) {
+  if constexpr (D == 64) return ((row >> 1) & 1) * 4 + ((row >> 2) & 1) * 2;
+  else return (row & 3) * 4 + ((row >> 2) & 1) * 2;
+}
+
+// ---------------------------------------------------------------------------
+// Which rows and keys a workgroup has.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ int clamped(int v, int lo, int hi) { return max(lo, min(v, hi)); }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// A value of an array that no kernel of the call writes, by a scalar load
+// where the index is the same in all lanes.
+__device__ __forceinline__ int32_t read_only(const int32_t* p, int64_t i) {
+  typedef __attribute__((address_space(4))) const int32_t constant_i32;
+  return ((constant_i32*)p)[i];
+}
+
+__device__ __forceinline__ int start_of(const AttnArgs& a, int b) {
+  return a.starts ? clamped(read_only(a.starts, b), 0, a.tokens) : b;
+}
+
+// First tile slot of a sequence whose queries start at token `start`.
+__device__ __forceinline__ int first_tile(const AttnArgs& a, int b, int start, int rows) {
+  if (!a.starts && a.group <= rows) return b;
+  return (int)(((uint32_t)start * (uint32_t)a.group) / (uint32_t)rows) + b;
+}
+
+// A sequence of the batch: its first token, its tokens and its own keys.
+struct Sequence {
+  int start, n, len;
+};
+__device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b) {
+  Sequence s{b, 1, clamped(read_only(a.lengths, b), 0, a.table_cols << a.page_shift)};
+  if (a.starts) {
+    s.start = clamped(read_only(a.starts, b), 0, a.tokens);
+    s.n = max(0, clamped(read_only(a.starts, b + 1), 0, a.tokens) - s.start);
+  }
+  return s;
+}
+
+// The sequence that a tile slot belongs to: the last whose first slot is not
+// past it, 64 sequences a step (every lane active, the same slot in each).
+__device__ __forceinline__ int sequence_of_slot(const AttnArgs& a, int slot, int rows) {
+  if (!a.starts && a.group <= rows) return min(slot, a.batch - 1);
+  const int lane = threadIdx.x & 63;
+  int count = 0;
+  for (int base = 0; base < a.batch; base += 64) {
+    const int b = base + lane;
+    const int c = __popcll(__ballot(b < a.batch && first_tile(a, b, start_of(a, min(b, a.batch - 1)), rows) <= slot));
+    count += c;
+    if (c < 64) break;
+  }
+  return max(count - 1, 0);
+}
+
+// Sums over the lanes up to each one (DPP row shifts, then row 0's total into
+// row 1 and row 2's into row 3, then the lower half's into the upper).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);  // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);  // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);  // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return v;
+}
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+__device__ __forceinline__ float wave_sum_f32(float v) {
+#pragma unroll
+  for (int s = 1; s < 64; s *= 2) v += __shfl_xor(v, s);
+  return v;
+}
+
+// Where keys are split over workgroups: the (sequence, row tile, key chunk) of
+// a unit. The tiles' keys are added up (in groups of 16, which the host has
+// checked to fit 32 bits), the sum cut into about `own_target` chunks of
+// `keys` keys, and each tile of a sequence gets ceil(len / keys) units of equal
+// shares of what it sees. Computed by each wave for itself, 64 sequences a
+// step, from the lengths on the device.
+struct Unit {
+  int b, first, tile, chunk, chunks;  // sequence, its first unit, row tile and chunk of the unit, chunks of a tile
+  int keys;
+  Sequence seq;
+};
+__device__ __forceinline__ int chunk_keys(int groups, int target, int grain) {
+  const int each = (int)((uint32_t)groups / (uint32_t)target) * 16 + 16;
+  return max(2 * grain, (each + grain - 1) / grain * grain);
+}
+// False if there is no such unit; keys is set in any case.
+__device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int rows, int grain, Unit* u) {
+  const int lane = threadIdx.x & 63, steps = (a.batch + 63) >> 6;
+  int groups = 0, before = 0;
+  Sequence s;
+  u->keys = 0;
+  // `steps` steps to add the keys up, `steps` more to find the unit; up to 64
+  // sequences are read once
+  for (int i = 0; i < 2 * steps; ++i) {
+    const int base = (i < steps ? i : i - steps) * 64;
+    if (i == 0 || steps > 1) {
+      s = sequence(a, min(base + lane, a.batch - 1));
+      if (base + lane >= a.batch) s.n = 0;
+    }
+    const int tiles = (int)((uint32_t)(s.n * a.group + rows - 1) / (uint32_t)rows);
+    if (i < steps) {
+      groups += lane_value(wave_scan(tiles * ((s.len + 15) >> 4)), 63);
+      if (i + 1 == steps) u->keys = uniform(chunk_keys(groups, a.p.own_target, grain));
+      continue;
+    }
+    const int chunks = (int)((uint32_t)(s.len + u->keys - 1) / (uint32_t)u->keys), n = tiles * chunks;
+    const int upto = wave_scan(n);
+    const uint64_t past = __ballot(before + upto > unit);
+    if (past) {
+      const int l = uniform(__ffsll((unsigned long long)past) - 1);
+      u->b = base + l;
+      u->first = before + lane_value(upto, l) - lane_value(n, l);
+      u->chunks = lane_value(chunks, l);
+      u->tile = uniform((int)((uint32_t)(unit - u->first) / (uint32_t)u->chunks));
+      u->chunk = unit - u->first - u->tile * u->chunks;
+      u->seq = Sequence{lane_value(s.start, l), lane_value(s.n, l), lane_value(s.len, l)};
+      return true;
+    }
+    before += lane_value(upto, 63);
+  }
+  return false;
+}
+
+// Own keys that the last of `rows` rows from row0 on sees.
+__device__ __forceinline__ int visible_keys(const Sequence& s, int row0, int rows, int group) {
+  return max(0, s.len - s.n + (int)((uint32_t)(row0 + rows - 1) / (uint32_t)group) + 1);
+}
+
+// A run of keys that a workgroup goes through: page ids, the first and the
+// last key (inclusive).
+struct Keys {
+  const int32_t* ids;
+  int first, last;
+};
+
+// What a workgroup does: up to two runs of keys (the prefix's, then the
+// sequence's own) for `rows` query rows, and where the result goes. Every
+// field is the same in all lanes.
+struct Job {
+  Keys prefix, own;
+  int tiles0, tiles;       // key tiles of the prefix, of both
+  int token0, row0, rows;  // query row r: token token0 + (row0 + r) / group
+  int own_base;            // own key index that row r sees last: own_base + (row0 + r) / group
+  bool whole;              // the result is the output; else the partial one of slot `part`
+  int64_t part;
+};
+
+// kWhole: a row tile's prefix and own keys, all of them. kOwn: one chunk of
+// its own keys. kPrefix: one share of the prefix for a tile of all the tokens'
+// rows.
+enum Mode { kWhole, kOwn, kPrefix };
+
+// Fills a job from the block index; false if the block has nothing to do.
+template <Mode MODE, int ROWS, int KT, int GRAIN>
+__device__ __forceinline__ bool find_job(const AttnArgs& a, int unit, int head, Job* j) {
+  j->prefix = j->own = Keys{a.prefix_pages, 0, -1};
+  j->tiles0 = 0;
+  j->part = (int64_t)unit * a.kv_heads + head;
+  if constexpr (MODE == kPrefix) {
+    const int splits = a.p.prefix_splits, tile = (int)((uint32_t)unit / (uint32_t)splits), s = unit - tile * splits;
+    const int each = (int)(((uint32_t)(a.prefix_len + splits - 1) / (uint32_t)splits + GRAIN - 1) / GRAIN) * GRAIN;
+    j->prefix.first = min(s * each, a.prefix_len);
+    j->prefix.last = min(j->prefix.first + each, a.prefix_len) - 1;
+    j->token0 = 0;
+    j->row0 = tile * ROWS;
+    j->rows = min(ROWS, a.tokens * a.group - j->row0);
+    j->own_base = -1;
+    j->whole = false;
+    j->tiles0 = j->tiles = (j->prefix.last - j->prefix.first + KT) / KT;
+    return true;
+  }
+  Sequence s;
+  int b, chunk = 0, chunks = 1;
+  if constexpr (MODE == kOwn) {
+    Unit u;
+    const bool found = find_unit(a, unit, ROWS, GRAIN, &u);
+    if (threadIdx.x == 0 && head == 0) {
+      if (unit == 0) a.info[0] = u.keys;
+      if (found && unit == u.first) a.info[1 + u.b] = u.first;
+    }
+    if (!found) return false;
+    s = Sequence{uniform(u.seq.start), uniform(u.seq.n), uniform(u.seq.len)};
+    b = uniform(u.b), chunk = uniform(u.chunk), chunks = uniform(u.chunks);
+    j->row0 = uniform(u.tile) * ROWS;
+  } else {
+    b = uniform(sequence_of_slot(a, unit, ROWS));
+    s = sequence(a, b);
+    s = Sequence{uniform(s.start), uniform(s.n), uniform(s.len)};
+    j->row0 = uniform((unit - first_tile(a, b, s.start, ROWS)) * ROWS);
+    // a slot before those of a first sequence that starts late
+    if (j->row0 < 0) return false;
+  }
+  j->rows = min(ROWS, s.n * a.group - j->row0);
+  if (j->rows <= 0) return false;
+  const int visible = uniform(visible_keys(s, j->row0, j->rows, a.group));
+  j->own.ids = a.table + b * a.table_stride;
+  j->own.last = visible - 1;
+  j->token0 = s.start;
+  j->own_base = s.len - s.n;
+  j->whole = true;
+  if constexpr (MODE == kOwn) {
+    const int each = uniform((int)(((uint32_t)(visible + chunks - 1) / (uint32_t)chunks + GRAIN - 1) / GRAIN) * GRAIN);
+    j->own.first = min(chunk * each, visible);
+    j->own.last = min(j->own.first + each, visible) - 1;
+    j->whole = chunks == 1 && a.prefix_len == 0;
+  } else {
+    j->prefix.last = a.prefix_len - 1;
+    j->tiles0 = (a.prefix_len + KT - 1) / KT;
+  }
+  j->tiles = j->tiles0 + (j->own.last - j->own.first + KT) / KT;
+  return true;
+}
+
+// A job's fields again as values that the compiler knows to be the same in all
+// lanes (page ids then come by scalar loads).
+__device__ __forceinline__ Keys uniform(const Keys& k) {
+  const uint64_t p = (uint64_t)k.ids;
+  const uint64_t ids = (uint32_t)uniform((int)(uint32_t)p) | (uint64_t)(uint32_t)uniform((int)(p >> 32)) << 32;
+  return Keys{(const int32_t*)ids, uniform(k.first), uniform(k.last)};
+}
+__device__ __forceinline__ Job uniform(const Job& j) {
+  return Job{uniform(j.prefix), uniform(j.own),  uniform(j.tiles0),   uniform(j.tiles),      uniform(j.token0),
+             uniform(j.row0),   uniform(j.rows), uniform(j.own_base), uniform(j.whole) != 0, j.part};
+}
+
+// One 1 KB copy of a key tile: rows [row, row + 1024 / (2 D)) of the tile that
+// starts at key0, from page memory to LDS. Keys past the run's last come from
+// its last 16 keys' group or are the last key again, so nothing outside a
+// sequence's keys is read; the scores mask them.
+template <int D>
+struct Copier {
+  const uint8_t* base;  // this head's first page
+  int64_t page_bytes;   // of all heads
+  int page_shift, pages;
+  __device__ __forceinline__ void operator()(const Keys& r, int key0, int row, uint8_t* dst, int swizzled_chunk,
+                                             int lane_row) const {
+    const int group = min((key0 + row) & ~15, r.last & ~15);  // one for the wave
+    const uint32_t id = min((uint32_t)max(read_only(r.ids, group >> page_shift), 0), (uint32_t)(pages - 1));
+    const uint8_t* from = base + (int64_t)id * page_bytes + (group & ((1 << page_shift) - 1)) * (2 * D);
+    const uint32_t at = (uint32_t)min((row & 15) + lane_row, r.last - group);
+    load_lds16(from + (at * (2 * D) + (uint32_t)swizzled_chunk * 16), dst);
+  }
+};
+
+__device__ __forceinline__ int copy_chunk(int lane, int chunks, int swizzle) { return (lane & (chunks - 1)) ^ swizzle; }
+
+// Output rows: o of channels d .. d + 3 of a row, as the 16-bit type.
+template <class H>
+__device__ __forceinline__ void store4(uint16_t* p, f32x4 o) {
+  *reinterpret_cast<uint2*>(p) = uint2{H::pack(o.x, o.y), H::pack(o.z, o.w)};
+}
+
+// Non-finite values of V where some row does not see them. 0 * V is not 0
+// there, so a key tile that is masked for any row is looked through before its
+// product; if it holds such values (rare), they are set to 0 in LDS and each
+// channel's first key of each kind is noted. A row sees a channel's values
+// if it sees the first, so at the end the output takes what the noted ones
+// bring: NaN, or an infinity of the one sign that it sees.
+constexpr int kNever = 0x7FFFFFFF, kAlways = -kNever;
+template <int D>
+struct NonFinite {
+  int first[3 * D];  // NaN, +inf, -inf of each channel: the key's index, kNever if there is none
+  int tile;          // a tile that holds some, plus 1
+};
+
+template <int D>
+__device__ __forceinline__ void init_non_finite(NonFinite<D>* n, int threads) {
+  for (int i = threadIdx.x; i < 3 * D; i += threads) n->first[i] = kNever;
+  if (threadIdx.x == 0) n->tile = 0;
+}
+
+// Whether any of the wave's 16-byte chunks of a tile (64 lanes x STEPS, from
+// v = tile + lane * 16 on) has all exponent bits set in some 16-bit value.
+template <class H, int STEPS>
+__device__ __forceinline__ bool holds_non_finite(const uint8_t* v) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const i32x4 x = lds_read16(v + i * 1024);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      bad |= ((uint32_t)x[e] & H::kInf) == H::kInf || (((uint32_t)x[e] >> 16) & H::kInf) == H::kInf;
+  }
+  return __any(bad);
+}
+
+// Sets the non-finite values of the same chunks to 0 and notes them. key0: key
+// index of the tile's row 0, or kAlways where every row sees the tile's keys;
+// rows past the run's last key (copies of it) are not noted.
+template <class H, int D, int STEPS>
+__device__ __forceinline__ void take_non_finite(uint8_t* tile, int chunk0, int key0, int rows, NonFinite<D>* n) {
+#pragma unroll 1
+  for (int i = 0; i < STEPS * 8; ++i) {
+    const int chunk = chunk0 + (i >> 3) * 64, row = chunk / (D / 8);
+    uint16_t* at = reinterpret_cast<uint16_t*>(tile + chunk * 16) + (i & 7);
+    const uint32_t x = *at, m = x & 0x7FFFu;
+    if (m < H::kInf) continue;
+    *at = 0;
+    if (row >= rows) continue;
+    const int d = ((chunk % (D / 8)) ^ v_swizzle<D>(row)) * 8 + (i & 7);
+    atomicMin(&n->first[(m > H::kInf ? 0 : x == H::kInf ? D : 2 * D) + d], key0 == kAlways ? kAlways : key0 + row);
+  }
+}
+
+// The output of channel d for a row that sees the own keys up to `sees`.
+template <int D>
+__device__ __forceinline__ float with_non_finite(float o, const NonFinite<D>& n, int d, int sees) {
+  const bool up = n.first[D + d] <= sees, down = n.first[2 * D + d] <= sees;
+  if (n.first[d] <= sees || (up && down)) return __builtin_nanf("");
+  return up ? o + __builtin_inff() : down ? o - __builtin_inff() : o;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows (up to 16): a decode step. HBM-bound: each wave streams 32-key
+// tiles of its own through its own ring of two stages, with no barrier, and
+// the waves' results meet in LDS at the end. 16x16x32 MFMA; a lane holds row
+// lane % 16 and keys 4 (lane / 16) + 0..3 of each 16.
+// ---------------------------------------------------------------------------
+template <int D>
+struct Few {
+  static constexpr int kWaves = D == 256 ? 2 : 4, kTile = 32, kStage = 2 * kTile * 2 * D, kGrain = kTile * kWaves;
+};
+
+template <class H, int D, Mode MODE>
+__global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArgs a) {
+  constexpr int W = Few<D>::kWaves, KT = Few<D>::kTile, STAGE = Few<D>::kStage, ROWB = 2 * D;
+  constexpr int COPIES = KT * ROWB / 1024, CHUNKS = D / 8, RPC = 64 / CHUNKS;  // copies of a tile, rows of a copy
+  constexpr int MERGE = W * kFewRows * (D + 2) * 4;
+  constexpr int LDS = W * 2 * STAGE > MERGE ? W * 2 * STAGE : MERGE;
+  // one array: with two, the compiler's wait for copies into the one before
+  // reads of the other would empty the ring at every tile
+  __shared__ __align__(1024) uint8_t lds[LDS + sizeof(NonFinite<D>)];
+  NonFinite<D>& bad = *reinterpret_cast<NonFinite<D>*>(lds + LDS);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  init_non_finite(&bad, 64 * W);
+  const int head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
+  Job found;
+  if (!find_job<MODE, kFewRows, KT, Few<D>::kGrain>(a, unit, head, &found)) return;
+  const Job j = uniform(found);
+  constexpr bool PREFIX = MODE == kPrefix;
+  const Keys run = PREFIX ? j.prefix : j.own;
+  const int group = a.group, li = lane & 15, quarter = lane >> 4;
+
+  // Q as the B operand: row li, channels 32 ks + 8 quarter ..
+  const int row = min(li, j.rows - 1);
+  const uint32_t qrow = (uint32_t)(j.row0 + row), qtoken = qrow / (uint32_t)group, qg = qrow % (uint32_t)group;
+  const uint16_t* qp = a.q + (j.token0 + (int64_t)qtoken) * a.q_ts + (int64_t)(head * group + (int)qg) * a.q_hs + quarter * 8;
+  i32x4 q[D / 32];
+#pragma unroll
+  for (int ks = 0; ks < D / 32; ++ks) q[ks] = *reinterpret_cast<const i32x4*>(qp + ks * 32);
+  const int sees = PREFIX ? run.last : min(j.own_base + (int)qtoken, run.last);
+  // below this key every row of the tile sees all
+  const int all_see = PREFIX ? run.last : min(j.own_base + (int)((uint32_t)j.row0 / (uint32_t)group), run.last);
+
+  uint8_t* ring = lds + wave * 2 * STAGE;
+  const int64_t page_bytes = ((int64_t)a.kv_heads * ROWB) << a.page_shift, head_off = ((int64_t)head * ROWB) << a.page_shift;
+  const Copier<D> copy_k{reinterpret_cast<const uint8_t*>(a.k_pages) + head_off, page_bytes, a.page_shift, a.pages};
+  const Copier<D> copy_v{reinterpret_cast<const uint8_t*>(a.v_pages) + head_off, page_bytes, a.page_shift, a.pages};
+  const int copy_row = lane / CHUNKS;
+  const int n_tiles = (j.tiles - wave + W - 1) / W;  // this wave's: wave, wave + W, ..
+  const auto issue = [&](int t) {
+    const int key0 = run.first + (t * W + wave) * KT;
+    uint8_t* dst = ring + (t & 1) * STAGE;
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i)
+      copy_k(run, key0, i * RPC, dst + i * 1024, copy_chunk(lane, CHUNKS, k_swizzle<D>(i * RPC + copy_row)), copy_row);
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i)
+      copy_v(run, key0, i * RPC, dst + KT * ROWB + i * 1024, copy_chunk(lane, CHUNKS, v_swizzle<D>(i * RPC + copy_row)), copy_row);
+  };
+
+  f32x4 o[D / 16];
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float ref = -__builtin_inff(), sum = 0.0f;
+  lds_barrier();  // `bad` is set up
+  if (n_tiles > 0) issue(0);
+  for (int t = 0; t < n_tiles; ++t) {
+    const int key0 = run.first + (t * W + wave) * KT;
+    const uint8_t* kt = ring + (t & 1) * STAGE;
+    uint8_t* vt = ring + (t & 1) * STAGE + KT * ROWB;
+    if (t + 1 < n_tiles) {
+      issue(t + 1);
+      wait_vmem_below<3 * COPIES>();
+    } else {
+      wait_vmem_below<COPIES>();
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 s[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int r = h * 16 + li;
+#pragma unroll
+      for (int ks = 0; ks < D / 32; ++ks)
+        s[h] = H::mfma16(lds_read16(kt + r * ROWB + (((ks * 4 + quarter) ^ k_swizzle<D>(r)) * 16)), q[ks], s[h]);
+    }
+    const bool masked = key0 + KT - 1 > all_see;
+    if (masked) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (key0 + h * 16 + quarter * 4 + e > sees) s[h][e] = -__builtin_inff();
+    }
+    float top = fmaxf(fmaxf(fmaxf(s[0].x, s[0].y), fmaxf(s[0].z, s[0].w)), fmaxf(fmaxf(s[1].x, s[1].y), fmaxf(s[1].z, s[1].w)));
+    if (__any(top * a.scale_log2 > ref + kRescaleAt)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float next = top * a.scale_log2 > ref + kRescaleAt ? top * a.scale_log2 : ref;
+      const float f = ref == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - next);
+      sum *= f;
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt) o[dt] *= f;
+      ref = next;
+    }
+    const float sub = ref == -__builtin_inff() ? 0.0f : ref - H::kShift;
+    uint32_t p[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[h][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][e], a.scale_log2, -sub));
+        sum += s[h][e];
+      }
+      p[2 * h] = H::pack(s[h].x, s[h].y);
+      p[2 * h + 1] = H::pack(s[h].z, s[h].w);
+    }
+    asm volatile("" : "+v"(sum));  // added up here, not after the weights' last use
+    const i32x4 pb{(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
+    if (t + 1 < n_tiles) wait_vmem_below<2 * COPIES>();
+    else wait_vmem_below<0>();
+    __builtin_amdgcn_sched_barrier(0);
+    if (masked && holds_non_finite<H, COPIES>(vt + lane * 16)) {
+      take_non_finite<H, D, COPIES>(vt, lane, PREFIX ? kAlways : key0, run.last - key0 + 1, &bad);
+      if (lane == 0) bad.tile = 1;
+    }
+    // V^T: channels 16 dt + li, keys 4 quarter + 0..3 and 16 + those; a chunk's
+    // swizzle changes its lower four bits only, so dt + 8 lies 256 bytes on
+    constexpr int AHEAD = D == 64 ? 4 : 8;
+    uint32_t at[AHEAD];
+    {
+      const int r = quarter * 4 + (li >> 2);
+      const uint32_t base = lds_address(vt) + r * ROWB + (li & 1) * 8;
+#pragma unroll
+      for (int dt = 0; dt < AHEAD; ++dt) at[dt] = base + (((dt * 2 + ((li >> 1) & 1)) ^ v_swizzle<D>(r)) * 16);
+    }
+    i32x4 v[D / 16];
+#pragma unroll
+    for (int dt = 0; dt < AHEAD; dt += 4) lds_read_tr4<0, 16 * ROWB>(at[dt], at[dt + 1], at[dt + 2], at[dt + 3], v + dt);
+    if constexpr (D == 256) {
+#pragma unroll
+      for (int dt = 0; dt < AHEAD; dt += 4) lds_read_tr4<256, 16 * ROWB>(at[dt], at[dt + 1], at[dt + 2], at[dt + 3], v + 8 + dt);
+    }
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) o[dt] = H::mfma16(v[dt], pb, o[dt]);
+  }
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+
+  // The waves' results, in wave order: [wave][row][D + 2] floats over the rings.
+  __syncthreads();
+  float* m = reinterpret_cast<float*>(lds);
+  {
+    float* mine = m + (wave * kFewRows + li) * (D + 2);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine[dt * 16 + quarter * 4 + e] = o[dt][e];
+    if (quarter == 0) mine[D] = ref, mine[D + 1] = sum;
+  }
+  __syncthreads();
+  float* part_o = (PREFIX ? a.prefix_o : a.part_o) + j.part * (kFewRows * D);
+  float2* part_ml = (PREFIX ? a.prefix_ml : a.part_ml) + j.part * kFewRows;
+  for (int i = threadIdx.x; i < j.rows * (D / 4); i += 64 * W) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    float top = -__builtin_inff(), f[W], total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = fmaxf(top, m[(w * kFewRows + r) * (D + 2) + D]);
+    f32x4 out{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float* from = m + (w * kFewRows + r) * (D + 2);
+      f[w] = from[D] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(from[D] - top);
+      total += f[w] * from[D + 1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] += f[w] * from[d + e];
+    }
+    const uint32_t rr = (uint32_t)(j.row0 + r), tk = rr / (uint32_t)group, g = rr % (uint32_t)group;
+    if (bad.tile) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = with_non_finite(out[e], bad, d + e, PREFIX ? 0 : j.own_base + (int)tk);
+    }
+    if (j.whole) {
+      const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+      store4<H>(a.out + ((j.token0 + (int64_t)tk) * a.q_heads + head * group + (int)g) * D + d, out * inv);
+    } else {
+      *reinterpret_cast<f32x4*>(part_o + r * D + d) = out;
+      if (d == 0) part_ml[r] = float2{top, total};
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: tiles of 128, four waves of 32 rows that share the key tiles.
+// MFMA-bound for long prompts. 32x32x16 MFMA; a lane holds row lane % 32 and
+// keys 8 i + 4 (lane / 32) + 0..3. Two stages: while a tile is multiplied the
+// next one's copies are in flight; one barrier a tile.
+// ---------------------------------------------------------------------------
+template <int D>
+struct Many {
+  static constexpr int kTile = D == 256 ? 32 : 64, kGrain = 64;
+  static constexpr int kPerCu = D == 256 ? 1 : 2;  // workgroups of a CU: 512 or 256 registers a lane
+};
+
+template <class H, int D, Mode MODE>
+__global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnArgs a) {
+  constexpr int KT = Many<D>::kTile, SUB = KT / 32, ROWB = 2 * D, STAGE = 2 * KT * ROWB;
+  constexpr int CHUNKS = D / 8, RPC = 64 / CHUNKS, COPIES = KT * ROWB / 1024 / 4;  // copies of a wave, of K and of V
+  __shared__ __align__(1024) uint8_t lds[2 * STAGE + sizeof(NonFinite<D>)];  // one array, as above
+  NonFinite<D>& bad = *reinterpret_cast<NonFinite<D>*>(lds + 2 * STAGE);
+  init_non_finite(&bad, 256);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = blockIdx.x % a.kv_heads;
+  // whole rows of keys at once: the last tiles, which see the most, come first
+  const int unit = MODE == kWhole ? a.p.own_units - 1 - (int)(blockIdx.x / a.kv_heads) : (int)(blockIdx.x / a.kv_heads);
+  const int group = a.group, li = lane & 31, half = lane >> 5;
+  if (MODE == kWhole && unit == 0) {
+    // tokens that belong to no sequence come out as 0
+    for (int t = a.starts ? clamped(read_only(a.starts, a.batch), 0, a.tokens) : a.tokens; t < a.tokens; ++t)
+      for (int i = threadIdx.x; i < group * D; i += 256) a.out[((int64_t)t * a.q_heads + head * group) * D + i] = 0;
+  }
+  Job found;
+  if (!find_job<MODE, kManyRows, KT, Many<D>::kGrain>(a, unit, head, &found)) return;
+  const Job j = uniform(found);
+
+  const int row = min(wave * 32 + li, j.rows - 1);
+  const uint32_t qrow = (uint32_t)(j.row0 + row), qtoken = qrow / (uint32_t)group, qg = qrow % (uint32_t)group;
+  const uint16_t* qp = a.q + (j.token0 + (int64_t)qtoken) * a.q_ts + (int64_t)(head * group + (int)qg) * a.q_hs + half * 8;
+  i32x4 q[D / 16];
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) q[ks] = *reinterpret_cast<const i32x4*>(qp + ks * 16);
+  const int sees = j.own_base + (int)qtoken;
+  // own keys that every row of the wave sees, and every row of the workgroup
+  const int all_see = j.own_base + (int)((uint32_t)(j.row0 + min(wave * 32, j.rows - 1)) / (uint32_t)group);
+  const int wg_sees = j.own_base + (int)((uint32_t)j.row0 / (uint32_t)group);
+
+  const int64_t page_bytes = ((int64_t)a.kv_heads * ROWB) << a.page_shift, head_off = ((int64_t)head * ROWB) << a.page_shift;
+  const Copier<D> copy_k{reinterpret_cast<const uint8_t*>(a.k_pages) + head_off, page_bytes, a.page_shift, a.pages};
+  const Copier<D> copy_v{reinterpret_cast<const uint8_t*>(a.v_pages) + head_off, page_bytes, a.page_shift, a.pages};
+  const int copy_row = lane / CHUNKS;
+  const auto issue = [&](int t) {
+    const bool first = MODE == kPrefix || (MODE == kWhole && t < j.tiles0);
+    const Keys run{first ? j.prefix.ids : j.own.ids, first ? j.prefix.first : j.own.first, first ? j.prefix.last : j.own.last};
+    const int key0 = run.first + (first ? t : t - j.tiles0) * KT;
+    uint8_t* dst = lds + (t & 1) * STAGE;
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      const int r = (wave * COPIES + i) * RPC;
+      copy_k(run, key0, r, dst + r * ROWB, copy_chunk(lane, CHUNKS, k_swizzle<D>(r + copy_row)), copy_row);
+      copy_v(run, key0, r, dst + (KT + r) * ROWB, copy_chunk(lane, CHUNKS, v_swizzle<D>(r + copy_row)), copy_row);
+    }
+  };
+
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+  float ref = -__builtin_inff(), sum = 0.0f;
+  if (j.tiles > 0) issue(0);
+  if (j.tiles > 1) issue(1);
+  if (j.tiles > 1) wait_vmem_below<2 * COPIES>();
+  else wait_vmem_below<0>();
+  lds_barrier();
+  for (int t = 0; t < j.tiles; ++t) {
+    // Tile t is in LDS. The copies of tile t + 1 are in flight until the reads
+    // of V (before which the compiler waits for them), and those of t + 2
+    // start when every wave has read tile t.
+    const bool first = MODE == kPrefix || (MODE == kWhole && t < j.tiles0);
+    const int key0 = first ? j.prefix.first + t * KT : j.own.first + (t - j.tiles0) * KT;
+    const int last = first ? j.prefix.last : j.own.last;
+    const int row_last = first ? last : min(sees, last);
+    const uint8_t* kt = lds + (t & 1) * STAGE;
+    uint8_t* vt = lds + (t & 1) * STAGE + KT * ROWB;
+    f32x16 s[SUB];
+#pragma unroll
+    for (int b = 0; b < SUB; ++b) {
+      const int r = b * 32 + li;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks)
+        s[b] = H::mfma32(lds_read16(kt + r * ROWB + (((ks * 2 + half) ^ k_swizzle<D>(r)) * 16)), q[ks], s[b]);
+    }
+    const bool masked = key0 + KT - 1 > (first ? last : min(all_see, last));
+    if (masked) {
+#pragma unroll
+      for (int b = 0; b < SUB; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (key0 + b * 32 + (e >> 2) * 8 + half * 4 + (e & 3) > row_last) s[b][e] = -__builtin_inff();
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < SUB; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[b][e]);
+    if (__any(top * a.scale_log2 > ref + kRescaleAt)) {
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float next = top * a.scale_log2 > ref + kRescaleAt ? top * a.scale_log2 : ref;
+      const float f = ref == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - next);
+      sum *= f;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) o[dt] *= f;
+      ref = next;
+    }
+    const float sub = ref == -__builtin_inff() ? 0.0f : ref - H::kShift;
+    i32x4 p[2 * SUB];
+#pragma unroll
+    for (int b = 0; b < SUB; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], a.scale_log2, -sub));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e + 1], a.scale_log2, -sub));
+        sum += x + y;
+        p[2 * b + (e >> 3)][(e & 7) >> 1] = (int)H::pack(x, y);
+      }
+    asm volatile("" : "+v"(sum));  // added up here, not after the weights' last use
+    if (key0 + KT - 1 > (first ? last : min(wg_sees, last))) {
+      // masked for some wave: each looks through the quarter that it copied
+      if (holds_non_finite<H, COPIES>(vt + wave * COPIES * 1024 + lane * 16) && lane == 0) bad.tile = t + 1;
+      lds_barrier();
+      if (bad.tile == t + 1) {
+        take_non_finite<H, D, COPIES>(vt, wave * COPIES * 64 + lane, first ? kAlways : key0, last - key0 + 1, &bad);
+        lds_barrier();
+      }
+    }
+    // V^T: channels 32 dt + li, keys 16 ks + 4 half + 0..3 and 8 more
+    const auto v_frag = [&](int dt, int ks) {
+      const int r = ks * 16 + half * 4 + ((li & 15) >> 2), c = dt * 4 + (li >> 4) * 2 + ((li >> 1) & 1), off = (li & 1) * 8;
+      return cat_tr(lds_read_tr(vt + r * ROWB + ((c ^ v_swizzle<D>(r)) * 16) + off),
+                    lds_read_tr(vt + (r + 8) * ROWB + ((c ^ v_swizzle<D>(r + 8)) * 16) + off));
+    };
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int ks = 0; ks < 2 * SUB; ++ks) o[dt] = H::mfma32(v_frag(dt, ks), p[ks], o[dt]);
+    wait_vmem_below<0>();
+    lds_barrier();
+    if (t + 2 < j.tiles) issue(t + 2);
+  }
+  sum += __shfl_xor(sum, 32);
+  if (wave * 32 + li >= j.rows) return;
+  if (j.tiles > 0 && bad.tile) {
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        o[dt][e] = with_non_finite(o[dt][e], bad, dt * 32 + (e >> 2) * 8 + half * 4 + (e & 3), MODE == kPrefix ? 0 : sees);
+  }
+  if (j.whole) {
+    uint16_t* to = a.out + ((j.token0 + (int64_t)qtoken) * a.q_heads + head * group + (int)qg) * D + half * 4;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        store4<H>(to + dt * 32 + e * 2, f32x4{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]} * inv);
+  } else {
+    float* to = (MODE == kPrefix ? a.prefix_o : a.part_o) + (j.part * kManyRows + row) * D + half * 4;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<f32x4*>(to + dt * 32 + e * 2) = f32x4{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]};
+    if (half == 0) (MODE == kPrefix ? a.prefix_ml : a.part_ml)[j.part * kManyRows + row] = float2{ref, sum};
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Joins a row's partial results, its prefix chunks and its own, in that order:
+// one wave a (token, head).
+// ---------------------------------------------------------------------------
+template <class H, int D>
+__global__ __launch_bounds__(256) void combine_kernel(AttnArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (id >= (int64_t)a.tokens * a.q_heads) return;
+  const int token = (int)((uint32_t)id / (uint32_t)a.q_heads), qh = (int)((uint32_t)id % (uint32_t)a.q_heads);
+  const int head = (int)((uint32_t)qh / (uint32_t)a.group), g = qh - head * a.group;
+
+  // own partials
+  const int rows = a.p.few_own ? kFewRows : kManyRows;
+  int b = token, count = 0;
+  if (a.starts) {
+    for (int base = 0; base < a.batch; base += 64) {
+      const int c = __popcll(__ballot(base + lane < a.batch && start_of(a, min(base + lane, a.batch - 1)) <= token));
+      count += c;
+      if (c < 64) break;
+    }
+    b = count - 1;
+  }
+  bool mine = b >= 0;
+  int n_own = 0, first = 0, own_row = 0;
+  if (mine) {
+    // the last sequence that starts at or before the token: those after it hold no token
+    const Sequence s = sequence(a, uniform(b));
+    const int r = uniform((token - s.start) * a.group + g);
+    mine = r < s.n * a.group;
+    if (mine) {
+      const int keys = a.info[0];
+      n_own = (int)((uint32_t)(s.len + keys - 1) / (uint32_t)keys);
+      if (n_own) first = a.info[1 + b] + (int)((uint32_t)r / (uint32_t)rows) * n_own;
+      own_row = (int)((uint32_t)r % (uint32_t)rows);
+    }
+  }
+  const int n_pre = mine && a.prefix_len ? a.p.prefix_splits : 0;
+  if (mine && n_pre == 0 && n_own == 1) return;  // written already
+  const int prows = a.p.few_prefix ? kFewRows : kManyRows, prow = token * a.group + g;
+  const int64_t pre_unit = (int64_t)(prow / prows) * a.p.prefix_splits;
+  const auto part_of = [&](int i) -> int64_t {
+    const int64_t u = i < n_pre ? pre_unit + i : first + i - n_pre;
+    return (u * a.kv_heads + head) * (i < n_pre ? prows : rows) + (i < n_pre ? prow % prows : own_row);
+  };
+  const auto o_of = [&](int i) { return (i < n_pre ? a.prefix_o : a.part_o) + part_of(i) * D; };
+  const auto ml_of = [&](int i) { return (i < n_pre ? a.prefix_ml : a.part_ml)[part_of(i)]; };
+  // 64 parts a step, their references and sums one a lane; the running result
+  // is scaled when a step's largest reference exceeds those before it.
+  constexpr int PER = D / 64, AHEAD = 8;
+  const int n = n_pre + n_own;
+  float o[PER], total = 0.0f, top = -__builtin_inff();
+#pragma unroll
+  for (int e = 0; e < PER; ++e) o[e] = 0.0f;
+  for (int base = 0; base < n; base += 64) {
+    const int parts = min(64, n - base);
+    const float2 ml = ml_of(base + min(lane, parts - 1));
+    const float mine = lane < parts ? ml.x : -__builtin_inff();
+    float next = fmaxf(top, mine);
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) next = fmaxf(next, __shfl_xor(next, s));
+    const float f = mine == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mine - next);
+    const float scale = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top - next);
+    top = next;
+    total = total * scale + wave_sum_f32(f == 0.0f ? 0.0f : f * ml.y);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] = scale == 0.0f ? 0.0f : o[e] * scale;
+    for (int i = 0; i < parts; i += AHEAD) {
+      float x[AHEAD][PER];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const float* from = o_of(base + min(i + u, parts - 1)) + lane * PER;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x[u][e] = from[e];
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const float w = i + u < parts ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), min(i + u, parts - 1))) : 0.0f;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) o[e] = w == 0.0f ? o[e] : __builtin_fmaf(w, x[u][e], o[e]);
+      }
+    }
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  uint16_t* to = a.out + id * D + lane * PER;
+  if constexpr (PER == 1) {
+    to[0] = (uint16_t)H::pack(o[0] * inv, 0.0f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < PER; e += 2) reinterpret_cast<uint32_t*>(to)[e / 2] = H::pack(o[e] * inv, o[e + 1] * inv);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The plan and the launches.
+// ---------------------------------------------------------------------------
+AttnPlan attention_plan(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t prefix_len, bool ragged,
+                        int cus) {
+  AttnPlan p{};
+  const int64_t group = q_heads / kv_heads, all_rows = tokens * group;
+  p.few_own = all_rows <= batch * kFewRows;
+  p.few_prefix = all_rows <= kFewRows;
+  const int64_t rows = p.few_own ? kFewRows : kManyRows;
+  const int64_t tiles = !ragged && group <= rows ? batch : all_rows / rows + batch;
+  p.own_units = (int)tiles;
+  p.split = p.few_own || tiles * kv_heads < 2 * cus;
+  if (!p.split) return p;
+  const int64_t want = std::max<int64_t>(1, 2 * cus / kv_heads);
+  p.own_target = (int)want;
+  p.own_units = (int)(want + tiles);
+  if (prefix_len > 0) {
+    const int64_t prows = p.few_prefix ? kFewRows : kManyRows;
+    p.prefix_tiles = (int)((all_rows + prows - 1) / prows);
+    p.prefix_splits = (int)std::max<int64_t>(1, std::min<int64_t>((want + p.prefix_tiles - 1) / p.prefix_tiles, (prefix_len + 255) / 256));
+  }
+  return p;
+}
+
+static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
+
+int64_t attention_workspace(const AttnPlan& p, int64_t batch, int64_t kv_heads, int64_t dim) {
+  if (!p.split) return 0;
+  const int64_t own = (int64_t)p.own_units * kv_heads * (p.few_own ? kFewRows : kManyRows);
+  const int64_t pre = (int64_t)p.prefix_tiles * p.prefix_splits * kv_heads * (p.few_prefix ? kFewRows : kManyRows);
+  return up256(own * dim * 4) + up256(own * 8) + up256(pre * dim * 4) + up256(pre * 8) + up256(4 * (batch + 1));
+}
+
+template <class H, int D>
+static void launch_attention(const AttnArgs& a, hipStream_t stream) {
+  const AttnPlan& p = a.p;
+  if (p.split && a.prefix_len) {
+    const unsigned grid = (unsigned)(p.prefix_tiles * p.prefix_splits * a.kv_heads);
+    if (p.few_prefix) attend_few_kernel<H, D, kPrefix><<<grid, 64 * Few<D>::kWaves, 0, stream>>>(a);
+    else attend_many_kernel<H, D, kPrefix><<<grid, 256, 0, stream>>>(a);
+  }
+  const unsigned grid = (unsigned)(p.own_units * a.kv_heads);
+  if (p.few_own) attend_few_kernel<H, D, kOwn><<<grid, 64 * Few<D>::kWaves, 0, stream>>>(a);
+  else if (p.split) attend_many_kernel<H, D, kOwn><<<grid, 256, 0, stream>>>(a);
+  else attend_many_kernel<H, D, kWhole><<<grid, 256, 0, stream>>>(a);
+  if (p.split) combine_kernel<H, D><<<(unsigned)(((int64_t)a.tokens * a.q_heads + 3) / 4), 256, 0, stream>>>(a);
+}
+
+hipError_t paged_attention(AttnArgs a, int dim, bool fp16, void* workspace, hipStream_t stream) {
+  if (a.p.split) {
+    const int64_t own = (int64_t)a.p.own_units * a.kv_heads * (a.p.few_own ? kFewRows : kManyRows);
+    const int64_t pre = (int64_t)a.p.prefix_tiles * a.p.prefix_splits * a.kv_heads * (a.p.few_prefix ? kFewRows : kManyRows);
+    uint8_t* w = (uint8_t*)workspace;
+    a.part_o = (float*)w, w += up256(own * dim * 4);
+    a.part_ml = (float2*)w, w += up256(own * 8);
+    a.prefix_o = (float*)w, w += up256(pre * dim * 4);
+    a.prefix_ml = (float2*)w, w += up256(pre * 8);
+    a.info = (int32_t*)w;
+  }
+  if (dim == 64) fp16 ? launch_attention<Fp16, 64>(a, stream) : launch_attention<Bf16, 64>(a, stream);
+  else if (dim == 128) fp16 ? launch_attention<Fp16, 128>(a, stream) : launch_attention<Bf16, 128>(a, stream);
+  else if (dim == 256) fp16 ? launch_attention<Fp16, 256>(a, stream) : launch_attention<Bf16, 256>(a, stream);
+  else return hipErrorInvalidValue;
+  return hipGetLastError();
+}
+
+}  // namespace jv

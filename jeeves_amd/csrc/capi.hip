@@ -9,10 +9,11 @@
 
 #include "../../include/jeeves_fp8.h"
 #include "kernels.h"
+#include "status.h"
 
-namespace {
+namespace jv {
 
-thread_local char g_last_error[512] = "";
+static thread_local char g_last_error[512] = "";
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -28,7 +29,7 @@ int hip_status(hipError_t e, const char* what) {
 }
 
 constexpr int kMaxDevices = 64;
-std::atomic<int> g_cu_count[kMaxDevices];
+static std::atomic<int> g_cu_count[kMaxDevices];
 
 int cu_count_of(int device) {
   if (device < 0 && hipGetDevice(&device) != hipSuccess) return -1;
@@ -40,6 +41,15 @@ int cu_count_of(int device) {
   g_cu_count[device].store(n, std::memory_order_relaxed);
   return n;
 }
+
+}  // namespace jv
+
+namespace {
+
+using jv::cu_count_of;
+using jv::fail;
+using jv::hip_status;
+using jv::kMaxDevices;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -242,7 +252,7 @@ int scratch_of_current_device(uint8_t** out) {
 
 extern "C" {
 
-const char* jv_fp8_last_error(void) { return g_last_error; }
+const char* jv_fp8_last_error(void) { return jv::g_last_error; }
 
 int jv_device_cu_count(int device) { return cu_count_of(device); }
 
