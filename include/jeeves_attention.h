@@ -54,6 +54,8 @@ int jv_append_kv(const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64
                  int64_t q_hs, const float* q_weight, void* q_out, int64_t q_heads, int64_t tokens, int64_t kv_heads,
                  int64_t dim, int fp16, void* stream);
 
+#define JV_ATTENTION_COUNTERS 65536
+
 /* Bytes of workspace jv_paged_attention needs for these sizes on the current
  * device (0: none); -1 if it cannot be queried or the sizes are refused. */
 int64_t jv_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
@@ -71,14 +73,17 @@ int64_t jv_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_
  * 0 where a token sees no key or belongs to no sequence. Keys that a token
  * does not see have no effect, whatever their values. Lengths are taken up to
  * the table's width, page ids into the cache's range.
- * workspace: 256-byte aligned. The role of _decode_attention_split and
+ * workspace: 256-byte aligned. counters: int32, JV_ATTENTION_COUNTERS of them
+ * serve every call; zero before the first call and left at zero by each, one
+ * set for each stream whose calls can overlap. The role of _decode_attention_split and
  * _decode_attention_combine (model/triton_kernels.py:118-171).
  */
 int jv_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k_pages, const void* v_pages, int64_t pages,
                        int64_t page_size, const int32_t* table, int64_t table_stride, int64_t table_cols,
                        const int32_t* lengths, const int32_t* starts, int64_t batch, const int32_t* prefix_pages,
                        int64_t prefix_len, float scale, void* out, int64_t tokens, int64_t q_heads, int64_t kv_heads,
-                       int64_t dim, int fp16, void* workspace, int64_t workspace_bytes, void* stream);
+                       int64_t dim, int fp16, void* workspace, int64_t workspace_bytes, int32_t* counters,
+                       int64_t n_counters, void* stream);
 
 #ifdef __cplusplus
 }

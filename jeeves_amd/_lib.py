@@ -60,7 +60,7 @@ SIGNATURES: dict[str, tuple] = {
     "jv_paged_attention_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int]),
     "jv_paged_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                    c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_float, c_void_p, c_int64, c_int64, c_int64,
-                                   c_int64, c_int, c_void_p, c_int64, c_void_p]),
+                                   c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
 }
 
 _lib = None

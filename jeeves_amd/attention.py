@@ -26,7 +26,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .fp8 import FP8Linear, _device_guard, _stream
+from .fp8 import _CURRENT, TILE_COUNTER_SLOTS, FP8Linear, _stream_counters
 
 HEAD_DIMS = (64, 128, 256)
 _FP16 = {torch.bfloat16: 0, torch.float16: 1}
@@ -54,6 +54,13 @@ class PagedKVCache:
             raise ValueError("the cache's pages must be contiguous and 16-byte aligned")
         self.k, self.v = k, v
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        self._goes_with = (k.dtype, k.get_device(), self.head_dim)
+
+    def check(self, dtype: torch.dtype, index: int, dim: int) -> None:
+        """Refuses heads of another type, device (its index) or size than the cache's."""
+        if (dtype, index, dim) != self._goes_with:
+            raise ValueError(f"heads of {dim} channels of {dtype} on HIP device {index} do not go with a cache of "
+                             f"{tuple(self.k.shape)} {self.k.dtype} on {self.k.device}")
 
     @classmethod
     def allocate(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
@@ -73,53 +80,68 @@ def rope_table(positions: int, rotary: int, base: float = 10000.0, device: torch
     return torch.cat([angle.cos(), angle.sin()], 1).float().to(device)
 
 
-def _heads(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> torch.Tensor:
-    """``t`` as [tokens, heads, head_dim] with 16-byte aligned rows."""
-    if t.dim() != 3 or t.dtype not in _FP16 or t.shape[2] not in HEAD_DIMS:
-        raise ValueError(f"{name} must be bfloat16 or float16 [tokens, heads, head_dim] with a head size of {HEAD_DIMS}, got "
-                         f"{tuple(t.shape)} {t.dtype}")
-    if like is not None and (t.dtype != like.dtype or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2]
-                             or t.device != like.device):
-        raise ValueError(f"{name} {tuple(t.shape)} {t.dtype} on {t.device} does not go with {tuple(like.shape)} {like.dtype} on "
-                         f"{like.device}")
-    if not t.is_cuda:
-        raise ValueError(f"the attention kernels run on a HIP device; {name} is on {t.device}")
+# The calls below are a few microseconds of work on small batches, so their
+# host path is kept short: sizes and devices are compared as they come from the
+# tensors, once, and formatted only where they are refused.
+def _refuse(name: str, t: torch.Tensor, wanted: str) -> None:
+    raise ValueError(f"{name} must be {wanted}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def _heads(name: str, t: torch.Tensor, dtype: torch.dtype, index: int, tokens: int, dim: int) -> tuple:
+    """``t`` [tokens, heads, dim] with 16-byte aligned rows: (the tensor, its
+    address, its token and head strides, its heads)."""
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or t.dtype is not dtype or t.get_device() != index:
+        _refuse(name, t, f"{dtype} [{tokens}, heads, {dim}] on HIP device {index}")
     ts, hs, unit = t.stride()
-    if unit != 1 or ts % 8 or hs % 8 or t.data_ptr() % 16:
+    ptr = t.data_ptr()
+    if unit != 1 or (ts | hs) & 7 or ptr & 15:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        (ts, hs, _), ptr = t.stride(), t.data_ptr()
+    return t, ptr, ts, hs, shape[1]
 
 
-def _indices(name: str, t: torch.Tensor, tokens: int, dev: torch.device) -> torch.Tensor:
-    if t.dtype not in _WIDE or t.shape != (tokens,) or t.device != dev:
-        raise ValueError(f"{name} must be int32 or int64 [{tokens}] on {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    return t if t.stride(0) == 1 or tokens < 2 else t.contiguous()
+def _first(name: str, t: torch.Tensor) -> tuple:
+    """(dtype, device index, tokens, head size) that the other operands go by."""
+    shape, dtype, index = t.shape, t.dtype, t.get_device()
+    if len(shape) != 3 or shape[2] not in HEAD_DIMS or dtype not in _FP16 or index < 0:
+        _refuse(name, t, f"bfloat16 or float16 [tokens, heads, head size of {HEAD_DIMS}] on a HIP device")
+    return dtype, index, shape[0], shape[2]
 
 
-def _rope_operands(rope: torch.Tensor | None, positions: torch.Tensor | None, tokens: int, dim: int, dev: torch.device):
+def _indices(name: str, t: torch.Tensor, tokens: int, index: int) -> torch.Tensor:
+    if t.dtype not in _WIDE or t.shape != (tokens,) or t.get_device() != index:
+        _refuse(name, t, f"int32 or int64 [{tokens}] on HIP device {index}")
+    return t if tokens < 2 or t.stride(0) == 1 else t.contiguous()
+
+
+_NO_ROPE = (None, None, 0, 0, None, None, 0)
+
+
+def _rope_operands(rope: torch.Tensor | None, positions: torch.Tensor | None, tokens: int, dim: int, index: int) -> tuple:
+    """(table, its address, positions and channels; positions, their address, whether wide); the tensors to hold."""
     if rope is None:
-        return None, 0, 0, None, 0
-    if rope.dtype != torch.float32 or rope.dim() != 2 or rope.device != dev or rope.shape[1] % 16 or not 0 < rope.shape[1] <= dim:
-        raise ValueError(f"rope must be float32 [positions, rotary] on {dev} with rotary a multiple of 16 up to {dim}, got "
-                         f"{tuple(rope.shape)} {rope.dtype} on {rope.device}")
+        return _NO_ROPE
+    shape = rope.shape
+    if rope.dtype is not torch.float32 or len(shape) != 2 or rope.get_device() != index or shape[1] & 15 or not 0 < shape[1] <= dim:
+        _refuse("rope", rope, f"float32 [positions, a multiple of 16 channels up to {dim}] on HIP device {index}")
     if positions is None:
         raise ValueError("the rotation needs the tokens' positions")
-    if not rope.is_contiguous() or rope.data_ptr() % 16:
+    if not rope.is_contiguous() or rope.data_ptr() & 15:
         rope = rope.clone(memory_format=torch.contiguous_format)
-    positions = _indices("positions", positions, tokens, dev)
-    return rope, rope.shape[0], rope.shape[1], positions, _WIDE[positions.dtype]
+    positions = _indices("positions", positions, tokens, index)
+    return rope, rope.data_ptr(), shape[0], shape[1], positions, positions.data_ptr(), _WIDE[positions.dtype]
 
 
-def _head_weight(name: str, w: torch.Tensor | None, dim: int, dev: torch.device) -> torch.Tensor | None:
-    if w is None:
-        return None
-    if w.shape != (dim,) or w.device != dev:
-        raise ValueError(f"{name} must be [{dim}] on {dev}, got {tuple(w.shape)} on {w.device}")
-    return w if w.dtype == torch.float32 and w.is_contiguous() else w.to(torch.float32).contiguous()
+def _head_weight(name: str, w: torch.Tensor, dim: int, index: int) -> torch.Tensor:
+    if w.shape != (dim,) or w.get_device() != index:
+        _refuse(name, w, f"[{dim}] on HIP device {index}")
+    return w if w.dtype is torch.float32 and w.is_contiguous() else w.to(torch.float32).contiguous()
 
 
-def _ptr(t: torch.Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
+def _on(index: int):
+    """``torch.cuda.device`` of a device index, which costs two switches even where it is current."""
+    return _CURRENT if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor | None, positions: torch.Tensor | None, *,
@@ -135,27 +157,24 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor | None, po
     The inputs may be views of a merged projection's output. A token whose
     position the table does not have comes out as NaN.
     """
-    q = _heads("q", q)
-    k = _heads("k", k, q)
-    tokens, q_heads, dim = q.shape
-    dev = q.device
-    rope, n_pos, rotary, positions, wide = _rope_operands(rope, positions, tokens, dim, dev)
-    q_weight, k_weight = _head_weight("q_weight", q_weight, dim, dev), _head_weight("k_weight", k_weight, dim, dev)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    k_out = torch.empty(k.shape, dtype=q.dtype, device=dev)
+    dtype, index, tokens, dim = _first("q", q)
+    q, q_ptr, q_ts, q_hs, q_heads = _heads("q", q, dtype, index, tokens, dim)
+    k, k_ptr, k_ts, k_hs, kv_heads = _heads("k", k, dtype, index, tokens, dim)
+    rope, rope_ptr, n_pos, rotary, positions, pos_ptr, wide = _rope_operands(rope, positions, tokens, dim, index)
+    if q_weight is not None:
+        q_weight = _head_weight("q_weight", q_weight, dim, index)
+    if k_weight is not None:
+        k_weight = _head_weight("k_weight", k_weight, dim, index)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     if tokens:
-        with _device_guard(dev):
-            _lib.check(_lib.lib().jv_norm_rope(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                                               _ptr(rope), n_pos, rotary, _ptr(positions), wide, _ptr(q_weight), _ptr(k_weight), eps,
-                                               q_out.data_ptr(), k_out.data_ptr(), tokens, q_heads, k.shape[1], dim,
-                                               _FP16[q.dtype], _stream(dev)))
+        with _on(index):
+            _lib.check(_lib.lib().jv_norm_rope(
+                q_ptr, q_ts, q_hs, k_ptr, k_ts, k_hs, rope_ptr, n_pos, rotary, pos_ptr, wide,
+                None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps,
+                q_out.data_ptr(), k_out.data_ptr(), tokens, q_heads, kv_heads, dim, _FP16[dtype],
+                torch._C._cuda_getCurrentRawStream(index)))
     return q_out, k_out
-
-
-def _check_cache(cache: PagedKVCache, t: torch.Tensor) -> None:
-    if t.device != cache.k.device or t.dtype != cache.k.dtype or t.shape[2] != cache.head_dim:
-        raise ValueError(f"{tuple(t.shape)} {t.dtype} on {t.device} does not go with a cache of {tuple(cache.k.shape)} {cache.k.dtype} "
-                         f"on {cache.k.device}")
 
 
 def append_kv(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, *, rope: torch.Tensor | None = None,
@@ -167,48 +186,48 @@ def append_kv(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, slots: torc
     (padding). Slots are meant to differ: of two tokens with one slot either's
     row may stay. With ``q`` the same launch norms and rotates the queries,
     which are returned as a new contiguous tensor."""
-    k = _heads("k", k)
-    v = _heads("v", v, k)
-    tokens, kv_heads, dim = k.shape
-    dev = k.device
-    _check_cache(cache, k)
-    if kv_heads != cache.kv_heads or v.shape[1] != kv_heads:
-        raise ValueError(f"the cache has {cache.kv_heads} heads, got {kv_heads} of k and {v.shape[1]} of v")
-    slots = _indices("slots", slots, tokens, dev)
-    rope, n_pos, rotary, positions, wide = _rope_operands(rope, positions, tokens, dim, dev)
-    k_weight, q_weight = _head_weight("k_weight", k_weight, dim, dev), _head_weight("q_weight", q_weight, dim, dev)
-    q_out, q_heads, q_ts, q_hs = None, 0, 0, 0
+    dtype, index, tokens, dim = _first("k", k)
+    cache.check(dtype, index, dim)
+    k, k_ptr, k_ts, k_hs, kv_heads = _heads("k", k, dtype, index, tokens, dim)
+    v, v_ptr, v_ts, v_hs, v_heads = _heads("v", v, dtype, index, tokens, dim)
+    if kv_heads != cache.kv_heads or v_heads != kv_heads:
+        raise ValueError(f"the cache has {cache.kv_heads} heads, got {kv_heads} of k and {v_heads} of v")
+    slots = _indices("slots", slots, tokens, index)
+    rope, rope_ptr, n_pos, rotary, positions, pos_ptr, wide = _rope_operands(rope, positions, tokens, dim, index)
+    if k_weight is not None:
+        k_weight = _head_weight("k_weight", k_weight, dim, index)
+    if q_weight is not None:
+        q_weight = _head_weight("q_weight", q_weight, dim, index)
+    q_out, q_ptr, q_ts, q_hs, q_heads = None, None, 0, 0, 0
     if q is not None:
-        q = _heads("q", q, k)
-        q_heads, (q_ts, q_hs, _) = q.shape[1], q.stride()
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        q, q_ptr, q_ts, q_hs, q_heads = _heads("q", q, dtype, index, tokens, dim)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if tokens:
-        with _device_guard(dev):
-            _lib.check(_lib.lib().jv_append_kv(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                                               slots.data_ptr(), _WIDE[slots.dtype], cache.k.data_ptr(), cache.v.data_ptr(),
-                                               cache.pages, cache.page_size, _ptr(rope), n_pos, rotary, _ptr(positions), wide,
-                                               _ptr(k_weight), eps, _ptr(q), q_ts, q_hs, _ptr(q_weight), _ptr(q_out), q_heads,
-                                               tokens, kv_heads, dim, _FP16[k.dtype], _stream(dev)))
+        with _on(index):
+            _lib.check(_lib.lib().jv_append_kv(
+                k_ptr, k_ts, k_hs, v_ptr, v_ts, v_hs, slots.data_ptr(), _WIDE[slots.dtype], cache.k.data_ptr(), cache.v.data_ptr(),
+                cache.pages, cache.page_size, rope_ptr, n_pos, rotary, pos_ptr, wide,
+                None if k_weight is None else k_weight.data_ptr(), eps, q_ptr, q_ts, q_hs,
+                None if q_weight is None else q_weight.data_ptr(), None if q is None else q_out.data_ptr(), q_heads, tokens,
+                kv_heads, dim, _FP16[dtype], torch._C._cuda_getCurrentRawStream(index)))
     return q_out
 
 
 @lru_cache(maxsize=4096)
-def _workspace(device: torch.device, tokens: int, batch: int, q_heads: int, kv_heads: int, dim: int, prefix: int,
-               ragged: bool) -> int:
-    """Workspace bytes for these sizes on ``device``, which is current."""
+def _workspace(index: int, tokens: int, batch: int, q_heads: int, kv_heads: int, dim: int, prefix: int, ragged: bool) -> int:
+    """Workspace bytes for these sizes on a device, which is current; 0: none, and no counters."""
     n = _lib.lib().jv_paged_attention_workspace_bytes(tokens, batch, q_heads, kv_heads, dim, prefix, ragged)
     if n < 0:
         raise ValueError(f"the attention does not take {tokens} tokens of {batch} sequences, {q_heads} and {kv_heads} heads")
     return n
 
 
-def _int32(name: str, t: torch.Tensor, dims: int, dev: torch.device) -> torch.Tensor:
-    if t.dim() != dims or t.device != dev or t.dtype not in _WIDE:
-        raise ValueError(f"{name} must be an int32 or int64 tensor of {dims} dimensions on {dev}, got {tuple(t.shape)} {t.dtype} on "
-                         f"{t.device}")
-    if t.dtype != torch.int32:
+def _int32(name: str, t: torch.Tensor, shape: tuple, index: int) -> torch.Tensor:
+    if t.dtype not in _WIDE or t.shape != shape or t.get_device() != index:
+        _refuse(name, t, f"int32 or int64 {list(shape)} on HIP device {index}")
+    if t.dtype is not torch.int32:
         t = t.to(torch.int32)
-    return t if t.stride(-1) == 1 or t.shape[-1] < 2 else t.contiguous()
+    return t if t.stride(-1) == 1 or shape[-1] < 2 else t.contiguous()
 
 
 def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, lengths: torch.Tensor, *,
@@ -220,54 +239,62 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     Sequence b of the batch owns the first ``lengths[b]`` keys of the pages
     ``page_table[b]`` ([batch, columns]); its queries are the tokens
     ``query_starts[b]`` to ``query_starts[b + 1] - 1`` ([batch + 1], not
-    decreasing from 0; None: one token each), the last of them at its last key: query i
-    of n sees the own keys up to ``lengths[b] - n + i``. With
+    decreasing from 0; None: one token each), the last of them at its last key:
+    query i of n sees the own keys up to ``lengths[b] - n + i``. With
     ``prefix_length`` all queries of the batch also see that many keys of
-    ``prefix_pages``, which come before all own ones; they are read once for
-    the batch, not once for each sequence.
+    ``prefix_pages``, which come before all own ones; where each sequence has
+    few queries they are read once for the batch, not once for each sequence.
     Query head h reads key head ``h // (q_heads / kv_heads)``; ``scale``
     defaults to ``head_dim ** -0.5``.
 
     A token that sees no key, or that belongs to no sequence, comes out as 0.
     Keys that a token does not see have no effect on it, even infinite or NaN
-    ones; nor has what the table holds past a sequence's length. The sums are
-    in 32 bits; the softmax's weights are rounded to the 16-bit type for the
-    product with the values.
+    ones; nor has what the table holds past a sequence's length, nor the other
+    sequences. The sums are in 32 bits; the softmax's weights are rounded to
+    the 16-bit type for the product with the values.
+
+    As a split-K GEMM of ``jeeves_amd.fp8`` does, a call whose keys are split
+    over workgroups counts them in on the stream's tile counters, so run one on
+    a stream before capturing a graph on it.
     """
-    q = _heads("q", q)
-    tokens, q_heads, dim = q.shape
-    dev = q.device
-    _check_cache(cache, q)
-    if q_heads % cache.kv_heads:
-        raise ValueError(f"{q_heads} query heads are no multiple of the cache's {cache.kv_heads}")
-    page_table = _int32("page_table", page_table, 2, dev)
-    lengths = _int32("lengths", lengths, 1, dev)
-    batch = lengths.shape[0]
-    if page_table.shape[0] != batch:
-        raise ValueError(f"page_table has {page_table.shape[0]} rows for {batch} lengths")
-    if query_starts is None:
-        if tokens != batch:
-            raise ValueError(f"without query_starts each of the {batch} sequences has one query, got {tokens}")
-    else:
-        query_starts = _int32("query_starts", query_starts, 1, dev)
-        if query_starts.shape[0] != batch + 1:
-            raise ValueError(f"query_starts must have {batch + 1} values, got {query_starts.shape[0]}")
-    if prefix_length < 0 or (prefix_length and prefix_pages is None):
-        raise ValueError(f"a prefix of {prefix_length} keys needs its pages")
+    dtype, index, tokens, dim = _first("q", q)
+    cache.check(dtype, index, dim)
+    q, q_ptr, q_ts, q_hs, q_heads = _heads("q", q, dtype, index, tokens, dim)
+    kv_heads = cache.kv_heads
+    if q_heads % kv_heads:
+        raise ValueError(f"{q_heads} query heads are no multiple of the cache's {kv_heads}")
+    if page_table.dim() != 2:
+        _refuse("page_table", page_table, "int32 or int64 [batch, columns]")
+    batch, columns = shape = page_table.shape
+    page_table = _int32("page_table", page_table, shape, index)
+    lengths = _int32("lengths", lengths, (batch,), index)
+    starts_ptr = prefix_ptr = None
+    if query_starts is not None:
+        query_starts = _int32("query_starts", query_starts, (batch + 1,), index)
+        starts_ptr = query_starts.data_ptr()
+    elif tokens != batch:
+        raise ValueError(f"without query_starts each of the {batch} sequences has one query, got {tokens}")
     if prefix_length:
-        prefix_pages = _int32("prefix_pages", prefix_pages, 1, dev)
+        if prefix_length < 0 or prefix_pages is None or prefix_pages.dim() != 1:
+            raise ValueError(f"a prefix of {prefix_length} keys needs its pages, int32 or int64 [n]")
+        prefix_pages = _int32("prefix_pages", prefix_pages, prefix_pages.shape, index)
         if prefix_pages.shape[0] * cache.page_size < prefix_length:
             raise ValueError(f"{prefix_pages.shape[0]} pages of {cache.page_size} do not hold a prefix of {prefix_length} keys")
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        prefix_ptr = prefix_pages.data_ptr()
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if tokens:
-        with _device_guard(dev):
-            ws_bytes = _workspace(dev, tokens, batch, q_heads, cache.kv_heads, dim, prefix_length, query_starts is not None)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        with _on(index):
+            ws_bytes = _workspace(index, tokens, batch, q_heads, kv_heads, dim, prefix_length, query_starts is not None)
+            ws_ptr, counters_ptr, n_counters = None, None, 0
+            if ws_bytes:
+                ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+                counters = _stream_counters(q.device)
+                ws_ptr, counters_ptr, n_counters = ws.data_ptr(), counters.data_ptr(), TILE_COUNTER_SLOTS
             _lib.check(_lib.lib().jv_paged_attention(
-                q.data_ptr(), q.stride(0), q.stride(1), cache.k.data_ptr(), cache.v.data_ptr(), cache.pages, cache.page_size,
-                page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lengths.data_ptr(), _ptr(query_starts), batch,
-                _ptr(prefix_pages) if prefix_length else None, prefix_length, dim ** -0.5 if scale is None else scale,
-                out.data_ptr(), tokens, q_heads, cache.kv_heads, dim, _FP16[q.dtype], _ptr(ws), ws_bytes, _stream(dev)))
+                q_ptr, q_ts, q_hs, cache.k.data_ptr(), cache.v.data_ptr(), cache.pages, cache.page_size, page_table.data_ptr(),
+                page_table.stride(0), columns, lengths.data_ptr(), starts_ptr, batch, prefix_ptr, prefix_length,
+                dim ** -0.5 if scale is None else scale, out.data_ptr(), tokens, q_heads, kv_heads, dim, _FP16[dtype], ws_ptr,
+                ws_bytes, counters_ptr, n_counters, torch._C._cuda_getCurrentRawStream(index)))
     return out
 
 

@@ -34,6 +34,9 @@ struct Bf16 {
   static __device__ __forceinline__ f32x4 mfma16(i32x4 a, i32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
+  static __device__ __forceinline__ f32x4 mfma16k16(s16x4 a, s16x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
+  }
 };
 
 struct Fp16 {
@@ -49,6 +52,10 @@ struct Fp16 {
   }
   static __device__ __forceinline__ f32x4 mfma16(i32x4 a, i32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mfma16k16(s16x4 a, s16x4 b, f32x4 c) {
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
   }
 };
 
@@ -85,12 +92,15 @@ hipError_t norm_rope(const RopeArgs& a, int dim, bool fp16, hipStream_t stream);
 // token and sequence counts alone while the starts stay on the device.
 constexpr int kFewRows = 16, kManyRows = 128;
 
+// Counters a call may use at most; what does not fit is split less.
+constexpr int64_t kAttnCounters = 65536;
+
 struct AttnPlan {
   bool few_own, few_prefix;  // tiles of kFewRows rows instead of kManyRows
-  bool split;                // keys of a tile go to several workgroups: partial results and a combining launch
+  bool split;                // the keys of a row tile may go to several workgroups
   int own_units;             // tile slots, or with a split the most units (tile, key chunk) that there can be
-  int own_target;            // units to cut the own keys into, before rounding
-  int prefix_tiles, prefix_splits;
+  int own_target;            // units to cut the keys into, before rounding
+  int prefix_tiles, prefix_splits;  // where the prefix is gone through apart, for all tokens' rows
 };
 
 struct AttnArgs {
@@ -107,18 +117,16 @@ struct AttnArgs {
   int tokens, batch, q_heads, kv_heads, group;
   float scale_log2;  // scale * log2(e)
   uint16_t* out;     // [tokens, q_heads, dim]
-  float* part_o;     // own units, then prefix units: [unit, kv_head, rows, dim]
-  float2* part_ml;   // the same without dim: (reference exponent, sum)
-  float* prefix_o;
-  float2* prefix_ml;
-  int32_t* info;  // [0]: keys of a chunk; [1 + sequence]: its first unit
+  float *part_o, *prefix_o;      // partial results: [unit, kv_head, rows, dim]
+  float2 *part_ml, *prefix_ml;   // their references and sums: [unit, kv_head, rows]
+  int32_t* counters;             // 0 before and after each call
   AttnPlan p;
 };
 
 // Chosen by the sizes that the host knows.
-AttnPlan attention_plan(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t prefix_len, bool ragged,
-                        int cus);
-int64_t attention_workspace(const AttnPlan& p, int64_t batch, int64_t kv_heads, int64_t dim);
+AttnPlan attention_plan(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t prefix_len,
+                        bool ragged, int cus);
+int64_t attention_workspace(const AttnPlan& p, int64_t kv_heads, int64_t dim);
 hipError_t paged_attention(AttnArgs a, int dim, bool fp16, void* workspace, hipStream_t stream);
 
 }  // namespace jv

@@ -46,36 +46,46 @@ __device__ __forceinline__ void wait_vmem_below() {
 
 __device__ __forceinline__ i32x4 lds_read16(const uint8_t* p) { return *reinterpret_cast<const i32x4*>(p); }
 
-// Four 16-bit values of one column: of the 4 x 16 block that 16 consecutive
-// lanes address (8 bytes a lane, four lanes a row), lane i gets column i.
-__device__ __forceinline__ s16x4 lds_read_tr(const uint8_t* p) {
-  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
+// Lane constants that feed many addresses go through this once a key tile, so
+// that the compiler computes the addresses there (an XOR each) and does not
+// keep all of them in registers over the loop.
+__device__ __forceinline__ uint32_t fresh(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 
-// The same for four addresses, each at OFF and at OFF + STEP bytes: the four
-// 8-value operands that the pairs make. As one block with its wait, because
+__device__ __forceinline__ i32x4 lds_read16(uint32_t at, uint32_t offset) {
+  typedef __attribute__((address_space(3))) const i32x4 lds_i32x4;
+  typedef __attribute__((address_space(3))) const uint8_t lds_u8;
+  return *(lds_i32x4*)((lds_u8*)(uintptr_t)at + offset);
+}
+
+// Four 16-bit values of one column: of the 4 x 16 block that 16 consecutive
+// lanes address (8 bytes a lane, four lanes a row), lane i gets column i.
+__device__ __forceinline__ s16x4 lds_read_tr(uint32_t at, uint32_t offset) {
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  typedef __attribute__((address_space(3))) uint8_t lds_u8;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((lds_u8*)(uintptr_t)at + offset));
+}
+
+// The same for four addresses plus OFF bytes, as one block with its wait:
 // before the builtin the compiler waits for every copy to LDS in flight, the
 // next tile's too; the block waits for the LDS reads alone.
-template <int OFF, int STEP>
-__device__ __forceinline__ void lds_read_tr4(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, i32x4* out) {
+template <int OFF>
+__device__ __forceinline__ void lds_read_tr4(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, s16x4* out) {
   typedef int i32x2 __attribute__((ext_vector_type(2)));
-  i32x2 x[8];
+  i32x2 x0, x1, x2, x3;
   asm volatile(
-      "ds_read_b64_tr_b16 %0, %8 offset:%c12\n"
-      "ds_read_b64_tr_b16 %1, %8 offset:%c13\n"
-      "ds_read_b64_tr_b16 %2, %9 offset:%c12\n"
-      "ds_read_b64_tr_b16 %3, %9 offset:%c13\n"
-      "ds_read_b64_tr_b16 %4, %10 offset:%c12\n"
-      "ds_read_b64_tr_b16 %5, %10 offset:%c13\n"
-      "ds_read_b64_tr_b16 %6, %11 offset:%c12\n"
-      "ds_read_b64_tr_b16 %7, %11 offset:%c13\n"
+      "ds_read_b64_tr_b16 %0, %4 offset:%c8\n"
+      "ds_read_b64_tr_b16 %1, %5 offset:%c8\n"
+      "ds_read_b64_tr_b16 %2, %6 offset:%c8\n"
+      "ds_read_b64_tr_b16 %3, %7 offset:%c8\n"
       "s_waitcnt lgkmcnt(0)"
-      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
-      : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(OFF), "n"(OFF + STEP)
+      : "=&v"(x0), "=&v"(x1), "=&v"(x2), "=&v"(x3)
+      : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(OFF)
       : "memory");
-#pragma unroll
-  for (int i = 0; i < 4; ++i) out[i] = i32x4{x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y};
+  out[0] = __builtin_bit_cast(s16x4, x0), out[1] = __builtin_bit_cast(s16x4, x1);
+  out[2] = __builtin_bit_cast(s16x4, x2), out[3] = __builtin_bit_cast(s16x4, x3);
 }
 
 // LDS byte address of a pointer into a __shared__ array.
@@ -88,6 +98,8 @@ __device__ __forceinline__ i32x4 cat_tr(s16x4 a, s16x4 b) {
   return __builtin_bit_cast(i32x4, s16x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w});
 }
 
+// Both are linear over XOR: swizzle(r | s) = swizzle(r) ^ swizzle(s) for rows
+// without common bits, and so are the addresses made from them.
 // A tile's rows are D / 8 chunks of 16 bytes; what XORs a row's chunk index.
 // LDS serves 256 bytes (64 banks) at a time. K is read 16 rows at one chunk:
 // the row within the rows that start at bank 0 separates them. V is read by
@@ -174,25 +186,28 @@ __device__ __forceinline__ float wave_sum_f32(float v) {
 
 // Where keys are split over workgroups: the (sequence, row tile, key chunk) of
 // a unit. The tiles' keys are added up (in groups of 16, which the host has
-// checked to fit 32 bits), the sum cut into about `own_target` chunks of
-// `keys` keys, and each tile of a sequence gets ceil(len / keys) units of equal
-// shares of what it sees. Computed by each wave for itself, 64 sequences a
-// step, from the lengths on the device.
+// checked to fit 32 bits), the sum cut into about `own_target` chunks, and each
+// tile of a sequence gets one unit for each chunk's worth of keys that its
+// sequence has begun, one at least, with equal shares of what it sees. `shared`:
+// keys before the own ones that count too. Computed by each wave for itself,
+// 64 sequences a step, from the lengths on the device.
 struct Unit {
   int b, first, tile, chunk, chunks;  // sequence, its first unit, row tile and chunk of the unit, chunks of a tile
-  int keys;
   Sequence seq;
 };
-__device__ __forceinline__ int chunk_keys(int groups, int target, int grain) {
+// Each tile may begin one chunk more than its share of the target: where the
+// tiles are few those are taken off, so that the units do not pass the target
+// (which is what the device holds at a time) by a few that run alone at the end.
+__device__ __forceinline__ int chunk_keys(int groups, int tiles, int target, int grain) {
+  if (target >= 2 * tiles) target -= tiles;
   const int each = (int)((uint32_t)groups / (uint32_t)target) * 16 + 16;
   return max(2 * grain, (each + grain - 1) / grain * grain);
 }
-// False if there is no such unit; keys is set in any case.
-__device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int rows, int grain, Unit* u) {
+// False if there is no such unit.
+__device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int rows, int grain, int shared, Unit* u) {
   const int lane = threadIdx.x & 63, steps = (a.batch + 63) >> 6;
-  int groups = 0, before = 0;
+  int groups = 0, all_tiles = 0, before = 0, keys = 0;
   Sequence s;
-  u->keys = 0;
   // `steps` steps to add the keys up, `steps` more to find the unit; up to 64
   // sequences are read once
   for (int i = 0; i < 2 * steps; ++i) {
@@ -203,11 +218,12 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int rows,
     }
     const int tiles = (int)((uint32_t)(s.n * a.group + rows - 1) / (uint32_t)rows);
     if (i < steps) {
-      groups += lane_value(wave_scan(tiles * ((s.len + 15) >> 4)), 63);
-      if (i + 1 == steps) u->keys = uniform(chunk_keys(groups, a.p.own_target, grain));
+      groups += lane_value(wave_scan(tiles * ((shared + s.len + 15) >> 4)), 63);
+      all_tiles += lane_value(wave_scan(tiles), 63);
+      if (i + 1 == steps) keys = uniform(chunk_keys(groups, all_tiles, a.p.own_target, grain));
       continue;
     }
-    const int chunks = (int)((uint32_t)(s.len + u->keys - 1) / (uint32_t)u->keys), n = tiles * chunks;
+    const int chunks = max(1, (int)((uint32_t)(shared + s.len + keys - 1) / (uint32_t)keys)), n = tiles * chunks;
     const int upto = wave_scan(n);
     const uint64_t past = __ballot(before + upto > unit);
     if (past) {
@@ -238,28 +254,25 @@ struct Keys {
 };
 
 // What a workgroup does: up to two runs of keys (the prefix's, then the
-// sequence's own) for `rows` query rows, and where the result goes. Every
-// field is the same in all lanes.
+// sequence's own) for `rows` query rows. Every field is the same in all lanes.
 struct Job {
   Keys prefix, own;
   int tiles0, tiles;       // key tiles of the prefix, of both
   int token0, row0, rows;  // query row r: token token0 + (row0 + r) / group
   int own_base;            // own key index that row r sees last: own_base + (row0 + r) / group
-  bool whole;              // the result is the output; else the partial one of slot `part`
-  int64_t part;
+  int first, chunk, chunks;  // the units of these rows, which of them this one is
 };
 
-// kWhole: a row tile's prefix and own keys, all of them. kOwn: one chunk of
-// its own keys. kPrefix: one share of the prefix for a tile of all the tokens'
-// rows.
-enum Mode { kWhole, kOwn, kPrefix };
+// kWhole: all keys of a row tile, the prefix's and its own. kSplit: a chunk of
+// them. kOwn: a chunk of its own keys; the prefix's come as partial results
+// from kPrefix: a share of the prefix for a tile of all the tokens' rows.
+enum Mode { kWhole, kSplit, kOwn, kPrefix };
 
 // Fills a job from the block index; false if the block has nothing to do.
 template <Mode MODE, int ROWS, int KT, int GRAIN>
-__device__ __forceinline__ bool find_job(const AttnArgs& a, int unit, int head, Job* j) {
+__device__ __forceinline__ bool find_job(const AttnArgs& a, int unit, Job* j) {
   j->prefix = j->own = Keys{a.prefix_pages, 0, -1};
-  j->tiles0 = 0;
-  j->part = (int64_t)unit * a.kv_heads + head;
+  j->first = unit, j->chunk = 0, j->chunks = 1;
   if constexpr (MODE == kPrefix) {
     const int splits = a.p.prefix_splits, tile = (int)((uint32_t)unit / (uint32_t)splits), s = unit - tile * splits;
     const int each = (int)(((uint32_t)(a.prefix_len + splits - 1) / (uint32_t)splits + GRAIN - 1) / GRAIN) * GRAIN;
@@ -269,48 +282,46 @@ __device__ __forceinline__ bool find_job(const AttnArgs& a, int unit, int head, 
     j->row0 = tile * ROWS;
     j->rows = min(ROWS, a.tokens * a.group - j->row0);
     j->own_base = -1;
-    j->whole = false;
     j->tiles0 = j->tiles = (j->prefix.last - j->prefix.first + KT) / KT;
     return true;
   }
+  const int shared = MODE == kOwn ? 0 : a.prefix_len;
   Sequence s;
-  int b, chunk = 0, chunks = 1;
-  if constexpr (MODE == kOwn) {
-    Unit u;
-    const bool found = find_unit(a, unit, ROWS, GRAIN, &u);
-    if (threadIdx.x == 0 && head == 0) {
-      if (unit == 0) a.info[0] = u.keys;
-      if (found && unit == u.first) a.info[1 + u.b] = u.first;
-    }
-    if (!found) return false;
-    s = Sequence{uniform(u.seq.start), uniform(u.seq.n), uniform(u.seq.len)};
-    b = uniform(u.b), chunk = uniform(u.chunk), chunks = uniform(u.chunks);
-    j->row0 = uniform(u.tile) * ROWS;
-  } else {
+  int b;
+  if constexpr (MODE == kWhole) {
     b = uniform(sequence_of_slot(a, unit, ROWS));
     s = sequence(a, b);
     s = Sequence{uniform(s.start), uniform(s.n), uniform(s.len)};
     j->row0 = uniform((unit - first_tile(a, b, s.start, ROWS)) * ROWS);
     // a slot before those of a first sequence that starts late
     if (j->row0 < 0) return false;
+  } else {
+    Unit u;
+    if (!find_unit(a, unit, ROWS, GRAIN, shared, &u)) return false;
+    s = Sequence{uniform(u.seq.start), uniform(u.seq.n), uniform(u.seq.len)};
+    b = uniform(u.b), j->chunk = uniform(u.chunk), j->chunks = uniform(u.chunks);
+    j->row0 = uniform(u.tile) * ROWS;
+    j->first = unit - j->chunk;
   }
   j->rows = min(ROWS, s.n * a.group - j->row0);
   if (j->rows <= 0) return false;
-  const int visible = uniform(visible_keys(s, j->row0, j->rows, a.group));
-  j->own.ids = a.table + b * a.table_stride;
-  j->own.last = visible - 1;
+  const int visible = shared + uniform(visible_keys(s, j->row0, j->rows, a.group));
   j->token0 = s.start;
   j->own_base = s.len - s.n;
-  j->whole = true;
-  if constexpr (MODE == kOwn) {
-    const int each = uniform((int)(((uint32_t)(visible + chunks - 1) / (uint32_t)chunks + GRAIN - 1) / GRAIN) * GRAIN);
-    j->own.first = min(chunk * each, visible);
-    j->own.last = min(j->own.first + each, visible) - 1;
-    j->whole = chunks == 1 && a.prefix_len == 0;
-  } else {
-    j->prefix.last = a.prefix_len - 1;
-    j->tiles0 = (a.prefix_len + KT - 1) / KT;
+  j->own.ids = a.table + b * a.table_stride;
+  // this chunk's keys [k0, k1) of those that the rows see, the prefix's before the own
+  int k0 = 0, k1 = visible;
+  if constexpr (MODE != kWhole) {
+    const int each = uniform((int)(((uint32_t)(visible + j->chunks - 1) / (uint32_t)j->chunks + GRAIN - 1) / GRAIN) * GRAIN);
+    k0 = min(j->chunk * each, visible);
+    k1 = min(k0 + each, visible);
   }
+  j->prefix.first = min(k0, shared), j->prefix.last = min(k1, shared) - 1;
+  // own keys are aligned to their pages: a chunk's bounds go down to whole groups of 16 of them
+  const int o0 = max(0, k0 - shared), o1 = max(0, k1 - shared);
+  j->own.first = o0 & ~15;
+  j->own.last = (k0 == k1 ? j->own.first : k1 == visible ? o1 : o1 & ~15) - 1;
+  j->tiles0 = (j->prefix.last - j->prefix.first + KT) / KT;
   j->tiles = j->tiles0 + (j->own.last - j->own.first + KT) / KT;
   return true;
 }
@@ -323,8 +334,51 @@ __device__ __forceinline__ Keys uniform(const Keys& k) {
   return Keys{(const int32_t*)ids, uniform(k.first), uniform(k.last)};
 }
 __device__ __forceinline__ Job uniform(const Job& j) {
-  return Job{uniform(j.prefix), uniform(j.own),  uniform(j.tiles0),   uniform(j.tiles),      uniform(j.token0),
-             uniform(j.row0),   uniform(j.rows), uniform(j.own_base), uniform(j.whole) != 0, j.part};
+  return Job{uniform(j.prefix), uniform(j.own),      uniform(j.tiles0), uniform(j.tiles), uniform(j.token0), uniform(j.row0),
+             uniform(j.rows),   uniform(j.own_base), uniform(j.first),  uniform(j.chunk), uniform(j.chunks)};
+}
+
+// ---------------------------------------------------------------------------
+// Joining the chunks of a row tile: each workgroup writes its partial result
+// with device-scope stores, which gfx950 performs past the XCD's L2, waits for
+// them, and counts in on the tile's counter; the one that counts last joins
+// the partials, in chunk order whichever it is, and leaves the counter at 0.
+// No cache-wide fence, one launch.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void store_device(float* p, float x, float y) {
+  const uint64_t v = (uint64_t)__float_as_uint(x) | (uint64_t)__float_as_uint(y) << 32;
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_device(const float* p) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return float2{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
+}
+// Whether this workgroup is the tile's last; `flag`: a word of LDS.
+__device__ __forceinline__ bool counts_last(int32_t* counter, int chunks, volatile int* flag) {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == chunks - 1;
+    if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = last;
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+// The factors that bring a result with reference `top` and one with reference
+// `ref` to their common one, which becomes `top`. A part without keys has the
+// reference -inf and counts for nothing.
+__device__ __forceinline__ float2 join_factors(float* top, float ref) {
+  const float next = fmaxf(*top, ref);
+  const float2 f{*top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(*top - next),
+                 ref == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - next)};
+  *top = next;
+  return f;
+}
+// a f.x + b f.y, where a factor of 0 takes its value out whatever that is.
+__device__ __forceinline__ float joined(float2 f, float a, float b) {
+  return (f.x == 0.0f ? 0.0f : a * f.x) + (f.y == 0.0f ? 0.0f : b * f.y);
 }
 
 // One 1 KB copy of a key tile: rows [row, row + 1024 / (2 D)) of the tile that
@@ -415,21 +469,44 @@ __device__ __forceinline__ float with_non_finite(float o, const NonFinite<D>& n,
 }
 
 // ---------------------------------------------------------------------------
-// Few rows (up to 16): a decode step. HBM-bound: each wave streams 32-key
+// Few rows (up to 16): a decode step. HBM-bound: each wave streams 16-key
 // tiles of its own through its own ring of two stages, with no barrier, and
-// the waves' results meet in LDS at the end. 16x16x32 MFMA; a lane holds row
-// lane % 16 and keys 4 (lane / 16) + 0..3 of each 16.
+// the waves' results meet in LDS at the end. 16x16 MFMA; a lane holds row
+// lane % 16 and keys 4 (lane / 16) + 0..3 of a tile.
 // ---------------------------------------------------------------------------
+// Partial results that a thread has in flight when it joins them.
+constexpr int kJoinAhead = 8;
+
+// Tokens that belong to no sequence come out as 0: those past the last start.
+template <int D>
+__device__ __forceinline__ void zero_loose_tokens(const AttnArgs& a, int head, int threads) {
+  const int end = a.starts ? clamped(read_only(a.starts, a.batch), 0, a.tokens) : a.tokens;
+  for (int t = end; t < a.tokens; ++t)
+    for (int i = threadIdx.x; i < a.group * D; i += threads) a.out[((int64_t)t * a.q_heads + head * a.group) * D + i] = 0;
+}
+
+// Four channels of a row put together from parts.
+struct Joined {
+  float top = -__builtin_inff(), total = 0.0f;
+  f32x4 o{0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(float ref, float sum, f32x4 x) {
+    const float2 f = join_factors(&top, ref);
+    total = joined(f, total, sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = joined(f, o[e], x[e]);
+  }
+};
+
 template <int D>
 struct Few {
-  static constexpr int kWaves = D == 256 ? 2 : 4, kTile = 32, kStage = 2 * kTile * 2 * D, kGrain = kTile * kWaves;
+  static constexpr int kWaves = 4, kTile = 16, kStage = 2 * kTile * 2 * D, kGrain = kTile * kWaves;
 };
 
 template <class H, int D, Mode MODE>
 __global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArgs a) {
   constexpr int W = Few<D>::kWaves, KT = Few<D>::kTile, STAGE = Few<D>::kStage, ROWB = 2 * D;
   constexpr int COPIES = KT * ROWB / 1024, CHUNKS = D / 8, RPC = 64 / CHUNKS;  // copies of a tile, rows of a copy
-  constexpr int MERGE = W * kFewRows * (D + 2) * 4;
+  constexpr int MERGE = W * kFewRows * (D + 2) * 4 + 64 * W * 24;
   constexpr int LDS = W * 2 * STAGE > MERGE ? W * 2 * STAGE : MERGE;
   // one array: with two, the compiler's wait for copies into the one before
   // reads of the other would empty the ring at every tile
@@ -438,8 +515,9 @@ __global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArg
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   init_non_finite(&bad, 64 * W);
   const int head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
+  if (MODE == kOwn && unit == 0) zero_loose_tokens<D>(a, head, 64 * W);
   Job found;
-  if (!find_job<MODE, kFewRows, KT, Few<D>::kGrain>(a, unit, head, &found)) return;
+  if (!find_job<MODE, kFewRows, KT, Few<D>::kGrain>(a, unit, &found)) return;
   const Job j = uniform(found);
   constexpr bool PREFIX = MODE == kPrefix;
   const Keys run = PREFIX ? j.prefix : j.own;
@@ -490,24 +568,17 @@ __global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArg
       wait_vmem_below<COPIES>();
     }
     __builtin_amdgcn_sched_barrier(0);
-    f32x4 s[2];
+    f32x4 s{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const int r = h * 16 + li;
-#pragma unroll
-      for (int ks = 0; ks < D / 32; ++ks)
-        s[h] = H::mfma16(lds_read16(kt + r * ROWB + (((ks * 4 + quarter) ^ k_swizzle<D>(r)) * 16)), q[ks], s[h]);
-    }
+    for (int ks = 0; ks < D / 32; ++ks)
+      s = H::mfma16(lds_read16(kt + li * ROWB + (((ks * 4 + quarter) ^ k_swizzle<D>(li)) * 16)), q[ks], s);
     const bool masked = key0 + KT - 1 > all_see;
     if (masked) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (key0 + h * 16 + quarter * 4 + e > sees) s[h][e] = -__builtin_inff();
+      for (int e = 0; e < 4; ++e)
+        if (key0 + quarter * 4 + e > sees) s[e] = -__builtin_inff();
     }
-    float top = fmaxf(fmaxf(fmaxf(s[0].x, s[0].y), fmaxf(s[0].z, s[0].w)), fmaxf(fmaxf(s[1].x, s[1].y), fmaxf(s[1].z, s[1].w)));
+    float top = fmaxf(fmaxf(s.x, s.y), fmaxf(s.z, s.w));
     if (__any(top * a.scale_log2 > ref + kRescaleAt)) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
@@ -519,19 +590,14 @@ __global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArg
       ref = next;
     }
     const float sub = ref == -__builtin_inff() ? 0.0f : ref - H::kShift;
-    uint32_t p[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[h][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][e], a.scale_log2, -sub));
-        sum += s[h][e];
-      }
-      p[2 * h] = H::pack(s[h].x, s[h].y);
-      p[2 * h + 1] = H::pack(s[h].z, s[h].w);
+    for (int e = 0; e < 4; ++e) {
+      s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.scale_log2, -sub));
+      sum += s[e];
     }
     asm volatile("" : "+v"(sum));  // added up here, not after the weights' last use
-    const i32x4 pb{(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
+    const uint2 pw{H::pack(s.x, s.y), H::pack(s.z, s.w)};
+    const s16x4 pb = __builtin_bit_cast(s16x4, pw);
     if (t + 1 < n_tiles) wait_vmem_below<2 * COPIES>();
     else wait_vmem_below<0>();
     __builtin_amdgcn_sched_barrier(0);
@@ -539,8 +605,8 @@ __global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArg
       take_non_finite<H, D, COPIES>(vt, lane, PREFIX ? kAlways : key0, run.last - key0 + 1, &bad);
       if (lane == 0) bad.tile = 1;
     }
-    // V^T: channels 16 dt + li, keys 4 quarter + 0..3 and 16 + those; a chunk's
-    // swizzle changes its lower four bits only, so dt + 8 lies 256 bytes on
+    // V^T: channels 16 dt + li, keys 4 quarter + 0..3; a chunk's swizzle changes
+    // its lower four bits only, so dt + 8 lies 256 bytes on
     constexpr int AHEAD = D == 64 ? 4 : 8;
     uint32_t at[AHEAD];
     {
@@ -549,18 +615,19 @@ __global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArg
 #pragma unroll
       for (int dt = 0; dt < AHEAD; ++dt) at[dt] = base + (((dt * 2 + ((li >> 1) & 1)) ^ v_swizzle<D>(r)) * 16);
     }
-    i32x4 v[D / 16];
+    s16x4 v[D / 16];
 #pragma unroll
-    for (int dt = 0; dt < AHEAD; dt += 4) lds_read_tr4<0, 16 * ROWB>(at[dt], at[dt + 1], at[dt + 2], at[dt + 3], v + dt);
+    for (int dt = 0; dt < AHEAD; dt += 4) lds_read_tr4<0>(at[dt], at[dt + 1], at[dt + 2], at[dt + 3], v + dt);
     if constexpr (D == 256) {
 #pragma unroll
-      for (int dt = 0; dt < AHEAD; dt += 4) lds_read_tr4<256, 16 * ROWB>(at[dt], at[dt + 1], at[dt + 2], at[dt + 3], v + 8 + dt);
+      for (int dt = 0; dt < AHEAD; dt += 4) lds_read_tr4<256>(at[dt], at[dt + 1], at[dt + 2], at[dt + 3], v + 8 + dt);
     }
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) o[dt] = H::mfma16(v[dt], pb, o[dt]);
+    for (int dt = 0; dt < D / 16; ++dt) o[dt] = H::mfma16k16(v[dt], pb, o[dt]);
   }
   sum += __shfl_xor(sum, 16);
   sum += __shfl_xor(sum, 32);
+  if (sum != sum) ref = sum;  // a NaN that no score set the reference for
 
   // The waves' results, in wave order: [wave][row][D + 2] floats over the rings.
   __syncthreads();
@@ -574,34 +641,98 @@ __global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArg
     if (quarter == 0) mine[D] = ref, mine[D + 1] = sum;
   }
   __syncthreads();
-  float* part_o = (PREFIX ? a.prefix_o : a.part_o) + j.part * (kFewRows * D);
-  float2* part_ml = (PREFIX ? a.prefix_ml : a.part_ml) + j.part * kFewRows;
-  for (int i = threadIdx.x; i < j.rows * (D / 4); i += 64 * W) {
+  const int items = j.rows * (D / 4);  // four channels of a row each
+  const int64_t part = (int64_t)unit * a.kv_heads + head;
+  // the only chunk: its result need not go through memory to meet the prefix's
+  const bool alone = !PREFIX && j.chunks == 1 && (items <= 64 * W || a.p.prefix_splits == 0);
+  Joined kept;
+  const auto write = [&](int i, const Joined& x) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
-    float top = -__builtin_inff(), f[W], total = 0.0f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) top = fmaxf(top, m[(w * kFewRows + r) * (D + 2) + D]);
-    f32x4 out{0.f, 0.f, 0.f, 0.f};
+    const uint32_t rr = (uint32_t)(j.row0 + r), tk = rr / (uint32_t)group, g = rr % (uint32_t)group;
+    store4<H>(a.out + ((j.token0 + (int64_t)tk) * a.q_heads + head * group + (int)g) * D + d,
+              x.o * (x.total == 0.0f ? 0.0f : 1.0f / x.total));
+  };
+  // The prefix's shares (from the launch before) and, after the last chunk,
+  // the chunks' results: `threads per item` threads take turns on an item's
+  // parts, several in flight each, and meet in LDS.
+  const int n_pre = PREFIX ? 0 : a.p.prefix_splits;
+  for (int i = threadIdx.x; i < items; i += 64 * W) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    Joined x;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const float* from = m + (w * kFewRows + r) * (D + 2);
-      f[w] = from[D] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(from[D] - top);
-      total += f[w] * from[D + 1];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] += f[w] * from[d + e];
+      x.add(from[D], from[D + 1], f32x4{from[d], from[d + 1], from[d + 2], from[d + 3]});
     }
-    const uint32_t rr = (uint32_t)(j.row0 + r), tk = rr / (uint32_t)group, g = rr % (uint32_t)group;
     if (bad.tile) {
+      const int sees_own = j.own_base + (int)((uint32_t)(j.row0 + r) / (uint32_t)group);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] = with_non_finite(out[e], bad, d + e, PREFIX ? 0 : j.own_base + (int)tk);
+      for (int e = 0; e < 4; ++e) x.o[e] = with_non_finite(x.o[e], bad, d + e, PREFIX ? 0 : sees_own);
     }
-    if (j.whole) {
-      const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-      store4<H>(a.out + ((j.token0 + (int64_t)tk) * a.q_heads + head * group + (int)g) * D + d, out * inv);
+    if constexpr (PREFIX) {
+      *reinterpret_cast<f32x4*>(a.prefix_o + (part * kFewRows + r) * D + d) = x.o;
+      if (d == 0) a.prefix_ml[part * kFewRows + r] = float2{x.top, x.total};
+    } else if (alone && n_pre == 0) {
+      write(i, x);
+    } else if (alone) {
+      kept = x;
     } else {
-      *reinterpret_cast<f32x4*>(part_o + r * D + d) = out;
-      if (d == 0) part_ml[r] = float2{top, total};
+      float* to = a.part_o + (part * kFewRows + r) * D + d;
+      store_device(to, x.o.x, x.o.y);
+      store_device(to + 2, x.o.z, x.o.w);
+      if (d == 0) store_device(reinterpret_cast<float*>(a.part_ml + part * kFewRows + r), x.top, x.total);
     }
+  }
+  if (PREFIX || (alone && n_pre == 0)) return;
+  if (!alone && !counts_last(a.counters + (int64_t)j.first * a.kv_heads + head, j.chunks, &bad.tile)) return;
+  const int each = items >= 64 * W ? 1 : 64 * W / items;  // threads of an item
+  const int prows = a.p.few_prefix ? kFewRows : kManyRows;
+  for (int base = 0; base < items; base += 64 * W) {
+    const int turn = each == 1 ? 0 : (int)((uint32_t)threadIdx.x / (uint32_t)items);
+    const int i = base + (int)threadIdx.x - turn * items;
+    const bool active = i < items && turn < each;
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    Joined x;
+    if (turn == 0) x = kept;  // nothing where the result went through memory
+    if (active) {
+      const uint32_t rr = (uint32_t)(j.row0 + r), prow = (uint32_t)j.token0 * (uint32_t)group + rr;
+      const int64_t pre0 = ((int64_t)(prow / (uint32_t)prows) * n_pre * a.kv_heads + head) * prows + prow % (uint32_t)prows;
+      const int64_t own0 = ((int64_t)j.first * a.kv_heads + head) * kFewRows + r;
+      const int n = alone ? n_pre : n_pre + j.chunks;
+      for (int c = turn; c < n; c += each * kJoinAhead) {
+        float2 ml[kJoinAhead], v[kJoinAhead][2];
+#pragma unroll
+        for (int u = 0; u < kJoinAhead; ++u) {
+          const int k = min(c + u * each, n - 1);
+          const bool pre = k < n_pre;
+          const int64_t at = pre ? pre0 + (int64_t)k * a.kv_heads * prows : own0 + (int64_t)(k - n_pre) * a.kv_heads * kFewRows;
+          const float* po = (pre ? a.prefix_o : a.part_o) + at * D + d;
+          ml[u] = load_device(reinterpret_cast<const float*>((pre ? a.prefix_ml : a.part_ml) + at));
+          v[u][0] = load_device(po);
+          v[u][1] = load_device(po + 2);
+        }
+#pragma unroll
+        for (int u = 0; u < kJoinAhead; ++u)
+          if (c + u * each < n) x.add(ml[u].x, ml[u].y, f32x4{v[u][0].x, v[u][0].y, v[u][1].x, v[u][1].y});
+      }
+    }
+    if (each > 1) {
+      float* red = m + W * kFewRows * (D + 2);
+      if (active && turn > 0) {
+        float* to = red + threadIdx.x * 6;
+        to[0] = x.top, to[1] = x.total;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[2 + e] = x.o[e];
+      }
+      __syncthreads();
+      if (turn == 0) {
+        for (int k = 1; k < each; ++k) {
+          const float* from = red + (threadIdx.x + k * items) * 6;
+          x.add(from[0], from[1], f32x4{from[2], from[3], from[4], from[5]});
+        }
+      }
+    }
+    if (active && turn == 0) write(i, x);
   }
 }
 
@@ -614,7 +745,7 @@ __global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArg
 template <int D>
 struct Many {
   static constexpr int kTile = D == 256 ? 32 : 64, kGrain = 64;
-  static constexpr int kPerCu = D == 256 ? 1 : 2;  // workgroups of a CU: 512 or 256 registers a lane
+  static constexpr int kPerCu = 2;  // workgroups of a CU: 512 or 256 registers a lane
 };
 
 template <class H, int D, Mode MODE>
@@ -629,13 +760,9 @@ __global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnA
   // whole rows of keys at once: the last tiles, which see the most, come first
   const int unit = MODE == kWhole ? a.p.own_units - 1 - (int)(blockIdx.x / a.kv_heads) : (int)(blockIdx.x / a.kv_heads);
   const int group = a.group, li = lane & 31, half = lane >> 5;
-  if (MODE == kWhole && unit == 0) {
-    // tokens that belong to no sequence come out as 0
-    for (int t = a.starts ? clamped(read_only(a.starts, a.batch), 0, a.tokens) : a.tokens; t < a.tokens; ++t)
-      for (int i = threadIdx.x; i < group * D; i += 256) a.out[((int64_t)t * a.q_heads + head * group) * D + i] = 0;
-  }
+  if (MODE != kPrefix && unit == 0) zero_loose_tokens<D>(a, head, 256);
   Job found;
-  if (!find_job<MODE, kManyRows, KT, Many<D>::kGrain>(a, unit, head, &found)) return;
+  if (!find_job<MODE, kManyRows, KT, Many<D>::kGrain>(a, unit, &found)) return;
   const Job j = uniform(found);
 
   const int row = min(wave * 32 + li, j.rows - 1);
@@ -653,18 +780,28 @@ __global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnA
   const Copier<D> copy_k{reinterpret_cast<const uint8_t*>(a.k_pages) + head_off, page_bytes, a.page_shift, a.pages};
   const Copier<D> copy_v{reinterpret_cast<const uint8_t*>(a.v_pages) + head_off, page_bytes, a.page_shift, a.pages};
   const int copy_row = lane / CHUNKS;
+  // the 16-byte chunk that a lane copies of a row, for the copy's rows from 0 on
+  const uint32_t k_chunk = (uint32_t)((lane & (CHUNKS - 1)) ^ k_swizzle<D>(copy_row));
+  const uint32_t v_chunk = (uint32_t)((lane & (CHUNKS - 1)) ^ v_swizzle<D>(copy_row));
   const auto issue = [&](int t) {
-    const bool first = MODE == kPrefix || (MODE == kWhole && t < j.tiles0);
+    const bool first = MODE == kPrefix || t < j.tiles0;
     const Keys run{first ? j.prefix.ids : j.own.ids, first ? j.prefix.first : j.own.first, first ? j.prefix.last : j.own.last};
     const int key0 = run.first + (first ? t : t - j.tiles0) * KT;
     uint8_t* dst = lds + (t & 1) * STAGE;
+    const uint32_t kc = fresh(k_chunk), vc = fresh(v_chunk);
 #pragma unroll
     for (int i = 0; i < COPIES; ++i) {
       const int r = (wave * COPIES + i) * RPC;
-      copy_k(run, key0, r, dst + r * ROWB, copy_chunk(lane, CHUNKS, k_swizzle<D>(r + copy_row)), copy_row);
-      copy_v(run, key0, r, dst + (KT + r) * ROWB, copy_chunk(lane, CHUNKS, v_swizzle<D>(r + copy_row)), copy_row);
+      copy_k(run, key0, r, dst + r * ROWB, (int)kc ^ k_swizzle<D>(r), copy_row);
+      copy_v(run, key0, r, dst + (KT + r) * ROWB, (int)vc ^ v_swizzle<D>(r), copy_row);
     }
   };
+  // LDS addresses in stage 0: K row li, channels 8 half ..; V rows 4 half + ..,
+  // channels (li / 16) 16 .. for the transposing read
+  const int v_row = half * 4 + ((li & 15) >> 2);
+  const uint32_t k_at = lds_address(lds) + li * ROWB + ((half ^ k_swizzle<D>(li)) * 16);
+  const uint32_t v_at = lds_address(lds) + (KT + v_row) * ROWB +
+                        ((((li >> 4) * 2 + ((li >> 1) & 1)) ^ v_swizzle<D>(v_row)) * 16) + (li & 1) * 8;
 
   f32x16 o[D / 32];
 #pragma unroll
@@ -681,22 +818,33 @@ __global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnA
     // Tile t is in LDS. The copies of tile t + 1 are in flight until the reads
     // of V (before which the compiler waits for them), and those of t + 2
     // start when every wave has read tile t.
-    const bool first = MODE == kPrefix || (MODE == kWhole && t < j.tiles0);
+    const bool first = MODE == kPrefix || t < j.tiles0;
     const int key0 = first ? j.prefix.first + t * KT : j.own.first + (t - j.tiles0) * KT;
     const int last = first ? j.prefix.last : j.own.last;
     const int row_last = first ? last : min(sees, last);
-    const uint8_t* kt = lds + (t & 1) * STAGE;
-    uint8_t* vt = lds + (t & 1) * STAGE + KT * ROWB;
+    const uint32_t stage = (uint32_t)(t & 1) * STAGE;
+    // masked for some wave's rows: each wave looks through the quarter of V that it copied
+    if (key0 + KT - 1 > (first ? last : min(wg_sees, last))) {
+      uint8_t* vt = lds + stage + KT * ROWB;
+      if (holds_non_finite<H, COPIES>(vt + wave * COPIES * 1024 + lane * 16) && lane == 0) bad.tile = t + 1;
+      lds_barrier();
+      if (bad.tile == t + 1) {
+        take_non_finite<H, D, COPIES>(vt, wave * COPIES * 64 + lane, first ? kAlways : key0, last - key0 + 1, &bad);
+        lds_barrier();
+      }
+    }
+    if (wave * 32 < j.rows) {  // a wave without rows has its copies and its looking through alone
+    const uint32_t kt = fresh(k_at) + stage;
     f32x16 s[SUB];
 #pragma unroll
-    for (int b = 0; b < SUB; ++b) {
-      const int r = b * 32 + li;
+    for (int b = 0; b < SUB; ++b)
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
+    // channels 16 ks + 8 half ..: the chunk's index takes 2 ks by XOR
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks)
-        s[b] = H::mfma32(lds_read16(kt + r * ROWB + (((ks * 2 + half) ^ k_swizzle<D>(r)) * 16)), q[ks], s[b]);
-    }
+    for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+      for (int b = 0; b < SUB; ++b) s[b] = H::mfma32(lds_read16(kt ^ (ks * 32), b * 32 * ROWB), q[ks], s[b]);
     const bool masked = key0 + KT - 1 > (first ? last : min(all_see, last));
     if (masked) {
 #pragma unroll
@@ -731,31 +879,23 @@ __global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnA
         p[2 * b + (e >> 3)][(e & 7) >> 1] = (int)H::pack(x, y);
       }
     asm volatile("" : "+v"(sum));  // added up here, not after the weights' last use
-    if (key0 + KT - 1 > (first ? last : min(wg_sees, last))) {
-      // masked for some wave: each looks through the quarter that it copied
-      if (holds_non_finite<H, COPIES>(vt + wave * COPIES * 1024 + lane * 16) && lane == 0) bad.tile = t + 1;
-      lds_barrier();
-      if (bad.tile == t + 1) {
-        take_non_finite<H, D, COPIES>(vt, wave * COPIES * 64 + lane, first ? kAlways : key0, last - key0 + 1, &bad);
-        lds_barrier();
+    // V^T: channels 32 dt + li (the chunk takes 4 dt by XOR), keys 16 ks + 4 half
+    // + 0..3 and 8 more
+    const uint32_t vt = fresh(v_at) + stage;
+#pragma unroll
+    for (int ks = 0; ks < 2 * SUB; ++ks)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) {
+        const uint32_t at = vt ^ (dt * 64);
+        o[dt] = H::mfma32(cat_tr(lds_read_tr(at, ks * 16 * ROWB), lds_read_tr(at, (ks * 16 + 8) * ROWB)), p[ks], o[dt]);
       }
     }
-    // V^T: channels 32 dt + li, keys 16 ks + 4 half + 0..3 and 8 more
-    const auto v_frag = [&](int dt, int ks) {
-      const int r = ks * 16 + half * 4 + ((li & 15) >> 2), c = dt * 4 + (li >> 4) * 2 + ((li >> 1) & 1), off = (li & 1) * 8;
-      return cat_tr(lds_read_tr(vt + r * ROWB + ((c ^ v_swizzle<D>(r)) * 16) + off),
-                    lds_read_tr(vt + (r + 8) * ROWB + ((c ^ v_swizzle<D>(r + 8)) * 16) + off));
-    };
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (int ks = 0; ks < 2 * SUB; ++ks) o[dt] = H::mfma32(v_frag(dt, ks), p[ks], o[dt]);
     wait_vmem_below<0>();
     lds_barrier();
     if (t + 2 < j.tiles) issue(t + 2);
   }
   sum += __shfl_xor(sum, 32);
-  if (wave * 32 + li >= j.rows) return;
+  if (sum != sum) ref = sum;  // a NaN that no score set the reference for
   if (j.tiles > 0 && bad.tile) {
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
@@ -763,136 +903,87 @@ __global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnA
       for (int e = 0; e < 16; ++e)
         o[dt][e] = with_non_finite(o[dt][e], bad, dt * 32 + (e >> 2) * 8 + half * 4 + (e & 3), MODE == kPrefix ? 0 : sees);
   }
-  if (j.whole) {
-    uint16_t* to = a.out + ((j.token0 + (int64_t)qtoken) * a.q_heads + head * group + (int)qg) * D + half * 4;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4)
-        store4<H>(to + dt * 32 + e * 2, f32x4{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]} * inv);
-  } else {
-    float* to = (MODE == kPrefix ? a.prefix_o : a.part_o) + (j.part * kManyRows + row) * D + half * 4;
+  const bool mine = wave * 32 + li < j.rows;
+  const int64_t part = (int64_t)unit * a.kv_heads + head;
+  if constexpr (MODE == kPrefix) {
+    if (!mine) return;
+    float* to = a.prefix_o + (part * kManyRows + row) * D + half * 4;
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
         *reinterpret_cast<f32x4*>(to + dt * 32 + e * 2) = f32x4{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]};
-    if (half == 0) (MODE == kPrefix ? a.prefix_ml : a.part_ml)[j.part * kManyRows + row] = float2{ref, sum};
+    if (half == 0) a.prefix_ml[part * kManyRows + row] = float2{ref, sum};
+    return;
   }
-}
-
-// ---------------------------------------------------------------------------
-// Joins a row's partial results, its prefix chunks and its own, in that order:
-// one wave a (token, head).
-// ---------------------------------------------------------------------------
-template <class H, int D>
-__global__ __launch_bounds__(256) void combine_kernel(AttnArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (id >= (int64_t)a.tokens * a.q_heads) return;
-  const int token = (int)((uint32_t)id / (uint32_t)a.q_heads), qh = (int)((uint32_t)id % (uint32_t)a.q_heads);
-  const int head = (int)((uint32_t)qh / (uint32_t)a.group), g = qh - head * a.group;
-
-  // own partials
-  const int rows = a.p.few_own ? kFewRows : kManyRows;
-  int b = token, count = 0;
-  if (a.starts) {
-    for (int base = 0; base < a.batch; base += 64) {
-      const int c = __popcll(__ballot(base + lane < a.batch && start_of(a, min(base + lane, a.batch - 1)) <= token));
-      count += c;
-      if (c < 64) break;
-    }
-    b = count - 1;
-  }
-  bool mine = b >= 0;
-  int n_own = 0, first = 0, own_row = 0;
-  if (mine) {
-    // the last sequence that starts at or before the token: those after it hold no token
-    const Sequence s = sequence(a, uniform(b));
-    const int r = uniform((token - s.start) * a.group + g);
-    mine = r < s.n * a.group;
-    if (mine) {
-      const int keys = a.info[0];
-      n_own = (int)((uint32_t)(s.len + keys - 1) / (uint32_t)keys);
-      if (n_own) first = a.info[1 + b] + (int)((uint32_t)r / (uint32_t)rows) * n_own;
-      own_row = (int)((uint32_t)r % (uint32_t)rows);
-    }
-  }
-  const int n_pre = mine && a.prefix_len ? a.p.prefix_splits : 0;
-  if (mine && n_pre == 0 && n_own == 1) return;  // written already
-  const int prows = a.p.few_prefix ? kFewRows : kManyRows, prow = token * a.group + g;
-  const int64_t pre_unit = (int64_t)(prow / prows) * a.p.prefix_splits;
-  const auto part_of = [&](int i) -> int64_t {
-    const int64_t u = i < n_pre ? pre_unit + i : first + i - n_pre;
-    return (u * a.kv_heads + head) * (i < n_pre ? prows : rows) + (i < n_pre ? prow % prows : own_row);
-  };
-  const auto o_of = [&](int i) { return (i < n_pre ? a.prefix_o : a.part_o) + part_of(i) * D; };
-  const auto ml_of = [&](int i) { return (i < n_pre ? a.prefix_ml : a.part_ml)[part_of(i)]; };
-  // 64 parts a step, their references and sums one a lane; the running result
-  // is scaled when a step's largest reference exceeds those before it.
-  constexpr int PER = D / 64, AHEAD = 8;
-  const int n = n_pre + n_own;
-  float o[PER], total = 0.0f, top = -__builtin_inff();
+  if (MODE == kSplit && j.chunks > 1) {
+    // partials in register order: a wave's value pairs are 512 bytes apart
+    const auto slot = [&](int c) { return (((int64_t)j.first + c) * a.kv_heads + head) * kManyRows; };
+    const auto o_at = [&](int c, int dt, int e) {
+      return a.part_o + slot(c) * D + wave * (32 * D) + ((dt * 8 + (e >> 1)) * 64 + lane) * 2;
+    };
+    const auto ml_at = [&](int c) { return reinterpret_cast<float*>(a.part_ml + slot(c) + wave * 32 + li); };
 #pragma unroll
-  for (int e = 0; e < PER; ++e) o[e] = 0.0f;
-  for (int base = 0; base < n; base += 64) {
-    const int parts = min(64, n - base);
-    const float2 ml = ml_of(base + min(lane, parts - 1));
-    const float mine = lane < parts ? ml.x : -__builtin_inff();
-    float next = fmaxf(top, mine);
+    for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-    for (int s = 1; s < 64; s *= 2) next = fmaxf(next, __shfl_xor(next, s));
-    const float f = mine == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mine - next);
-    const float scale = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top - next);
-    top = next;
-    total = total * scale + wave_sum_f32(f == 0.0f ? 0.0f : f * ml.y);
+      for (int e = 0; e < 16; e += 2) store_device(o_at(j.chunk, dt, e), o[dt][e], o[dt][e + 1]);
+    if (half == 0) store_device(ml_at(j.chunk), ref, sum);
+    if (!counts_last(a.counters + (int64_t)j.first * a.kv_heads + head, j.chunks, &bad.tile)) return;
+    // in chunk order, this one's from memory as well
+    float top = -__builtin_inff(), total = 0.0f;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) o[e] = scale == 0.0f ? 0.0f : o[e] * scale;
-    for (int i = 0; i < parts; i += AHEAD) {
-      float x[AHEAD][PER];
+    for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const float* from = o_of(base + min(i + u, parts - 1)) + lane * PER;
+      for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+    for (int c = 0; c < j.chunks; ++c) {
+      const float2 ml = load_device(ml_at(c));
+      const float2 f = join_factors(&top, ml.x);
+      total = joined(f, total, ml.y);
 #pragma unroll
-        for (int e = 0; e < PER; ++e) x[u][e] = from[e];
-      }
+      for (int dt = 0; dt < D / 32; ++dt) {
+        float2 x[8];
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const float w = i + u < parts ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), min(i + u, parts - 1))) : 0.0f;
+        for (int e = 0; e < 16; e += 2) x[e >> 1] = load_device(o_at(c, dt, e));
 #pragma unroll
-        for (int e = 0; e < PER; ++e) o[e] = w == 0.0f ? o[e] : __builtin_fmaf(w, x[u][e], o[e]);
+        for (int e = 0; e < 16; e += 2) {
+          o[dt][e] = joined(f, o[dt][e], x[e >> 1].x);
+          o[dt][e + 1] = joined(f, o[dt][e + 1], x[e >> 1].y);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // one 32-channel block's loads in flight, for the sake of registers
       }
     }
+    sum = total;
   }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  uint16_t* to = a.out + id * D + lane * PER;
-  if constexpr (PER == 1) {
-    to[0] = (uint16_t)H::pack(o[0] * inv, 0.0f);
-  } else {
+  if (!mine) return;
+  uint16_t* to = a.out + ((j.token0 + (int64_t)qtoken) * a.q_heads + head * group + (int)qg) * D + half * 4;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-    for (int e = 0; e < PER; e += 2) reinterpret_cast<uint32_t*>(to)[e / 2] = H::pack(o[e] * inv, o[e + 1] * inv);
-  }
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      store4<H>(to + dt * 32 + e * 2, f32x4{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]} * inv);
 }
 
 // ---------------------------------------------------------------------------
 // The plan and the launches.
 // ---------------------------------------------------------------------------
-AttnPlan attention_plan(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t prefix_len, bool ragged,
-                        int cus) {
+AttnPlan attention_plan(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t prefix_len,
+                        bool ragged, int cus) {
   AttnPlan p{};
   const int64_t group = q_heads / kv_heads, all_rows = tokens * group;
   p.few_own = all_rows <= batch * kFewRows;
-  p.few_prefix = all_rows <= kFewRows;
   const int64_t rows = p.few_own ? kFewRows : kManyRows;
   const int64_t tiles = !ragged && group <= rows ? batch : all_rows / rows + batch;
-  p.own_units = (int)tiles;
-  p.split = p.few_own || tiles * kv_heads < 2 * cus;
-  if (!p.split) return p;
-  const int64_t want = std::max<int64_t>(1, 2 * cus / kv_heads);
-  p.own_target = (int)want;
-  p.own_units = (int)(want + tiles);
-  if (prefix_len > 0) {
+  // workgroups that the CUs hold at a time: by their LDS, 2 of the many-row
+  // kernel, 4, 2 or 1 of the few-row kernel
+  const int64_t at_once = cus * (p.few_own ? 256 / dim : 2);
+  const int64_t want = std::max<int64_t>(1, at_once / kv_heads);
+  p.split = p.few_own || tiles < want;
+  // as many units as there are counters for
+  p.own_target = (int)std::max<int64_t>(1, std::min(want, kAttnCounters / kv_heads - tiles));
+  p.own_units = (int)(p.split ? p.own_target + tiles : tiles);
+  if (p.few_own && prefix_len > 0) {
+    p.few_prefix = all_rows <= kFewRows;
     const int64_t prows = p.few_prefix ? kFewRows : kManyRows;
     p.prefix_tiles = (int)((all_rows + prows - 1) / prows);
     p.prefix_splits = (int)std::max<int64_t>(1, std::min<int64_t>((want + p.prefix_tiles - 1) / p.prefix_tiles, (prefix_len + 255) / 256));
@@ -902,26 +993,25 @@ AttnPlan attention_plan(int64_t tokens, int64_t batch, int64_t q_heads, int64_t 
 
 static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
-int64_t attention_workspace(const AttnPlan& p, int64_t batch, int64_t kv_heads, int64_t dim) {
+int64_t attention_workspace(const AttnPlan& p, int64_t kv_heads, int64_t dim) {
   if (!p.split) return 0;
   const int64_t own = (int64_t)p.own_units * kv_heads * (p.few_own ? kFewRows : kManyRows);
   const int64_t pre = (int64_t)p.prefix_tiles * p.prefix_splits * kv_heads * (p.few_prefix ? kFewRows : kManyRows);
-  return up256(own * dim * 4) + up256(own * 8) + up256(pre * dim * 4) + up256(pre * 8) + up256(4 * (batch + 1));
+  return up256(own * dim * 4) + up256(own * 8) + up256(pre * dim * 4) + up256(pre * 8);
 }
 
 template <class H, int D>
 static void launch_attention(const AttnArgs& a, hipStream_t stream) {
   const AttnPlan& p = a.p;
-  if (p.split && a.prefix_len) {
+  if (p.prefix_tiles) {
     const unsigned grid = (unsigned)(p.prefix_tiles * p.prefix_splits * a.kv_heads);
     if (p.few_prefix) attend_few_kernel<H, D, kPrefix><<<grid, 64 * Few<D>::kWaves, 0, stream>>>(a);
     else attend_many_kernel<H, D, kPrefix><<<grid, 256, 0, stream>>>(a);
   }
   const unsigned grid = (unsigned)(p.own_units * a.kv_heads);
   if (p.few_own) attend_few_kernel<H, D, kOwn><<<grid, 64 * Few<D>::kWaves, 0, stream>>>(a);
-  else if (p.split) attend_many_kernel<H, D, kOwn><<<grid, 256, 0, stream>>>(a);
+  else if (p.split) attend_many_kernel<H, D, kSplit><<<grid, 256, 0, stream>>>(a);
   else attend_many_kernel<H, D, kWhole><<<grid, 256, 0, stream>>>(a);
-  if (p.split) combine_kernel<H, D><<<(unsigned)(((int64_t)a.tokens * a.q_heads + 3) / 4), 256, 0, stream>>>(a);
 }
 
 hipError_t paged_attention(AttnArgs a, int dim, bool fp16, void* workspace, hipStream_t stream) {
@@ -932,8 +1022,7 @@ hipError_t paged_attention(AttnArgs a, int dim, bool fp16, void* workspace, hipS
     a.part_o = (float*)w, w += up256(own * dim * 4);
     a.part_ml = (float2*)w, w += up256(own * 8);
     a.prefix_o = (float*)w, w += up256(pre * dim * 4);
-    a.prefix_ml = (float2*)w, w += up256(pre * 8);
-    a.info = (int32_t*)w;
+    a.prefix_ml = (float2*)w;
   }
   if (dim == 64) fp16 ? launch_attention<Fp16, 64>(a, stream) : launch_attention<Bf16, 64>(a, stream);
   else if (dim == 128) fp16 ? launch_attention<Fp16, 128>(a, stream) : launch_attention<Bf16, 128>(a, stream);

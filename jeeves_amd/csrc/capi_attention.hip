@@ -123,15 +123,16 @@ int64_t jv_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_
   if (tokens == 0 || batch == 0) return 0;
   const int cus = jv::cu_count_of(-1);
   if (cus <= 0) return -1;
-  return jv::attention_workspace(jv::attention_plan(tokens, batch, q_heads, kv_heads, prefix_len, ragged != 0, cus), batch,
-                                 kv_heads, dim);
+  return jv::attention_workspace(jv::attention_plan(tokens, batch, q_heads, kv_heads, dim, prefix_len, ragged != 0, cus), kv_heads,
+                                 dim);
 }
 
 int jv_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k_pages, const void* v_pages, int64_t pages,
                        int64_t page_size, const int32_t* table, int64_t table_stride, int64_t table_cols,
                        const int32_t* lengths, const int32_t* starts, int64_t batch, const int32_t* prefix_pages,
                        int64_t prefix_len, float scale, void* out, int64_t tokens, int64_t q_heads, int64_t kv_heads,
-                       int64_t dim, int fp16, void* workspace, int64_t workspace_bytes, void* stream) {
+                       int64_t dim, int fp16, void* workspace, int64_t workspace_bytes, int32_t* counters, int64_t n_counters,
+                       void* stream) {
   if (int rc = check_batch(tokens, batch, q_heads, kv_heads, dim, prefix_len)) return rc;
   if (int rc = check_cache(k_pages, v_pages, pages, page_size)) return rc;
   if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(JV_ERR_VALUE, "the scale must be positive and finite, got %g", scale);
@@ -139,7 +140,7 @@ int jv_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k_
     return fail(JV_ERR_VALUE, "without query starts each of the %lld sequences has one token, got %lld", (long long)batch,
                 (long long)tokens);
   if (table_cols < 0 || table_stride < 0 || table_cols > INT32_MAX / page_size ||
-      (batch + tokens * (q_heads / kv_heads) / 16) * (table_cols * page_size / 16 + 1) > INT32_MAX)
+      (batch + tokens * (q_heads / kv_heads) / 16) * ((table_cols * page_size + prefix_len) / 16 + 1) > INT32_MAX)
     return fail(JV_ERR_VALUE, "page table of %lld columns for a batch of %lld is too large", (long long)table_cols, (long long)batch);
   if (tokens == 0) return JV_OK;
   if (batch == 0) return fail(JV_ERR_VALUE, "%lld tokens of no sequence", (long long)tokens);
@@ -150,10 +151,13 @@ int jv_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k_
   const int cus = jv::cu_count_of(-1);
   if (cus <= 0) return fail(JV_ERR_HIP, "cannot query the device's compute units");
   jv::AttnArgs a{};
-  a.p = jv::attention_plan(tokens, batch, q_heads, kv_heads, prefix_len, starts != nullptr, cus);
-  const int64_t need = jv::attention_workspace(a.p, batch, kv_heads, dim);
+  a.p = jv::attention_plan(tokens, batch, q_heads, kv_heads, dim, prefix_len, starts != nullptr, cus);
+  const int64_t need = jv::attention_workspace(a.p, kv_heads, dim);
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
     return fail(JV_ERR_VALUE, "workspace needs %lld bytes, 256-byte aligned", (long long)need);
+  if (a.p.split && (!counters || n_counters < (int64_t)a.p.own_units * kv_heads))
+    return fail(JV_ERR_VALUE, "%lld units exceed the %lld counters", (long long)a.p.own_units * kv_heads, (long long)n_counters);
+  a.counters = counters;
   a.q = (const uint16_t*)q, a.q_ts = q_ts, a.q_hs = q_hs;
   a.k_pages = (const uint16_t*)k_pages, a.v_pages = (const uint16_t*)v_pages;
   a.pages = (int)pages, a.page_shift = page_shift_of(page_size);
