@@ -24,6 +24,8 @@
 // K and V tiles go from global memory to LDS directly (16 bytes a lane), with
 // their 16-byte chunks XOR-swizzled so that both kinds of reads meet 256
 // bytes of distinct banks.
+#include <type_traits>
+
 #include "attention.h"
 
 namespace jv {
@@ -60,17 +62,11 @@ __device__ __forceinline__ i32x4 lds_read16(uint32_t at, uint32_t offset) {
   return *(lds_i32x4*)((lds_u8*)(uintptr_t)at + offset);
 }
 
-// Four 16-bit values of one column: of the 4 x 16 block that 16 consecutive
-// lanes address (8 bytes a lane, four lanes a row), lane i gets column i.
-__device__ __forceinline__ s16x4 lds_read_tr(uint32_t at, uint32_t offset) {
-  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  typedef __attribute__((address_space(3))) uint8_t lds_u8;
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((lds_u8*)(uintptr_t)at + offset));
-}
-
-// The same for four addresses plus OFF bytes, as one block with its wait:
-// before the builtin the compiler waits for every copy to LDS in flight, the
-// next tile's too; the block waits for the LDS reads alone.
+// Transposing reads: of the 4 x 16 block of 16-bit values that 16 consecutive
+// lanes address (8 bytes a lane, four lanes a row), lane i gets column i. Four
+// addresses plus OFF bytes, as one block with its wait: before the builtin the
+// compiler waits for every copy to LDS in flight, the next tile's too; the
+// block waits for the LDS reads alone.
 template <int OFF>
 __device__ __forceinline__ void lds_read_tr4(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, s16x4* out) {
   typedef int i32x2 __attribute__((ext_vector_type(2)));
@@ -87,15 +83,33 @@ __device__ __forceinline__ void lds_read_tr4(uint32_t a0, uint32_t a1, uint32_t 
   out[0] = __builtin_bit_cast(s16x4, x0), out[1] = __builtin_bit_cast(s16x4, x1);
   out[2] = __builtin_bit_cast(s16x4, x2), out[3] = __builtin_bit_cast(s16x4, x3);
 }
+// Four 8-value operands from two addresses: of each address the reads at A0
+// and A1 make one, those at B0 and B1 another; in the order a A, b A, a B, b B.
+template <int A0, int A1, int B0, int B1>
+__device__ __forceinline__ void lds_read_tr8(uint32_t a, uint32_t b, i32x4* out) {
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  i32x2 x[8];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%c10\n"
+      "ds_read_b64_tr_b16 %1, %8 offset:%c11\n"
+      "ds_read_b64_tr_b16 %2, %9 offset:%c10\n"
+      "ds_read_b64_tr_b16 %3, %9 offset:%c11\n"
+      "ds_read_b64_tr_b16 %4, %8 offset:%c12\n"
+      "ds_read_b64_tr_b16 %5, %8 offset:%c13\n"
+      "ds_read_b64_tr_b16 %6, %9 offset:%c12\n"
+      "ds_read_b64_tr_b16 %7, %9 offset:%c13\n"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+      : "v"(a), "v"(b), "n"(A0), "n"(A1), "n"(B0), "n"(B1)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = i32x4{x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y};
+}
 
 // LDS byte address of a pointer into a __shared__ array.
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   typedef __attribute__((address_space(3))) const uint8_t lds_u8;
   return (uint32_t)(uintptr_t)(lds_u8*)p;
-}
-
-__device__ __forceinline__ i32x4 cat_tr(s16x4 a, s16x4 b) {
-  return __builtin_bit_cast(i32x4, s16x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w});
 }
 
 // Both are linear over XOR: swizzle(r | s) = swizzle(r) ^ swizzle(s) for rows
@@ -366,6 +380,14 @@ __device__ __forceinline__ bool counts_last(int32_t* counter, int chunks, volati
   return *flag != 0;
 }
 
+template <int N, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+  if constexpr (N > 0) {
+    static_for<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
+
 // The factors that bring a result with reference `top` and one with reference
 // `ref` to their common one, which becomes `top`. A part without keys has the
 // reference -inf and counts for nothing.
@@ -381,26 +403,24 @@ __device__ __forceinline__ float joined(float2 f, float a, float b) {
   return (f.x == 0.0f ? 0.0f : a * f.x) + (f.y == 0.0f ? 0.0f : b * f.y);
 }
 
-// One 1 KB copy of a key tile: rows [row, row + 1024 / (2 D)) of the tile that
-// starts at key0, from page memory to LDS. Keys past the run's last come from
-// its last 16 keys' group or are the last key again, so nothing outside a
-// sequence's keys is read; the scores mask them.
-template <int D>
-struct Copier {
-  const uint8_t* base;  // this head's first page
-  int64_t page_bytes;   // of all heads
-  int page_shift, pages;
-  __device__ __forceinline__ void operator()(const Keys& r, int key0, int row, uint8_t* dst, int swizzled_chunk,
-                                             int lane_row) const {
-    const int group = min((key0 + row) & ~15, r.last & ~15);  // one for the wave
-    const uint32_t id = min((uint32_t)max(read_only(r.ids, group >> page_shift), 0), (uint32_t)(pages - 1));
-    const uint8_t* from = base + (int64_t)id * page_bytes + (group & ((1 << page_shift) - 1)) * (2 * D);
-    const uint32_t at = (uint32_t)min((row & 15) + lane_row, r.last - group);
-    load_lds16(from + (at * (2 * D) + (uint32_t)swizzled_chunk * 16), dst);
-  }
+// Where the copies of a key tile come from. A wave copies rows of one aligned
+// group of 16 keys, which lies in one page: the page's id comes by a scalar
+// load a tile ahead of its use. Keys past a run's last come from its last
+// group or are the last key again, so nothing outside a sequence's keys is
+// read; the scores mask them.
+struct Group {
+  int first, left;  // key index of the group's first key, and how many the run has after it
+  int id;           // its page
 };
-
-__device__ __forceinline__ int copy_chunk(int lane, int chunks, int swizzle) { return (lane & (chunks - 1)) ^ swizzle; }
+__device__ __forceinline__ Group group_at(const AttnArgs& a, const Keys& run, int key) {
+  const int first = min(key & ~15, run.last & ~15);
+  return Group{first, run.last - first, read_only(run.ids, first >> a.page_shift)};
+}
+// Offset of the group in K and in V, for one head, in bytes.
+__device__ __forceinline__ int64_t group_offset(const AttnArgs& a, const Group& g, int head, int row_bytes) {
+  const uint32_t id = min((uint32_t)max(g.id, 0), (uint32_t)(a.pages - 1));
+  return ((((int64_t)id * a.kv_heads + head) << a.page_shift) + (g.first & ((1 << a.page_shift) - 1))) * row_bytes;
+}
 
 // Output rows: o of channels d .. d + 3 of a row, as the 16-bit type.
 template <class H>
@@ -535,20 +555,22 @@ __global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArg
   const int all_see = PREFIX ? run.last : min(j.own_base + (int)((uint32_t)j.row0 / (uint32_t)group), run.last);
 
   uint8_t* ring = lds + wave * 2 * STAGE;
-  const int64_t page_bytes = ((int64_t)a.kv_heads * ROWB) << a.page_shift, head_off = ((int64_t)head * ROWB) << a.page_shift;
-  const Copier<D> copy_k{reinterpret_cast<const uint8_t*>(a.k_pages) + head_off, page_bytes, a.page_shift, a.pages};
-  const Copier<D> copy_v{reinterpret_cast<const uint8_t*>(a.v_pages) + head_off, page_bytes, a.page_shift, a.pages};
   const int copy_row = lane / CHUNKS;
+  const uint32_t k_chunk = (uint32_t)((lane & (CHUNKS - 1)) ^ k_swizzle<D>(copy_row));
+  const uint32_t v_chunk = (uint32_t)((lane & (CHUNKS - 1)) ^ v_swizzle<D>(copy_row));
   const int n_tiles = (j.tiles - wave + W - 1) / W;  // this wave's: wave, wave + W, ..
-  const auto issue = [&](int t) {
-    const int key0 = run.first + (t * W + wave) * KT;
+  const auto group_of = [&](int t) { return group_at(a, run, run.first + (t * W + wave) * KT); };
+  const auto issue = [&](int t, const Group& g) {
     uint8_t* dst = ring + (t & 1) * STAGE;
+    const int64_t off = group_offset(a, g, head, ROWB);
+    const uint8_t *ks = reinterpret_cast<const uint8_t*>(a.k_pages) + off, *vs = reinterpret_cast<const uint8_t*>(a.v_pages) + off;
 #pragma unroll
     for (int i = 0; i < COPIES; ++i)
-      copy_k(run, key0, i * RPC, dst + i * 1024, copy_chunk(lane, CHUNKS, k_swizzle<D>(i * RPC + copy_row)), copy_row);
+      load_lds16(ks + ((uint32_t)min(i * RPC + copy_row, g.left) * ROWB + (k_chunk ^ k_swizzle<D>(i * RPC)) * 16), dst + i * 1024);
 #pragma unroll
     for (int i = 0; i < COPIES; ++i)
-      copy_v(run, key0, i * RPC, dst + KT * ROWB + i * 1024, copy_chunk(lane, CHUNKS, v_swizzle<D>(i * RPC + copy_row)), copy_row);
+      load_lds16(vs + ((uint32_t)min(i * RPC + copy_row, g.left) * ROWB + (v_chunk ^ v_swizzle<D>(i * RPC)) * 16),
+                 dst + KT * ROWB + i * 1024);
   };
 
   f32x4 o[D / 16];
@@ -556,13 +578,18 @@ __global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArg
   for (int dt = 0; dt < D / 16; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   float ref = -__builtin_inff(), sum = 0.0f;
   lds_barrier();  // `bad` is set up
-  if (n_tiles > 0) issue(0);
+  Group next{};
+  if (n_tiles > 0) {
+    issue(0, group_of(0));
+    next = group_of(min(1, n_tiles - 1));
+  }
   for (int t = 0; t < n_tiles; ++t) {
     const int key0 = run.first + (t * W + wave) * KT;
     const uint8_t* kt = ring + (t & 1) * STAGE;
     uint8_t* vt = ring + (t & 1) * STAGE + KT * ROWB;
     if (t + 1 < n_tiles) {
-      issue(t + 1);
+      issue(t + 1, next);
+      next = group_of(min(t + 2, n_tiles - 1));
       wait_vmem_below<3 * COPIES>();
     } else {
       wait_vmem_below<COPIES>();
@@ -776,24 +803,28 @@ __global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnA
   const int all_see = j.own_base + (int)((uint32_t)(j.row0 + min(wave * 32, j.rows - 1)) / (uint32_t)group);
   const int wg_sees = j.own_base + (int)((uint32_t)j.row0 / (uint32_t)group);
 
-  const int64_t page_bytes = ((int64_t)a.kv_heads * ROWB) << a.page_shift, head_off = ((int64_t)head * ROWB) << a.page_shift;
-  const Copier<D> copy_k{reinterpret_cast<const uint8_t*>(a.k_pages) + head_off, page_bytes, a.page_shift, a.pages};
-  const Copier<D> copy_v{reinterpret_cast<const uint8_t*>(a.v_pages) + head_off, page_bytes, a.page_shift, a.pages};
   const int copy_row = lane / CHUNKS;
   // the 16-byte chunk that a lane copies of a row, for the copy's rows from 0 on
   const uint32_t k_chunk = (uint32_t)((lane & (CHUNKS - 1)) ^ k_swizzle<D>(copy_row));
   const uint32_t v_chunk = (uint32_t)((lane & (CHUNKS - 1)) ^ v_swizzle<D>(copy_row));
-  const auto issue = [&](int t) {
+  constexpr int ROWS_OF_WAVE = COPIES * RPC;
+  static_assert(16 % ROWS_OF_WAVE == 0, "a wave's rows lie in one group of 16 keys");
+  const auto group_of = [&](int t) {
     const bool first = MODE == kPrefix || t < j.tiles0;
     const Keys run{first ? j.prefix.ids : j.own.ids, first ? j.prefix.first : j.own.first, first ? j.prefix.last : j.own.last};
-    const int key0 = run.first + (first ? t : t - j.tiles0) * KT;
-    uint8_t* dst = lds + (t & 1) * STAGE;
+    return group_at(a, run, run.first + (first ? t : t - j.tiles0) * KT + wave * ROWS_OF_WAVE);
+  };
+  const auto issue = [&](int t, const Group& g) {
+    uint8_t* dst = lds + (t & 1) * STAGE + wave * ROWS_OF_WAVE * ROWB;
+    const int64_t off = group_offset(a, g, head, ROWB);
+    const uint8_t *ks = reinterpret_cast<const uint8_t*>(a.k_pages) + off, *vs = reinterpret_cast<const uint8_t*>(a.v_pages) + off;
     const uint32_t kc = fresh(k_chunk), vc = fresh(v_chunk);
 #pragma unroll
     for (int i = 0; i < COPIES; ++i) {
-      const int r = (wave * COPIES + i) * RPC;
-      copy_k(run, key0, r, dst + r * ROWB, (int)kc ^ k_swizzle<D>(r), copy_row);
-      copy_v(run, key0, r, dst + (KT + r) * ROWB, (int)vc ^ v_swizzle<D>(r), copy_row);
+      const int r = wave * ROWS_OF_WAVE + i * RPC;  // row of the tile; of the group, r % 16
+      const uint32_t row = (uint32_t)min((r & 15) + copy_row, g.left) * ROWB;
+      load_lds16(ks + (row + (kc ^ k_swizzle<D>(r)) * 16), dst + i * 1024);
+      load_lds16(vs + (row + (vc ^ v_swizzle<D>(r)) * 16), dst + KT * ROWB + i * 1024);
     }
   };
   // LDS addresses in stage 0: K row li, channels 8 half ..; V rows 4 half + ..,
@@ -809,15 +840,20 @@ __global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnA
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
   float ref = -__builtin_inff(), sum = 0.0f;
-  if (j.tiles > 0) issue(0);
-  if (j.tiles > 1) issue(1);
-  if (j.tiles > 1) wait_vmem_below<2 * COPIES>();
-  else wait_vmem_below<0>();
-  lds_barrier();
+  Group next{};
+  if (j.tiles > 0) {
+    issue(0, group_of(0));
+    next = group_of(min(1, j.tiles - 1));
+  }
   for (int t = 0; t < j.tiles; ++t) {
-    // Tile t is in LDS. The copies of tile t + 1 are in flight until the reads
-    // of V (before which the compiler waits for them), and those of t + 2
-    // start when every wave has read tile t.
+    // this wave's copies of tile t have landed, then all waves': and all have
+    // read the stage that the next copies overwrite
+    wait_vmem_below<0>();
+    lds_barrier();
+    if (t + 1 < j.tiles) {
+      issue(t + 1, next);
+      next = group_of(min(t + 2, j.tiles - 1));
+    }
     const bool first = MODE == kPrefix || t < j.tiles0;
     const int key0 = first ? j.prefix.first + t * KT : j.own.first + (t - j.tiles0) * KT;
     const int last = first ? j.prefix.last : j.own.last;
@@ -880,19 +916,22 @@ __global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnA
       }
     asm volatile("" : "+v"(sum));  // added up here, not after the weights' last use
     // V^T: channels 32 dt + li (the chunk takes 4 dt by XOR), keys 16 ks + 4 half
-    // + 0..3 and 8 more
+    // + 0..3 and 8 more; two key steps and two channel blocks a read
     const uint32_t vt = fresh(v_at) + stage;
+    static_for<SUB>([&](auto bc) {
+      constexpr int K0 = decltype(bc)::value * 32 * ROWB;
 #pragma unroll
-    for (int ks = 0; ks < 2 * SUB; ++ks)
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) {
-        const uint32_t at = vt ^ (dt * 64);
-        o[dt] = H::mfma32(cat_tr(lds_read_tr(at, ks * 16 * ROWB), lds_read_tr(at, (ks * 16 + 8) * ROWB)), p[ks], o[dt]);
+      for (int dt = 0; dt < D / 32; dt += 2) {
+        i32x4 v[4];
+        lds_read_tr8<K0, K0 + 8 * ROWB, K0 + 16 * ROWB, K0 + 24 * ROWB>(vt ^ (dt * 64), vt ^ (dt * 64 + 64), v);
+        constexpr int ks = decltype(bc)::value * 2;
+        o[dt] = H::mfma32(v[0], p[ks], o[dt]);
+        o[dt + 1] = H::mfma32(v[1], p[ks], o[dt + 1]);
+        o[dt] = H::mfma32(v[2], p[ks + 1], o[dt]);
+        o[dt + 1] = H::mfma32(v[3], p[ks + 1], o[dt + 1]);
       }
+    });
     }
-    wait_vmem_below<0>();
-    lds_barrier();
-    if (t + 2 < j.tiles) issue(t + 2);
   }
   sum += __shfl_xor(sum, 32);
   if (sum != sum) ref = sum;  // a NaN that no score set the reference for
