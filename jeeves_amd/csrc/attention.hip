@@ -83,27 +83,38 @@ __device__ __forceinline__ void lds_read_tr4(uint32_t a0, uint32_t a1, uint32_t 
   out[0] = __builtin_bit_cast(s16x4, x0), out[1] = __builtin_bit_cast(s16x4, x1);
   out[2] = __builtin_bit_cast(s16x4, x2), out[3] = __builtin_bit_cast(s16x4, x3);
 }
-// Four 8-value operands from two addresses: of each address the reads at A0
-// and A1 make one, those at B0 and B1 another; in the order a A, b A, a B, b B.
-template <int A0, int A1, int B0, int B1>
-__device__ __forceinline__ void lds_read_tr8(uint32_t a, uint32_t b, i32x4* out) {
+// 8-value operands from N addresses (2 or 4), each of the reads at A0 and A1.
+template <int N, int A0, int A1>
+__device__ __forceinline__ void lds_read_tr8(const uint32_t* at, i32x4* out) {
   typedef int i32x2 __attribute__((ext_vector_type(2)));
-  i32x2 x[8];
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %8 offset:%c10\n"
-      "ds_read_b64_tr_b16 %1, %8 offset:%c11\n"
-      "ds_read_b64_tr_b16 %2, %9 offset:%c10\n"
-      "ds_read_b64_tr_b16 %3, %9 offset:%c11\n"
-      "ds_read_b64_tr_b16 %4, %8 offset:%c12\n"
-      "ds_read_b64_tr_b16 %5, %8 offset:%c13\n"
-      "ds_read_b64_tr_b16 %6, %9 offset:%c12\n"
-      "ds_read_b64_tr_b16 %7, %9 offset:%c13\n"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
-      : "v"(a), "v"(b), "n"(A0), "n"(A1), "n"(B0), "n"(B1)
-      : "memory");
+  i32x2 x[2 * N];
+  if constexpr (N == 4) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%c12\n"
+        "ds_read_b64_tr_b16 %1, %8 offset:%c13\n"
+        "ds_read_b64_tr_b16 %2, %9 offset:%c12\n"
+        "ds_read_b64_tr_b16 %3, %9 offset:%c13\n"
+        "ds_read_b64_tr_b16 %4, %10 offset:%c12\n"
+        "ds_read_b64_tr_b16 %5, %10 offset:%c13\n"
+        "ds_read_b64_tr_b16 %6, %11 offset:%c12\n"
+        "ds_read_b64_tr_b16 %7, %11 offset:%c13\n"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(A0), "n"(A1)
+        : "memory");
+  } else {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4 offset:%c6\n"
+        "ds_read_b64_tr_b16 %1, %4 offset:%c7\n"
+        "ds_read_b64_tr_b16 %2, %5 offset:%c6\n"
+        "ds_read_b64_tr_b16 %3, %5 offset:%c7\n"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+        : "v"(at[0]), "v"(at[1]), "n"(A0), "n"(A1)
+        : "memory");
+  }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) out[i] = i32x4{x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y};
+  for (int i = 0; i < N; ++i) out[i] = i32x4{x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y};
 }
 
 // LDS byte address of a pointer into a __shared__ array.
@@ -876,11 +887,22 @@ __global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnA
     for (int b = 0; b < SUB; ++b)
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
-    // channels 16 ks + 8 half ..: the chunk's index takes 2 ks by XOR
+    // channels 16 ks + 8 half ..: the chunk's index takes 2 ks by XOR. AHEAD
+    // reads are under way while as many before them are multiplied.
+    constexpr int AHEAD = D == 256 ? 2 : 4, STEPS = AHEAD / SUB, BATCHES = D / 16 / STEPS;
+    i32x4 kf[2][AHEAD];
+    const auto read_k = [&](int i) {
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
+      for (int u = 0; u < AHEAD; ++u) kf[i & 1][u] = lds_read16(kt ^ ((i * STEPS + u / SUB) * 32), (u % SUB) * 32 * ROWB);
+    };
+    read_k(0);
 #pragma unroll
-      for (int b = 0; b < SUB; ++b) s[b] = H::mfma32(lds_read16(kt ^ (ks * 32), b * 32 * ROWB), q[ks], s[b]);
+    for (int i = 0; i < BATCHES; ++i) {
+      if (i + 1 < BATCHES) read_k(i + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) s[u % SUB] = H::mfma32(kf[i & 1][u], q[i * STEPS + u / SUB], s[u % SUB]);
+    }
     const bool masked = key0 + KT - 1 > (first ? last : min(all_see, last));
     if (masked) {
 #pragma unroll
@@ -904,32 +926,41 @@ __global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnA
       ref = next;
     }
     const float sub = ref == -__builtin_inff() ? 0.0f : ref - H::kShift;
-    i32x4 p[2 * SUB];
+    // The weights of 16 keys, as the B operand of their step.
+    const auto weights = [&](int ks) {
+      i32x4 p;
 #pragma unroll
-    for (int b = 0; b < SUB; ++b)
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], a.scale_log2, -sub));
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e + 1], a.scale_log2, -sub));
-        sum += x + y;
-        p[2 * b + (e >> 3)][(e & 7) >> 1] = (int)H::pack(x, y);
+      for (int e = 0; e < 8; e += 2) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks >> 1][(ks & 1) * 8 + e], a.scale_log2, -sub));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks >> 1][(ks & 1) * 8 + e + 1], a.scale_log2, -sub));
+        const uint32_t w = H::pack(x, y);
+        sum = H::add2(w, sum);
+        p[e >> 1] = (int)w;
       }
-    asm volatile("" : "+v"(sum));  // added up here, not after the weights' last use
+      asm volatile("" : "+v"(sum));  // added up here, not after the weights' last use
+      return p;
+    };
     // V^T: channels 32 dt + li (the chunk takes 4 dt by XOR), keys 16 ks + 4 half
-    // + 0..3 and 8 more; two key steps and two channel blocks a read
+    // + 0..3 and 8 more. The next 16 keys' weights are worked out while a step's
+    // products run.
+    constexpr int NB = D == 64 ? 2 : 4;  // channel blocks of a read
     const uint32_t vt = fresh(v_at) + stage;
-    static_for<SUB>([&](auto bc) {
-      constexpr int K0 = decltype(bc)::value * 32 * ROWB;
+    i32x4 p = weights(0);
+    static_for<2 * SUB>([&](auto kc) {
+      constexpr int ks = decltype(kc)::value;
+      i32x4 next_p = p;
+      static_for<D / 32 / NB>([&](auto gc) {
+        constexpr int g = decltype(gc)::value;
+        uint32_t at[NB];
 #pragma unroll
-      for (int dt = 0; dt < D / 32; dt += 2) {
-        i32x4 v[4];
-        lds_read_tr8<K0, K0 + 8 * ROWB, K0 + 16 * ROWB, K0 + 24 * ROWB>(vt ^ (dt * 64), vt ^ (dt * 64 + 64), v);
-        constexpr int ks = decltype(bc)::value * 2;
-        o[dt] = H::mfma32(v[0], p[ks], o[dt]);
-        o[dt + 1] = H::mfma32(v[1], p[ks], o[dt + 1]);
-        o[dt] = H::mfma32(v[2], p[ks + 1], o[dt]);
-        o[dt + 1] = H::mfma32(v[3], p[ks + 1], o[dt + 1]);
-      }
+        for (int i = 0; i < NB; ++i) at[i] = vt ^ (uint32_t)((g * NB + i) * 64);
+        i32x4 v[NB];
+        lds_read_tr8<NB, ks * 16 * ROWB, (ks * 16 + 8) * ROWB>(at, v);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) o[g * NB + i] = H::mfma32(v[i], p, o[g * NB + i]);
+        if constexpr (g == 0 && ks + 1 < 2 * SUB) next_p = weights(ks + 1);
+      });
+      p = next_p;
     });
     }
   }
@@ -1025,7 +1056,7 @@ AttnPlan attention_plan(int64_t tokens, int64_t batch, int64_t q_heads, int64_t 
     p.few_prefix = all_rows <= kFewRows;
     const int64_t prows = p.few_prefix ? kFewRows : kManyRows;
     p.prefix_tiles = (int)((all_rows + prows - 1) / prows);
-    p.prefix_splits = (int)std::max<int64_t>(1, std::min<int64_t>((want + p.prefix_tiles - 1) / p.prefix_tiles, (prefix_len + 255) / 256));
+    p.prefix_splits = (int)std::max<int64_t>(1, std::min<int64_t>((cus / kv_heads + p.prefix_tiles - 1) / p.prefix_tiles, (prefix_len + 255) / 256));
   }
   return p;
 }
