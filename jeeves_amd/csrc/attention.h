@@ -101,14 +101,13 @@ hipError_t norm_rope(const RopeArgs& a, int dim, bool fp16, hipStream_t stream);
 // token and sequence counts alone while the starts stay on the device.
 constexpr int kFewRows = 16, kManyRows = 128;
 
-// Counters a call may use at most; what does not fit is split less.
+// Counters a call may use at most; where they do not suffice no keys are split.
 constexpr int64_t kAttnCounters = 65536;
 
 struct AttnPlan {
   bool few_own, few_prefix;  // tiles of kFewRows rows instead of kManyRows
   bool split;                // the keys of a row tile may go to several workgroups
   int own_units;             // tile slots, or with a split the most units (tile, key chunk) that there can be
-  int own_target;            // units to cut the keys into, before rounding
   int prefix_tiles, prefix_splits;  // where the prefix is gone through apart, for all tokens' rows
 };
 
@@ -129,13 +128,14 @@ struct AttnArgs {
   float *part_o, *prefix_o;      // partial results: [unit, kv_head, rows, dim]
   float2 *part_ml, *prefix_ml;   // their references and sums: [unit, kv_head, rows]
   int32_t* counters;             // 0 before and after each call
+  int2* info;                    // a sequence's first unit and its tiles' chunks, for join_kernel
   AttnPlan p;
 };
 
 // Chosen by the sizes that the host knows.
 AttnPlan attention_plan(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t prefix_len,
                         bool ragged, int cus);
-int64_t attention_workspace(const AttnPlan& p, int64_t kv_heads, int64_t dim);
+int64_t attention_workspace(const AttnPlan& p, int64_t batch, int64_t kv_heads, int64_t dim);
 hipError_t paged_attention(AttnArgs a, int dim, bool fp16, void* workspace, hipStream_t stream);
 
 }  // namespace jv

@@ -117,6 +117,12 @@ __device__ __forceinline__ void lds_read_tr8(const uint32_t* at, i32x4* out) {
   for (int i = 0; i < N; ++i) out[i] = i32x4{x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y};
 }
 
+// Waits out a 16x16 MFMA's result registers, which other instructions may not
+// read for up to 11 issue slots. Where a wave-uniform branch follows the MFMA
+// the compiler has left the wait out on the taken path (rows of scores then
+// differed from run to run), so it stands here, ahead of the branch.
+__device__ __forceinline__ void settle(f32x4* r) { asm volatile("s_nop 7\n\ts_nop 2" : "+v"(*r)); }
+
 // LDS byte address of a pointer into a __shared__ array.
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   typedef __attribute__((address_space(3))) const uint8_t lds_u8;
@@ -211,7 +217,7 @@ __device__ __forceinline__ float wave_sum_f32(float v) {
 
 // Where keys are split over workgroups: the (sequence, row tile, key chunk) of
 // a unit. The tiles' keys are added up (in groups of 16, which the host has
-// checked to fit 32 bits), the sum cut into about `own_target` chunks, and each
+// checked to fit 32 bits), the sum cut into up to `own_units` chunks, and each
 // tile of a sequence gets one unit for each chunk's worth of keys that its
 // sequence has begun, one at least, with equal shares of what it sees. `shared`:
 // keys before the own ones that count too. Computed by each wave for itself,
@@ -220,12 +226,10 @@ struct Unit {
   int b, first, tile, chunk, chunks;  // sequence, its first unit, row tile and chunk of the unit, chunks of a tile
   Sequence seq;
 };
-// Each tile may begin one chunk more than its share of the target: where the
-// tiles are few those are taken off, so that the units do not pass the target
-// (which is what the device holds at a time) by a few that run alone at the end.
+// Keys of a chunk: each tile may begin one chunk more than its share of the
+// target, so the tiles are taken off it and the units never pass it.
 __device__ __forceinline__ int chunk_keys(int groups, int tiles, int target, int grain) {
-  if (target >= 2 * tiles) target -= tiles;
-  const int each = (int)((uint32_t)groups / (uint32_t)target) * 16 + 16;
+  const int each = (int)((uint32_t)groups / (uint32_t)max(1, target - tiles)) * 16 + 16;
   return max(2 * grain, (each + grain - 1) / grain * grain);
 }
 // False if there is no such unit.
@@ -245,7 +249,7 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int rows,
     if (i < steps) {
       groups += lane_value(wave_scan(tiles * ((shared + s.len + 15) >> 4)), 63);
       all_tiles += lane_value(wave_scan(tiles), 63);
-      if (i + 1 == steps) keys = uniform(chunk_keys(groups, all_tiles, a.p.own_target, grain));
+      if (i + 1 == steps) keys = uniform(chunk_keys(groups, all_tiles, a.p.own_units, grain));
       continue;
     }
     const int chunks = max(1, (int)((uint32_t)(shared + s.len + keys - 1) / (uint32_t)keys)), n = tiles * chunks;
@@ -285,7 +289,7 @@ struct Job {
   int tiles0, tiles;       // key tiles of the prefix, of both
   int token0, row0, rows;  // query row r: token token0 + (row0 + r) / group
   int own_base;            // own key index that row r sees last: own_base + (row0 + r) / group
-  int first, chunk, chunks;  // the units of these rows, which of them this one is
+  int sequence, first, chunk, chunks;  // whose rows; their units, and which of them this one is
 };
 
 // kWhole: all keys of a row tile, the prefix's and its own. kSplit: a chunk of
@@ -297,7 +301,7 @@ enum Mode { kWhole, kSplit, kOwn, kPrefix };
 template <Mode MODE, int ROWS, int KT, int GRAIN>
 __device__ __forceinline__ bool find_job(const AttnArgs& a, int unit, Job* j) {
   j->prefix = j->own = Keys{a.prefix_pages, 0, -1};
-  j->first = unit, j->chunk = 0, j->chunks = 1;
+  j->sequence = 0, j->first = unit, j->chunk = 0, j->chunks = 1;
   if constexpr (MODE == kPrefix) {
     const int splits = a.p.prefix_splits, tile = (int)((uint32_t)unit / (uint32_t)splits), s = unit - tile * splits;
     const int each = (int)(((uint32_t)(a.prefix_len + splits - 1) / (uint32_t)splits + GRAIN - 1) / GRAIN) * GRAIN;
@@ -328,6 +332,7 @@ __device__ __forceinline__ bool find_job(const AttnArgs& a, int unit, Job* j) {
     j->row0 = uniform(u.tile) * ROWS;
     j->first = unit - j->chunk;
   }
+  j->sequence = b;
   j->rows = min(ROWS, s.n * a.group - j->row0);
   if (j->rows <= 0) return false;
   const int visible = shared + uniform(visible_keys(s, j->row0, j->rows, a.group));
@@ -360,7 +365,7 @@ __device__ __forceinline__ Keys uniform(const Keys& k) {
 }
 __device__ __forceinline__ Job uniform(const Job& j) {
   return Job{uniform(j.prefix), uniform(j.own),      uniform(j.tiles0), uniform(j.tiles), uniform(j.token0), uniform(j.row0),
-             uniform(j.rows),   uniform(j.own_base), uniform(j.first),  uniform(j.chunk), uniform(j.chunks)};
+             uniform(j.rows),   uniform(j.own_base), uniform(j.sequence), uniform(j.first), uniform(j.chunk), uniform(j.chunks)};
 }
 
 // ---------------------------------------------------------------------------
@@ -531,21 +536,18 @@ struct Joined {
 template <int D>
 struct Few {
   static constexpr int kWaves = 4, kTile = 16, kStage = 2 * kTile * 2 * D, kGrain = kTile * kWaves;
+  static constexpr int kRings = kWaves * 2 * kStage, kMerge = kWaves * kFewRows * (D + 2) * 4 + 64 * kWaves * 24;
+  static constexpr int kLds = kRings > kMerge ? kRings : kMerge;  // NonFinite comes after
 };
 
 template <class H, int D, Mode MODE>
-__global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArgs a) {
+__device__ __forceinline__ void attend_few(const AttnArgs& a, int block, uint8_t* lds) {
   constexpr int W = Few<D>::kWaves, KT = Few<D>::kTile, STAGE = Few<D>::kStage, ROWB = 2 * D;
   constexpr int COPIES = KT * ROWB / 1024, CHUNKS = D / 8, RPC = 64 / CHUNKS;  // copies of a tile, rows of a copy
-  constexpr int MERGE = W * kFewRows * (D + 2) * 4 + 64 * W * 24;
-  constexpr int LDS = W * 2 * STAGE > MERGE ? W * 2 * STAGE : MERGE;
-  // one array: with two, the compiler's wait for copies into the one before
-  // reads of the other would empty the ring at every tile
-  __shared__ __align__(1024) uint8_t lds[LDS + sizeof(NonFinite<D>)];
-  NonFinite<D>& bad = *reinterpret_cast<NonFinite<D>*>(lds + LDS);
+  NonFinite<D>& bad = *reinterpret_cast<NonFinite<D>*>(lds + Few<D>::kLds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   init_non_finite(&bad, 64 * W);
-  const int head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
+  const int unit = (int)((uint32_t)block / (uint32_t)a.kv_heads), head = block - unit * a.kv_heads;
   if (MODE == kOwn && unit == 0) zero_loose_tokens<D>(a, head, 64 * W);
   Job found;
   if (!find_job<MODE, kFewRows, KT, Few<D>::kGrain>(a, unit, &found)) return;
@@ -607,9 +609,12 @@ __global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArg
     }
     __builtin_amdgcn_sched_barrier(0);
     f32x4 s{0.f, 0.f, 0.f, 0.f};
+    i32x4 kf[D / 32];
 #pragma unroll
-    for (int ks = 0; ks < D / 32; ++ks)
-      s = H::mfma16(lds_read16(kt + li * ROWB + (((ks * 4 + quarter) ^ k_swizzle<D>(li)) * 16)), q[ks], s);
+    for (int ks = 0; ks < D / 32; ++ks) kf[ks] = lds_read16(kt + li * ROWB + (((ks * 4 + quarter) ^ k_swizzle<D>(li)) * 16));
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks) s = H::mfma16(kf[ks], q[ks], s);
+    settle(&s);
     const bool masked = key0 + KT - 1 > all_see;
     if (masked) {
 #pragma unroll
@@ -681,19 +686,15 @@ __global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArg
   __syncthreads();
   const int items = j.rows * (D / 4);  // four channels of a row each
   const int64_t part = (int64_t)unit * a.kv_heads + head;
-  // the only chunk: its result need not go through memory to meet the prefix's
-  const bool alone = !PREFIX && j.chunks == 1 && (items <= 64 * W || a.p.prefix_splits == 0);
-  Joined kept;
+  float* part_o = (PREFIX ? a.prefix_o : a.part_o) + part * kFewRows * D;
+  float2* part_ml = (PREFIX ? a.prefix_ml : a.part_ml) + part * kFewRows;
+  const bool joined_later = a.prefix_len > 0;  // by join_kernel, with the prefix's shares
   const auto write = [&](int i, const Joined& x) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
     const uint32_t rr = (uint32_t)(j.row0 + r), tk = rr / (uint32_t)group, g = rr % (uint32_t)group;
     store4<H>(a.out + ((j.token0 + (int64_t)tk) * a.q_heads + head * group + (int)g) * D + d,
               x.o * (x.total == 0.0f ? 0.0f : 1.0f / x.total));
   };
-  // The prefix's shares (from the launch before) and, after the last chunk,
-  // the chunks' results: `threads per item` threads take turns on an item's
-  // parts, several in flight each, and meet in LDS.
-  const int n_pre = PREFIX ? 0 : a.p.prefix_splits;
   for (int i = threadIdx.x; i < items; i += 64 * W) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
     Joined x;
@@ -707,51 +708,47 @@ __global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArg
 #pragma unroll
       for (int e = 0; e < 4; ++e) x.o[e] = with_non_finite(x.o[e], bad, d + e, PREFIX ? 0 : sees_own);
     }
-    if constexpr (PREFIX) {
-      *reinterpret_cast<f32x4*>(a.prefix_o + (part * kFewRows + r) * D + d) = x.o;
-      if (d == 0) a.prefix_ml[part * kFewRows + r] = float2{x.top, x.total};
-    } else if (alone && n_pre == 0) {
+    if (PREFIX || joined_later) {
+      *reinterpret_cast<f32x4*>(part_o + r * D + d) = x.o;
+      if (d == 0) part_ml[r] = float2{x.top, x.total};
+    } else if (j.chunks == 1) {
       write(i, x);
-    } else if (alone) {
-      kept = x;
     } else {
-      float* to = a.part_o + (part * kFewRows + r) * D + d;
-      store_device(to, x.o.x, x.o.y);
-      store_device(to + 2, x.o.z, x.o.w);
-      if (d == 0) store_device(reinterpret_cast<float*>(a.part_ml + part * kFewRows + r), x.top, x.total);
+      store_device(part_o + r * D + d, x.o.x, x.o.y);
+      store_device(part_o + r * D + d + 2, x.o.z, x.o.w);
+      if (d == 0) store_device(reinterpret_cast<float*>(part_ml + r), x.top, x.total);
     }
   }
-  if (PREFIX || (alone && n_pre == 0)) return;
-  if (!alone && !counts_last(a.counters + (int64_t)j.first * a.kv_heads + head, j.chunks, &bad.tile)) return;
-  const int each = items >= 64 * W ? 1 : 64 * W / items;  // threads of an item
-  const int prows = a.p.few_prefix ? kFewRows : kManyRows;
+  if (PREFIX) return;
+  if (joined_later) {
+    if (head == 0 && j.chunk == 0 && j.row0 == 0 && threadIdx.x == 0) a.info[j.sequence] = int2{j.first, j.chunks};
+    return;
+  }
+  if (j.chunks == 1) return;
+  if (!counts_last(a.counters + (int64_t)j.first * a.kv_heads + head, j.chunks, &bad.tile)) return;
+  // The chunks' results: `each` threads take turns on an item's parts, several
+  // in flight a thread, and meet in LDS.
+  const int each = items >= 64 * W ? 1 : 64 * W / items;
   for (int base = 0; base < items; base += 64 * W) {
     const int turn = each == 1 ? 0 : (int)((uint32_t)threadIdx.x / (uint32_t)items);
     const int i = base + (int)threadIdx.x - turn * items;
     const bool active = i < items && turn < each;
     const int r = i / (D / 4), d = i % (D / 4) * 4;
     Joined x;
-    if (turn == 0) x = kept;  // nothing where the result went through memory
     if (active) {
-      const uint32_t rr = (uint32_t)(j.row0 + r), prow = (uint32_t)j.token0 * (uint32_t)group + rr;
-      const int64_t pre0 = ((int64_t)(prow / (uint32_t)prows) * n_pre * a.kv_heads + head) * prows + prow % (uint32_t)prows;
-      const int64_t own0 = ((int64_t)j.first * a.kv_heads + head) * kFewRows + r;
-      const int n = alone ? n_pre : n_pre + j.chunks;
-      for (int c = turn; c < n; c += each * kJoinAhead) {
+      const int64_t first = ((int64_t)j.first * a.kv_heads + head) * kFewRows + r;
+      for (int c = turn; c < j.chunks; c += each * kJoinAhead) {
         float2 ml[kJoinAhead], v[kJoinAhead][2];
 #pragma unroll
         for (int u = 0; u < kJoinAhead; ++u) {
-          const int k = min(c + u * each, n - 1);
-          const bool pre = k < n_pre;
-          const int64_t at = pre ? pre0 + (int64_t)k * a.kv_heads * prows : own0 + (int64_t)(k - n_pre) * a.kv_heads * kFewRows;
-          const float* po = (pre ? a.prefix_o : a.part_o) + at * D + d;
-          ml[u] = load_device(reinterpret_cast<const float*>((pre ? a.prefix_ml : a.part_ml) + at));
-          v[u][0] = load_device(po);
-          v[u][1] = load_device(po + 2);
+          const int64_t at = first + (int64_t)min(c + u * each, j.chunks - 1) * a.kv_heads * kFewRows;
+          ml[u] = load_device(reinterpret_cast<const float*>(a.part_ml + at));
+          v[u][0] = load_device(a.part_o + at * D + d);
+          v[u][1] = load_device(a.part_o + at * D + d + 2);
         }
 #pragma unroll
         for (int u = 0; u < kJoinAhead; ++u)
-          if (c + u * each < n) x.add(ml[u].x, ml[u].y, f32x4{v[u][0].x, v[u][0].y, v[u][1].x, v[u][1].y});
+          if (c + u * each < j.chunks) x.add(ml[u].x, ml[u].y, f32x4{v[u][0].x, v[u][0].y, v[u][1].x, v[u][1].y});
       }
     }
     if (each > 1) {
@@ -783,20 +780,19 @@ __global__ __launch_bounds__(64 * Few<D>::kWaves) void attend_few_kernel(AttnArg
 template <int D>
 struct Many {
   static constexpr int kTile = D == 256 ? 32 : 64, kGrain = 64;
-  static constexpr int kPerCu = 2;  // workgroups of a CU: 512 or 256 registers a lane
+  static constexpr int kLds = 2 * 2 * kTile * 2 * D;  // two stages; NonFinite comes after
 };
 
 template <class H, int D, Mode MODE>
-__global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnArgs a) {
+__device__ __forceinline__ void attend_many(const AttnArgs& a, int block, uint8_t* lds) {
   constexpr int KT = Many<D>::kTile, SUB = KT / 32, ROWB = 2 * D, STAGE = 2 * KT * ROWB;
   constexpr int CHUNKS = D / 8, RPC = 64 / CHUNKS, COPIES = KT * ROWB / 1024 / 4;  // copies of a wave, of K and of V
-  __shared__ __align__(1024) uint8_t lds[2 * STAGE + sizeof(NonFinite<D>)];  // one array, as above
-  NonFinite<D>& bad = *reinterpret_cast<NonFinite<D>*>(lds + 2 * STAGE);
+  NonFinite<D>& bad = *reinterpret_cast<NonFinite<D>*>(lds + Many<D>::kLds);
   init_non_finite(&bad, 256);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int head = blockIdx.x % a.kv_heads;
+  const int nth = (int)((uint32_t)block / (uint32_t)a.kv_heads), head = block - nth * a.kv_heads;
   // whole rows of keys at once: the last tiles, which see the most, come first
-  const int unit = MODE == kWhole ? a.p.own_units - 1 - (int)(blockIdx.x / a.kv_heads) : (int)(blockIdx.x / a.kv_heads);
+  const int unit = MODE == kWhole ? a.p.own_units - 1 - nth : nth;
   const int group = a.group, li = lane & 31, half = lane >> 5;
   if (MODE != kPrefix && unit == 0) zero_loose_tokens<D>(a, head, 256);
   Job found;
@@ -880,7 +876,7 @@ __global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnA
         lds_barrier();
       }
     }
-    if (wave * 32 < j.rows) {  // a wave without rows has its copies and its looking through alone
+    if (wave * 32 >= j.rows) continue;  // a wave without rows has its copies and its looking through alone
     const uint32_t kt = fresh(k_at) + stage;
     f32x16 s[SUB];
 #pragma unroll
@@ -962,7 +958,6 @@ __global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnA
       });
       p = next_p;
     });
-    }
   }
   sum += __shfl_xor(sum, 32);
   if (sum != sum) ref = sum;  // a NaN that no score set the reference for
@@ -1035,6 +1030,105 @@ __global__ __launch_bounds__(256, Many<D>::kPerCu) void attend_many_kernel(AttnA
 }
 
 // ---------------------------------------------------------------------------
+// The kernels: workgroups of 256 threads; registers for two waves a SIMD. One
+// LDS array each: with two, the compiler's wait for copies into the one before
+// reads of the other would empty the ring at every tile.
+// ---------------------------------------------------------------------------
+template <class H, int D>
+__global__ __launch_bounds__(256) void attend_few_kernel(AttnArgs a) {
+  __shared__ __align__(1024) uint8_t lds[Few<D>::kLds + sizeof(NonFinite<D>)];
+  attend_few<H, D, kOwn>(a, blockIdx.x, lds);
+}
+
+template <class H, int D, Mode MODE>
+__global__ __launch_bounds__(256, 2) void attend_many_kernel(AttnArgs a) {
+  __shared__ __align__(1024) uint8_t lds[Many<D>::kLds + sizeof(NonFinite<D>)];
+  attend_many<H, D, MODE>(a, blockIdx.x, lds);
+}
+
+// A decode batch with a prefix: shares of the prefix for all rows (the first
+// workgroups) and chunks of the sequences' own keys side by side.
+template <class H, int D, bool FEW_PREFIX>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_shared_kernel(AttnArgs a) {
+  constexpr int LDS = FEW_PREFIX || Few<D>::kLds > Many<D>::kLds ? Few<D>::kLds : Many<D>::kLds;
+  __shared__ __align__(1024) uint8_t lds[LDS + sizeof(NonFinite<D>)];
+  const int prefix_blocks = a.p.prefix_tiles * a.p.prefix_splits * a.kv_heads, block = (int)blockIdx.x;
+  if (block >= prefix_blocks) attend_few<H, D, kOwn>(a, block - prefix_blocks, lds);
+  else if (FEW_PREFIX) attend_few<H, D, kPrefix>(a, block, lds);
+  else attend_many<H, D, kPrefix>(a, block, lds);
+}
+
+// Joins a row's parts after attend_shared_kernel, the prefix's shares, then its
+// own chunks: one wave a (token, head), all of up to 16 parts in flight.
+template <class H, int D>
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
+  constexpr int PER = D / 64, AHEAD = 16;
+  const int lane = threadIdx.x & 63, id = (int)blockIdx.x * 4 + uniform(threadIdx.x >> 6);
+  if (id >= a.tokens * a.q_heads) return;
+  const int token = (int)((uint32_t)id / (uint32_t)a.q_heads), qh = id - token * a.q_heads;
+  const int head = (int)((uint32_t)qh / (uint32_t)a.group), g = qh - head * a.group;
+  // The last sequence that starts at or before the token: those after it hold no token.
+  int b = token;
+  if (a.starts) {
+    int count = 0;
+    for (int base = 0; base < a.batch; base += 64) {
+      const int c = __popcll(__ballot(base + lane < a.batch && start_of(a, min(base + lane, a.batch - 1)) <= token));
+      count += c;
+      if (c < 64) break;
+    }
+    b = uniform(count - 1);
+  }
+  uint16_t* to = a.out + (int64_t)id * D + lane * PER;
+  const Sequence s = sequence(a, max(b, 0));
+  const int r = (token - s.start) * a.group + g;
+  if (b < 0 || r >= s.n * a.group) {  // a token of no sequence
+#pragma unroll
+    for (int e = 0; e < PER; ++e) to[e] = 0;
+    return;
+  }
+  const int2 own = a.info[b];  // first unit, chunks of a tile
+  const int prows = a.p.few_prefix ? kFewRows : kManyRows, prow = token * a.group + g, n_pre = a.p.prefix_splits;
+  const int64_t pre0 = ((int64_t)(prow / prows) * n_pre * a.kv_heads + head) * prows + prow % prows;
+  const int64_t own0 = ((int64_t)(own.x + r / kFewRows * own.y) * a.kv_heads + head) * kFewRows + r % kFewRows;
+  const int n = n_pre + own.y;
+  const auto part = [&](int i) {
+    return i < n_pre ? pre0 + (int64_t)i * a.kv_heads * prows : own0 + (int64_t)(i - n_pre) * a.kv_heads * kFewRows;
+  };
+  float o[PER], top = -__builtin_inff(), total = 0.0f;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) o[e] = 0.0f;
+  for (int i = 0; i < n; i += AHEAD) {
+    float2 ml[AHEAD];
+    float x[AHEAD][PER];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int k = min(i + u, n - 1);
+      const int64_t at = part(k);
+      const float* from = (k < n_pre ? a.prefix_o : a.part_o) + at * D + lane * PER;
+      ml[u] = (k < n_pre ? a.prefix_ml : a.part_ml)[at];
+#pragma unroll
+      for (int e = 0; e < PER; ++e) x[u][e] = from[e];
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (i + u < n) {
+        const float2 f = join_factors(&top, ml[u].x);
+        total = joined(f, total, ml[u].y);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) o[e] = joined(f, o[e], x[u][e]);
+      }
+    }
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  if constexpr (PER == 1) {
+    to[0] = (uint16_t)H::pack(o[0] * inv, 0.0f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < PER; e += 2) reinterpret_cast<uint32_t*>(to)[e / 2] = H::pack(o[e] * inv, o[e + 1] * inv);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // The plan and the launches.
 // ---------------------------------------------------------------------------
 AttnPlan attention_plan(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t prefix_len,
@@ -1044,56 +1138,68 @@ AttnPlan attention_plan(int64_t tokens, int64_t batch, int64_t q_heads, int64_t 
   p.few_own = all_rows <= batch * kFewRows;
   const int64_t rows = p.few_own ? kFewRows : kManyRows;
   const int64_t tiles = !ragged && group <= rows ? batch : all_rows / rows + batch;
-  // workgroups that the CUs hold at a time: by their LDS, 2 of the many-row
-  // kernel, 4, 2 or 1 of the few-row kernel
-  const int64_t at_once = cus * (p.few_own ? 256 / dim : 2);
-  const int64_t want = std::max<int64_t>(1, at_once / kv_heads);
-  p.split = p.few_own || tiles < want;
-  // as many units as there are counters for
-  p.own_target = (int)std::max<int64_t>(1, std::min(want, kAttnCounters / kv_heads - tiles));
-  p.own_units = (int)(p.split ? p.own_target + tiles : tiles);
+  // units that the device holds at a time: by LDS, two workgroups a CU of the
+  // many-row kernel, 4, 2 or 1 of the few-row kernel
+  const int64_t at_once = cus * (p.few_own ? 256 / dim : 2) / kv_heads;
+  // Many-row tiles that fill the device stay whole. Otherwise the keys are cut
+  // for as many units as it holds, or for a second chunk of the longer
+  // sequences where the tiles alone come near that.
+  p.split = p.few_own || tiles < at_once;
+  p.own_units = (int)(p.split ? std::max<int64_t>(at_once, 2 * tiles) : tiles);
+  // more units than counters: nothing is split
+  if (p.split && p.own_units * kv_heads > kAttnCounters) p.own_units = (int)tiles;
   if (p.few_own && prefix_len > 0) {
     p.few_prefix = all_rows <= kFewRows;
     const int64_t prows = p.few_prefix ? kFewRows : kManyRows;
     p.prefix_tiles = (int)((all_rows + prows - 1) / prows);
-    p.prefix_splits = (int)std::max<int64_t>(1, std::min<int64_t>((cus / kv_heads + p.prefix_tiles - 1) / p.prefix_tiles, (prefix_len + 255) / 256));
+    // one workgroup a CU, of 256 keys at least: each writes its rows' results in 32 bits
+    const int64_t share = std::max<int64_t>(1, cus / (kv_heads * p.prefix_tiles));
+    p.prefix_splits = (int)std::min(share, (prefix_len + 255) / 256);
   }
   return p;
 }
 
 static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
-int64_t attention_workspace(const AttnPlan& p, int64_t kv_heads, int64_t dim) {
+// Bytes of a call's workspace; with `a`, its parts from `base` on.
+static int64_t carve(const AttnPlan& p, int64_t batch, int64_t kv_heads, int64_t dim, uint8_t* base, AttnArgs* a) {
   if (!p.split) return 0;
   const int64_t own = (int64_t)p.own_units * kv_heads * (p.few_own ? kFewRows : kManyRows);
   const int64_t pre = (int64_t)p.prefix_tiles * p.prefix_splits * kv_heads * (p.few_prefix ? kFewRows : kManyRows);
-  return up256(own * dim * 4) + up256(own * 8) + up256(pre * dim * 4) + up256(pre * 8);
+  const int64_t sizes[] = {own * dim * 4, own * 8, pre * dim * 4, pre * 8, pre ? batch * 8 : 0};
+  int64_t at[6] = {0};
+  for (int i = 0; i < 5; ++i) at[i + 1] = at[i] + up256(sizes[i]);
+  if (a) {
+    a->part_o = (float*)(base + at[0]), a->part_ml = (float2*)(base + at[1]);
+    a->prefix_o = (float*)(base + at[2]), a->prefix_ml = (float2*)(base + at[3]);
+    a->info = (int2*)(base + at[4]);
+  }
+  return at[5];
+}
+
+int64_t attention_workspace(const AttnPlan& p, int64_t batch, int64_t kv_heads, int64_t dim) {
+  return carve(p, batch, kv_heads, dim, nullptr, nullptr);
 }
 
 template <class H, int D>
 static void launch_attention(const AttnArgs& a, hipStream_t stream) {
   const AttnPlan& p = a.p;
-  if (p.prefix_tiles) {
-    const unsigned grid = (unsigned)(p.prefix_tiles * p.prefix_splits * a.kv_heads);
-    if (p.few_prefix) attend_few_kernel<H, D, kPrefix><<<grid, 64 * Few<D>::kWaves, 0, stream>>>(a);
-    else attend_many_kernel<H, D, kPrefix><<<grid, 256, 0, stream>>>(a);
+  const unsigned own = (unsigned)(p.own_units * a.kv_heads), pre = (unsigned)(p.prefix_tiles * p.prefix_splits * a.kv_heads);
+  if (pre) {
+    if (p.few_prefix) attend_shared_kernel<H, D, true><<<pre + own, 256, 0, stream>>>(a);
+    else attend_shared_kernel<H, D, false><<<pre + own, 256, 0, stream>>>(a);
+    join_kernel<H, D><<<(unsigned)((a.tokens * a.q_heads + 3) / 4), 256, 0, stream>>>(a);
+  } else if (p.few_own) {
+    attend_few_kernel<H, D><<<own, 256, 0, stream>>>(a);
+  } else if (p.split) {
+    attend_many_kernel<H, D, kSplit><<<own, 256, 0, stream>>>(a);
+  } else {
+    attend_many_kernel<H, D, kWhole><<<own, 256, 0, stream>>>(a);
   }
-  const unsigned grid = (unsigned)(p.own_units * a.kv_heads);
-  if (p.few_own) attend_few_kernel<H, D, kOwn><<<grid, 64 * Few<D>::kWaves, 0, stream>>>(a);
-  else if (p.split) attend_many_kernel<H, D, kSplit><<<grid, 256, 0, stream>>>(a);
-  else attend_many_kernel<H, D, kWhole><<<grid, 256, 0, stream>>>(a);
 }
 
 hipError_t paged_attention(AttnArgs a, int dim, bool fp16, void* workspace, hipStream_t stream) {
-  if (a.p.split) {
-    const int64_t own = (int64_t)a.p.own_units * a.kv_heads * (a.p.few_own ? kFewRows : kManyRows);
-    const int64_t pre = (int64_t)a.p.prefix_tiles * a.p.prefix_splits * a.kv_heads * (a.p.few_prefix ? kFewRows : kManyRows);
-    uint8_t* w = (uint8_t*)workspace;
-    a.part_o = (float*)w, w += up256(own * dim * 4);
-    a.part_ml = (float2*)w, w += up256(own * 8);
-    a.prefix_o = (float*)w, w += up256(pre * dim * 4);
-    a.prefix_ml = (float2*)w;
-  }
+  carve(a.p, a.batch, a.kv_heads, dim, (uint8_t*)workspace, &a);
   if (dim == 64) fp16 ? launch_attention<Fp16, 64>(a, stream) : launch_attention<Bf16, 64>(a, stream);
   else if (dim == 128) fp16 ? launch_attention<Fp16, 128>(a, stream) : launch_attention<Bf16, 128>(a, stream);
   else if (dim == 256) fp16 ? launch_attention<Fp16, 256>(a, stream) : launch_attention<Bf16, 256>(a, stream);

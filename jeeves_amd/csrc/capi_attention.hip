@@ -123,8 +123,8 @@ int64_t jv_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_
   if (tokens == 0 || batch == 0) return 0;
   const int cus = jv::cu_count_of(-1);
   if (cus <= 0) return -1;
-  return jv::attention_workspace(jv::attention_plan(tokens, batch, q_heads, kv_heads, dim, prefix_len, ragged != 0, cus), kv_heads,
-                                 dim);
+  return jv::attention_workspace(jv::attention_plan(tokens, batch, q_heads, kv_heads, dim, prefix_len, ragged != 0, cus), batch,
+                                 kv_heads, dim);
 }
 
 int jv_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k_pages, const void* v_pages, int64_t pages,
@@ -152,11 +152,13 @@ int jv_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k_
   if (cus <= 0) return fail(JV_ERR_HIP, "cannot query the device's compute units");
   jv::AttnArgs a{};
   a.p = jv::attention_plan(tokens, batch, q_heads, kv_heads, dim, prefix_len, starts != nullptr, cus);
-  const int64_t need = jv::attention_workspace(a.p, kv_heads, dim);
+  const int64_t need = jv::attention_workspace(a.p, batch, kv_heads, dim);
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
     return fail(JV_ERR_VALUE, "workspace needs %lld bytes, 256-byte aligned", (long long)need);
-  if (a.p.split && (!counters || n_counters < (int64_t)a.p.own_units * kv_heads))
-    return fail(JV_ERR_VALUE, "%lld units exceed the %lld counters", (long long)a.p.own_units * kv_heads, (long long)n_counters);
+  // more units than counters are not split (attention_plan)
+  const int64_t units = (int64_t)a.p.own_units * kv_heads;
+  if (a.p.split && units <= JV_ATTENTION_COUNTERS && (!counters || n_counters < units))
+    return fail(JV_ERR_VALUE, "%lld units exceed the %lld counters", (long long)units, (long long)n_counters);
   a.counters = counters;
   a.q = (const uint16_t*)q, a.q_ts = q_ts, a.q_hs = q_hs;
   a.k_pages = (const uint16_t*)k_pages, a.v_pages = (const uint16_t*)v_pages;
