@@ -107,6 +107,7 @@ constexpr int64_t kAttnCounters = 65536;
 struct AttnPlan {
   bool few_own, few_prefix;  // tiles of kFewRows rows instead of kManyRows
   bool split;                // the keys of a row tile may go to several workgroups
+  int cu_units;              // workgroups of a head that come to the device's CUs first, one a CU
   int own_units;             // tile slots, or with a split the most units (tile, key chunk) that there can be
   int prefix_tiles, prefix_splits;  // where the prefix is gone through apart, for all tokens' rows
 };

@@ -783,6 +783,15 @@ struct Many {
   static constexpr int kLds = 2 * 2 * kTile * 2 * D;  // two stages; NonFinite comes after
 };
 
+// The tile of the nth workgroups of whole tiles. The last tiles, which see the
+// most keys, come first; of the workgroups that come to a CU second, though,
+// those of the fewest keys, so that a long and a short tile share a CU.
+__device__ __forceinline__ int whole_unit(const AttnPlan& p, int nth) {
+  const int both = min(p.own_units, 2 * p.cu_units);
+  if (nth >= p.cu_units && nth < both) nth = p.cu_units + both - 1 - nth;
+  return p.own_units - 1 - nth;
+}
+
 template <class H, int D, Mode MODE>
 __device__ __forceinline__ void attend_many(const AttnArgs& a, int block, uint8_t* lds) {
   constexpr int KT = Many<D>::kTile, SUB = KT / 32, ROWB = 2 * D, STAGE = 2 * KT * ROWB;
@@ -791,8 +800,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a, int block, uint8_
   init_non_finite(&bad, 256);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nth = (int)((uint32_t)block / (uint32_t)a.kv_heads), head = block - nth * a.kv_heads;
-  // whole rows of keys at once: the last tiles, which see the most, come first
-  const int unit = MODE == kWhole ? a.p.own_units - 1 - nth : nth;
+  const int unit = MODE == kWhole ? whole_unit(a.p, nth) : nth;
   const int group = a.group, li = lane & 31, half = lane >> 5;
   if (MODE != kPrefix && unit == 0) zero_loose_tokens<D>(a, head, 256);
   Job found;
@@ -1145,6 +1153,7 @@ AttnPlan attention_plan(int64_t tokens, int64_t batch, int64_t q_heads, int64_t 
   // for as many units as it holds, or for a second chunk of the longer
   // sequences where the tiles alone come near that.
   p.split = p.few_own || tiles < at_once;
+  p.cu_units = (int)(cus / kv_heads);
   p.own_units = (int)(p.split ? std::max<int64_t>(at_once, 2 * tiles) : tiles);
   // more units than counters: nothing is split
   if (p.split && p.own_units * kv_heads > kAttnCounters) p.own_units = (int)tiles;
