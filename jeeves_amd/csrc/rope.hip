@@ -7,11 +7,16 @@
 // z_{i + rotary/2} = y_{i + rotary/2} cos t_i + y_i sin t_i; the channels from
 // `rotary` on stay y. All of it in fp32, rounded once when z is stored.
 //
-// The rows are read and written once, so HBM bounds it. A group of dim / 8
-// lanes holds a row, 16 bytes a lane; the rotation's partner channels come
-// from another lane of the group, and a group takes up to HB heads of one
-// token in turn, with the token's angles and the head weights in registers
-// (they would be eight of the nine loads of every 16 bytes otherwise).
+// The rows are read and written once, so HBM bounds it: 7921 tokens of 40 heads
+// of 128 take 35 us, 4.7 TB/s of the 4.9 that a copy reaches; few tokens take
+// the 3 us of a launch and its two dependent loads. A group of dim / 8 lanes
+// holds a row, 16 bytes a lane; the rotation's partner channels come from
+// another lane of the group. A group takes kHeads heads of one token, with the
+// token's angles and the head weights in registers (they would be eight of the
+// nine loads of every 16 bytes otherwise). Two heads: with one those 7921 tokens
+// take 41 us and the append of 4096 tokens of 4 heads of 256 10.6 us; with two
+// 35.4 and 9.8; with four, which leave the device fewer waves, 34.6 and 11.3,
+// and 7.5 instead of 7.3 us for 800 tokens.
 #include "attention.h"
 
 namespace jv {
@@ -20,23 +25,25 @@ __device__ __forceinline__ int64_t load_index(const void* p, int wide, int i) {
   return wide ? reinterpret_cast<const int64_t*>(p)[i] : (int64_t)reinterpret_cast<const int32_t*>(p)[i];
 }
 
-template <class H, int D, int HB>
+constexpr int kHeads = 2;
+
+template <class H, int D>
 __global__ __launch_bounds__(256) void norm_rope_kernel(RopeArgs a, uint32_t q_blocks, uint32_t kv_blocks, uint32_t per_token,
                                                         uint32_t tasks) {
   constexpr int LPH = D / 8;  // lanes of a head
-  const uint32_t task = (blockIdx.x * 256 + threadIdx.x) / LPH;
+  const uint32_t task = blockIdx.x * (256 / LPH) + threadIdx.x / LPH;
   if (task >= tasks) return;
   const int token = (int)(task / per_token);
   const uint32_t j = task % per_token;
   const int c = threadIdx.x % LPH;  // this lane's 8 channels: 8 c ..
   const bool is_q = j < q_blocks, is_v = j >= q_blocks + kv_blocks;
-  const int h0 = (int)(is_q ? j : is_v ? j - q_blocks - kv_blocks : j - q_blocks) * HB;
+  const int h0 = (int)(is_q ? j : is_v ? j - q_blocks - kv_blocks : j - q_blocks) * kHeads;
   const int heads = is_q ? a.q_heads : a.kv_heads;
   const uint16_t* src = is_q ? a.q + token * a.q_ts : is_v ? a.v + token * a.v_ts : a.k + token * a.k_ts;
   const int64_t hs = is_q ? a.q_hs : is_v ? a.v_hs : a.k_hs;
-  uint4 x[HB];
+  uint4 x[kHeads];
 #pragma unroll
-  for (int i = 0; i < HB; ++i) x[i] = *reinterpret_cast<const uint4*>(src + min(h0 + i, heads - 1) * hs + c * 8);
+  for (int i = 0; i < kHeads; ++i) x[i] = *reinterpret_cast<const uint4*>(src + min(h0 + i, heads - 1) * hs + c * 8);
 
   // Where the row goes: q and k rows to their outputs, or k and v to a slot.
   uint16_t* dst;
@@ -78,7 +85,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(RopeArgs a, uint32_t q_b
       }
     }
 #pragma unroll
-    for (int i = 0; i < HB; ++i) {
+    for (int i = 0; i < kHeads; ++i) {
       const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
       float f[8], g[8];
 #pragma unroll
@@ -112,22 +119,16 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(RopeArgs a, uint32_t q_b
     }
   }
 #pragma unroll
-  for (int i = 0; i < HB; ++i)
+  for (int i = 0; i < kHeads; ++i)
     if (keep && h0 + i < heads) *reinterpret_cast<uint4*>(dst + (h0 + i) * dst_hs) = x[i];
 }
 
 template <class H, int D>
 static void launch_norm_rope(const RopeArgs& a, hipStream_t stream) {
-  const auto blocks = [](int heads, int hb) { return (uint32_t)((heads + hb - 1) / hb); };
-  const auto go = [&](auto kernel, int hb) {
-    const uint32_t qb = a.q ? blocks(a.q_heads, hb) : 0, kb = blocks(a.kv_heads, hb), per = qb + kb + (a.v ? kb : 0);
-    const uint32_t tasks = per * (uint32_t)a.tokens, groups = 256 / (D / 8);
-    kernel<<<(tasks + groups - 1) / groups, 256, 0, stream>>>(a, qb, kb, per, tasks);
-  };
-  if ((int64_t)a.tokens * (a.q_heads + a.kv_heads) >= 16384)
-    go(norm_rope_kernel<H, D, 4>, 4);
-  else
-    go(norm_rope_kernel<H, D, 1>, 1);
+  const auto blocks = [](int heads) { return (uint32_t)((heads + kHeads - 1) / kHeads); };
+  const uint32_t qb = a.q ? blocks(a.q_heads) : 0, kb = blocks(a.kv_heads), per = qb + kb + (a.v ? kb : 0);
+  const uint32_t tasks = per * (uint32_t)a.tokens, groups = 256 / (D / 8);
+  norm_rope_kernel<H, D><<<(tasks + groups - 1) / groups, 256, 0, stream>>>(a, qb, kb, per, tasks);
 }
 
 hipError_t norm_rope(const RopeArgs& a, int dim, bool fp16, hipStream_t stream) {
