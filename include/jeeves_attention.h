@@ -13,7 +13,8 @@
  * (`hs`), unit stride over dim and 16-byte aligned rows; dim is 64, 128 or 256.
  * The cache is two contiguous arrays [pages, kv_heads, page_size, dim], the
  * page size a power of two from 16 to 1024. Token `offset` of page `page` is
- * slot page * page_size + offset.
+ * slot page * page_size + offset. A call takes less than 2^28 rows (tokens times
+ * heads of q, k and v) and queries that can see up to 2^30 keys.
  */
 #ifndef JEEVES_ATTENTION_H
 #define JEEVES_ATTENTION_H

@@ -101,12 +101,13 @@ hipError_t norm_rope(const RopeArgs& a, int dim, bool fp16, hipStream_t stream);
 // token and sequence counts alone while the starts stay on the device.
 constexpr int kFewRows = 16, kManyRows = 128;
 
-// Counters a call may use at most; where they do not suffice no keys are split.
+// Counters a call may use at most; keys that would need more are not split.
 constexpr int64_t kAttnCounters = 65536;
 
 struct AttnPlan {
   bool few_own, few_prefix;  // tiles of kFewRows rows instead of kManyRows
   bool split;                // the keys of a row tile may go to several workgroups
+  int tiles;                 // at least the batch's row tiles
   int cu_units;              // workgroups of a head that come to the device's CUs first, one a CU
   int own_units;             // tile slots, or with a split the most units (tile, key chunk) that there can be
   int prefix_tiles, prefix_splits;  // where the prefix is gone through apart, for all tokens' rows

@@ -248,11 +248,14 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int rows,
     const int tiles = (int)((uint32_t)(s.n * a.group + rows - 1) / (uint32_t)rows);
     if (i < steps) {
       groups += lane_value(wave_scan(tiles * ((shared + s.len + 15) >> 4)), 63);
-      all_tiles += lane_value(wave_scan(tiles), 63);
-      if (i + 1 == steps) keys = uniform(chunk_keys(groups, all_tiles, a.p.own_units, grain));
+      all_tiles = min(all_tiles + lane_value(wave_scan(tiles), 63), (1 << 30) - 1);
+      if (i + 1 == steps) {
+        if (all_tiles > a.p.tiles) return false;  // starts that decrease
+        keys = uniform(chunk_keys(groups, all_tiles, a.p.own_units, grain));
+      }
       continue;
     }
-    const int chunks = max(1, (int)((uint32_t)(shared + s.len + keys - 1) / (uint32_t)keys)), n = tiles * chunks;
+    const int chunks = a.p.split ? max(1, (int)((uint32_t)(shared + s.len + keys - 1) / (uint32_t)keys)) : 1, n = tiles * chunks;
     const int upto = wave_scan(n);
     const uint64_t past = __ballot(before + upto > unit);
     if (past) {
@@ -1089,7 +1092,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
   uint16_t* to = a.out + (int64_t)id * D + lane * PER;
   const Sequence s = sequence(a, max(b, 0));
   const int r = (token - s.start) * a.group + g;
-  if (b < 0 || r >= s.n * a.group) {  // a token of no sequence
+  if (b < 0 || (uint32_t)r >= (uint32_t)(s.n * a.group)) {  // a token of no sequence
 #pragma unroll
     for (int e = 0; e < PER; ++e) to[e] = 0;
     return;
@@ -1097,10 +1100,12 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
   const int2 own = a.info[b];  // first unit, chunks of a tile
   const int prows = a.p.few_prefix ? kFewRows : kManyRows, prow = token * a.group + g, n_pre = a.p.prefix_splits;
   const int64_t pre0 = ((int64_t)(prow / prows) * n_pre * a.kv_heads + head) * prows + prow % prows;
-  const int64_t own0 = ((int64_t)(own.x + r / kFewRows * own.y) * a.kv_heads + head) * kFewRows + r % kFewRows;
-  const int n = n_pre + own.y;
+  // held in range: starts that decrease leave sequences without units
+  const int own0 = own.x + r / kFewRows * own.y, n = n_pre + clamped(own.y, 1, a.p.own_units);
   const auto part = [&](int i) {
-    return i < n_pre ? pre0 + (int64_t)i * a.kv_heads * prows : own0 + (int64_t)(i - n_pre) * a.kv_heads * kFewRows;
+    if (i < n_pre) return pre0 + (int64_t)i * a.kv_heads * prows;
+    const int unit = clamped(own0 + i - n_pre, 0, a.p.own_units - 1);
+    return ((int64_t)unit * a.kv_heads + head) * kFewRows + r % kFewRows;
   };
   float o[PER], top = -__builtin_inff(), total = 0.0f;
 #pragma unroll
@@ -1154,9 +1159,11 @@ AttnPlan attention_plan(int64_t tokens, int64_t batch, int64_t q_heads, int64_t 
   // sequences where the tiles alone come near that.
   p.split = p.few_own || tiles < at_once;
   p.cu_units = (int)(cus / kv_heads);
+  p.tiles = (int)tiles;
   p.own_units = (int)(p.split ? std::max<int64_t>(at_once, 2 * tiles) : tiles);
-  // more units than counters: nothing is split
-  if (p.split && p.own_units * kv_heads > kAttnCounters) p.own_units = (int)tiles;
+  // chunks that are not joined in a launch of their own are counted in
+  const bool counted = p.split && !(p.few_own && prefix_len > 0);
+  if (counted && p.own_units * kv_heads > kAttnCounters) p.split = false, p.own_units = (int)tiles;
   if (p.few_own && prefix_len > 0) {
     p.few_prefix = all_rows <= kFewRows;
     const int64_t prows = p.few_prefix ? kFewRows : kManyRows;
@@ -1172,8 +1179,8 @@ static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
 // Bytes of a call's workspace; with `a`, its parts from `base` on.
 static int64_t carve(const AttnPlan& p, int64_t batch, int64_t kv_heads, int64_t dim, uint8_t* base, AttnArgs* a) {
-  if (!p.split) return 0;
-  const int64_t own = (int64_t)p.own_units * kv_heads * (p.few_own ? kFewRows : kManyRows);
+  const bool parts = p.split || p.prefix_tiles;
+  const int64_t own = parts ? (int64_t)p.own_units * kv_heads * (p.few_own ? kFewRows : kManyRows) : 0;
   const int64_t pre = (int64_t)p.prefix_tiles * p.prefix_splits * kv_heads * (p.few_prefix ? kFewRows : kManyRows);
   const int64_t sizes[] = {own * dim * 4, own * 8, pre * dim * 4, pre * 8, pre ? batch * 8 : 0};
   int64_t at[6] = {0};
@@ -1198,7 +1205,7 @@ static void launch_attention(const AttnArgs& a, hipStream_t stream) {
     if (p.few_prefix) attend_shared_kernel<H, D, true><<<pre + own, 256, 0, stream>>>(a);
     else attend_shared_kernel<H, D, false><<<pre + own, 256, 0, stream>>>(a);
     join_kernel<H, D><<<(unsigned)((a.tokens * a.q_heads + 3) / 4), 256, 0, stream>>>(a);
-  } else if (p.few_own) {
+  } else if (p.few_own) {  // also where not split: a chunk a tile
     attend_few_kernel<H, D><<<own, 256, 0, stream>>>(a);
   } else if (p.split) {
     attend_many_kernel<H, D, kSplit><<<own, 256, 0, stream>>>(a);

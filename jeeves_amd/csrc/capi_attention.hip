@@ -13,10 +13,15 @@ using jv::hip_status;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// Rows of a call: its grids then stay below 2^24 workgroups of 256 threads.
+constexpr int64_t kMaxRows = (int64_t(1) << 28) - 1;
+// Keys that a query can see.
+constexpr int64_t kMaxKeys = int64_t(1) << 30;
+
 int check_heads(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t dim) {
   if (dim != 64 && dim != 128 && dim != 256) return fail(JV_ERR_VALUE, "heads of 64, 128 or 256 channels, got %lld", (long long)dim);
   if (tokens < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads > 65536 || kv_heads > 65536 ||
-      tokens > INT32_MAX / (q_heads + 2 * kv_heads))
+      tokens > kMaxRows / (q_heads + 2 * kv_heads))
     return fail(JV_ERR_VALUE, "bad sizes: %lld tokens, %lld query heads, %lld key heads", (long long)tokens, (long long)q_heads,
                 (long long)kv_heads);
   return JV_OK;
@@ -139,7 +144,7 @@ int jv_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k_
   if (!starts && tokens != batch)
     return fail(JV_ERR_VALUE, "without query starts each of the %lld sequences has one token, got %lld", (long long)batch,
                 (long long)tokens);
-  if (table_cols < 0 || table_stride < 0 || table_cols > INT32_MAX / page_size ||
+  if (table_cols < 0 || table_stride < 0 || table_cols > kMaxKeys / page_size || table_cols * page_size + prefix_len > kMaxKeys ||
       (batch + tokens * (q_heads / kv_heads) / 16) * ((table_cols * page_size + prefix_len) / 16 + 1) > INT32_MAX)
     return fail(JV_ERR_VALUE, "page table of %lld columns for a batch of %lld is too large", (long long)table_cols, (long long)batch);
   if (tokens == 0) return JV_OK;
@@ -155,9 +160,10 @@ int jv_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k_
   const int64_t need = jv::attention_workspace(a.p, batch, kv_heads, dim);
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
     return fail(JV_ERR_VALUE, "workspace needs %lld bytes, 256-byte aligned", (long long)need);
-  // more units than counters are not split (attention_plan)
-  const int64_t units = (int64_t)a.p.own_units * kv_heads;
-  if (a.p.split && units <= JV_ATTENTION_COUNTERS && (!counters || n_counters < units))
+  const int64_t units = (int64_t)a.p.own_units * kv_heads, shares = (int64_t)a.p.prefix_tiles * a.p.prefix_splits * kv_heads;
+  if (units + shares >= int64_t(1) << 24 || (shares && tokens * q_heads >= int64_t(1) << 26))
+    return fail(JV_ERR_VALUE, "too many rows for one call: %lld tokens, %lld heads", (long long)tokens, (long long)q_heads);
+  if (a.p.split && !shares && (!counters || n_counters < units))
     return fail(JV_ERR_VALUE, "%lld units exceed the %lld counters", (long long)units, (long long)n_counters);
   a.counters = counters;
   a.q = (const uint16_t*)q, a.q_ts = q_ts, a.q_hs = q_hs;

@@ -84,7 +84,7 @@ def test_norm_rope(dim, rotary, tokens, dtype):
 
 
 def test_norm_rope_many_heads_take_the_blocked_form():
-    """Enough rows for four heads a lane group, head counts that are no multiple of four."""
+    """Many rows, and odd head counts: a lane group takes two heads."""
     from jeeves_amd.attention import qk_norm_rope, rope_table
 
     g = gen(5)
@@ -267,6 +267,56 @@ def test_decode_long_keys_split_over_workgroups(dim, batch, length):
 def test_decode_large_ragged_batch():
     rng = random.Random(3)
     Batch(3, [round(math.exp(rng.uniform(0, math.log(900)))) for _ in range(150)], heads=(4, 1), dim=64).check()
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("prefix", [0, 37])
+def test_more_units_than_counters(ragged, prefix):
+    """Twice the row tiles of all heads pass the stream's counters: no keys are
+    split (with starts the tiles' bound is above their number, which must not
+    leave room for a split either), unless a launch of its own joins them."""
+    from jeeves_amd.attention import paged_attention
+
+    g = gen(23)
+    batch, heads, dim, page = 9001, 8, 64, 16
+    cache = new_cache(g, 700, heads, page, dim)
+    lengths = torch.randint(0, 49, (batch,), generator=g, device=DEV, dtype=torch.int32)
+    lengths[::50] = 300
+    table = torch.randint(0, 700, (batch, 19), generator=g, device=DEV, dtype=torch.int32)
+    shared = torch.randint(0, 700, (3,), generator=g, device=DEV, dtype=torch.int32)
+    q = randn(g, batch, heads, dim)
+    starts = torch.arange(batch + 1, device=DEV, dtype=torch.int32) if ragged else None
+
+    def run():
+        return paged_attention(q, cache, table, lengths, query_starts=starts, prefix_pages=shared if prefix else None,
+                               prefix_length=prefix)
+
+    out = run()
+    assert torch.equal(out, run())
+    for first in range(0, batch, 500):
+        ids = torch.cat([shared[None].expand(batch, -1), table], 1)[first:first + 500].long()
+        at = torch.arange(ids.shape[1] * page, device=DEV)
+        seen = (at[None] < prefix) | ((at[None] >= 48) & (at[None] - 48 < lengths[first:first + 500, None]))
+        k, v = (x[ids].permute(0, 2, 1, 3, 4).reshape(ids.shape[0], heads, -1, dim).double() for x in (cache.k, cache.v))
+        score = (k @ q[first:first + 500].double()[..., None])[..., 0] * dim ** -0.5
+        p = torch.softmax(score.masked_fill(~seen[:, None], -math.inf), -1).nan_to_num(0.0)[..., None, :]
+        exact, mag = (p @ v)[..., 0, :], (p @ v.abs())[..., 0, :]
+        err = (out[first:first + 500].double() - exact).abs()
+        assert (err <= 2 * 2.0 ** -9 * (exact.abs() + mag) + 2.0 ** -14 * mag).all()
+
+
+@pytest.mark.parametrize("prefix", [0, 100])
+@pytest.mark.parametrize("queries", [[1, 1, 1, 1], [200, 100, 300, 50]])
+def test_starts_that_decrease_leave_later_calls_right(queries, prefix):
+    """Outside the contract: whatever comes out, the next call's bits are the same."""
+    b = Batch(25, [700, 800, 900, 600], queries, prefix=prefix)
+    good, starts = b.check(), b.starts
+    n = sum(queries)
+    for bad in ([0, n, 0, n, n], [n, n - 1, 2, 1, 0], [-5, 2 ** 30, -7, n, 1], [0, n, n, 0, n]):
+        b.starts = torch.tensor(bad, dtype=torch.int32, device=DEV)
+        assert b.run().shape == b.q.shape
+    b.starts = starts
+    assert torch.equal(b.run(), good)
 
 
 @pytest.mark.parametrize("heads", [(16, 1), (17, 1), (32, 1), (64, 2)])
