@@ -216,56 +216,94 @@ __device__ __forceinline__ float wave_sum_f32(float v) {
 }
 
 // Where keys are split over workgroups: the (sequence, row tile, key chunk) of
-// a unit. The tiles' keys are added up (in groups of 16, which the host has
-// checked to fit 32 bits), the sum cut into up to `own_units` chunks, and each
-// tile of a sequence gets one unit for each chunk's worth of keys that its
-// sequence has begun, one at least, with equal shares of what it sees. `shared`:
-// keys before the own ones that count too. Computed by each wave for itself,
-// 64 sequences a step, from the lengths on the device.
+// a unit, computed by each wave for itself, 64 sequences a step, from the
+// lengths on the device. `shared`: keys before the own ones that count too.
+//
+// Keys are counted in steps of 16, or of the keys by which a row tile sees more
+// than the one before it. A tile that sees at most x + 1 steps is cut into
+// 1 + x / m chunks of equal shares. m, of CHUNK keys at least, is chosen so that
+// the chunks of all tiles, the units, fit `own_units`: with W the sum of the x, W / (own_units - tiles) + 1
+// does, as each tile begins one chunk more than its share.
+//
+// Tiles of few rows are cut alike within a sequence (what its last tile sees is
+// taken for all). Of many rows, tile t of a sequence has x = a + t, so that a
+// prompt's early tiles, which see little, are cut less, and up to 64 sequences
+// take the least of eight m from W / own_units on that fits.
 struct Unit {
-  int b, first, tile, chunk, chunks;  // sequence, its first unit, row tile and chunk of the unit, chunks of a tile
+  int b, tile, chunk, chunks;  // sequence, row tile and chunk of the unit, chunks of the tile
   Sequence seq;
 };
-// Keys of a chunk: each tile may begin one chunk more than its share of the
-// target, so the tiles are taken off it and the units never pass it.
-__device__ __forceinline__ int chunk_keys(int groups, int tiles, int target, int grain) {
-  const int each = (int)((uint32_t)groups / (uint32_t)max(1, target - tiles)) * 16 + 16;
-  return max(2 * grain, (each + grain - 1) / grain * grain);
+// Sum of i / m over the i below x, modulo 2^32.
+__device__ __forceinline__ uint32_t sum_below(uint32_t x, uint32_t m) {
+  const uint32_t q = x / m;
+  return m * (q * (q - 1) / 2) + q * (x - q * m);
 }
 // False if there is no such unit.
-__device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int rows, int grain, int shared, Unit* u) {
-  const int lane = threadIdx.x & 63, steps = (a.batch + 63) >> 6;
-  int groups = 0, all_tiles = 0, before = 0, keys = 0;
+template <int ROWS, int CHUNK>
+__device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int shared, Unit* u) {
+  constexpr bool MANY = ROWS == kManyRows;
+  const int lane = threadIdx.x & 63, batches = (a.batch + 63) >> 6, most = a.p.own_units;
+  const uint32_t step = MANY ? max(16u, (uint32_t)(ROWS + a.group - 1) / (uint32_t)a.group) : 16;
+  uint32_t weight = 0, m = 1;
+  int all_tiles = 0, before = 0;
   Sequence s;
-  // `steps` steps to add the keys up, `steps` more to find the unit; up to 64
-  // sequences are read once
-  for (int i = 0; i < 2 * steps; ++i) {
-    const int base = (i < steps ? i : i - steps) * 64;
-    if (i == 0 || steps > 1) {
+  // `batches` times to add the keys up, as often again to find the unit; up to
+  // 64 sequences are read once
+  for (int i = 0; i < 2 * batches; ++i) {
+    const int base = (i < batches ? i : i - batches) * 64;
+    if (i == 0 || batches > 1) {
       s = sequence(a, min(base + lane, a.batch - 1));
       if (base + lane >= a.batch) s.n = 0;
     }
-    const int tiles = (int)((uint32_t)(s.n * a.group + rows - 1) / (uint32_t)rows);
-    if (i < steps) {
-      groups += lane_value(wave_scan(tiles * ((shared + s.len + 15) >> 4)), 63);
-      all_tiles = min(all_tiles + lane_value(wave_scan(tiles), 63), (1 << 30) - 1);
-      if (i + 1 == steps) {
-        if (all_tiles > a.p.tiles) return false;  // starts that decrease
-        keys = uniform(chunk_keys(groups, all_tiles, a.p.own_units, grain));
+    const uint32_t tiles = (uint32_t)(s.n * a.group + ROWS - 1) / (uint32_t)ROWS;
+    // x of the first tile, or of all
+    const uint32_t x = MANY ? ((uint32_t)(shared + max(0, s.len - s.n)) + step - 1) / step : (uint32_t)max(shared + s.len - 1, 0) / step;
+    const auto units = [&](uint32_t m) {
+      return (int)(MANY ? tiles + sum_below(x + tiles, m) - sum_below(x, m) : a.p.split ? tiles * (1 + x / m) : tiles);
+    };
+    if (i < batches) {
+      weight += (uint32_t)lane_value(wave_scan((int)(tiles * x + (MANY ? tiles * (tiles - 1) / 2 : 0))), 63);
+      all_tiles = min(all_tiles + lane_value(wave_scan((int)tiles), 63), (1 << 30) - 1);
+      if (i + 1 < batches) continue;
+      if (all_tiles > a.p.tiles) return false;  // starts that decrease
+      const uint32_t least = (CHUNK + step - 1) / step;
+      m = max(least, weight / (uint32_t)max(1, most - all_tiles) + 1);
+      if (MANY && batches == 1) {
+        const uint32_t low = max(least, weight / (uint32_t)most + 1), each = (m - low + 6) / 7;
+        for (uint32_t t = low; t < m; t += each) {
+          if (lane_value(wave_scan(units(t)), 63) <= most) m = t;
+        }
       }
+      m = (uint32_t)uniform((int)m);
       continue;
     }
-    const int chunks = a.p.split ? max(1, (int)((uint32_t)(shared + s.len + keys - 1) / (uint32_t)keys)) : 1, n = tiles * chunks;
+    const int n = units(m);
     const int upto = wave_scan(n);
     const uint64_t past = __ballot(before + upto > unit);
     if (past) {
       const int l = uniform(__ffsll((unsigned long long)past) - 1);
+      const int of = unit - (before + lane_value(upto, l) - lane_value(n, l));  // the sequence's
+      const int its_tiles = lane_value((int)tiles, l);
+      const uint32_t its_x = (uint32_t)lane_value((int)x, l);
       u->b = base + l;
-      u->first = before + lane_value(upto, l) - lane_value(n, l);
-      u->chunks = lane_value(chunks, l);
-      u->tile = uniform((int)((uint32_t)(unit - u->first) / (uint32_t)u->chunks));
-      u->chunk = unit - u->first - u->tile * u->chunks;
       u->seq = Sequence{lane_value(s.start, l), lane_value(s.n, l), lane_value(s.len, l)};
+      if (!MANY) {
+        u->chunks = a.p.split ? uniform((int)(1 + its_x / m)) : 1;
+        u->tile = uniform((int)((uint32_t)of / (uint32_t)u->chunks));
+        u->chunk = of - u->tile * u->chunks;
+        return true;
+      }
+      // the last tile whose units begin at or before this one, 64 tiles a step
+      u->tile = 0, u->chunk = of;
+      const uint32_t sum0 = sum_below(its_x, m);
+      for (int t0 = 0; t0 < its_tiles; t0 += 64) {
+        const int t = t0 + lane, begins = t + (int)(sum_below(its_x + (uint32_t)t, m) - sum0);
+        const int count = __popcll(__ballot(t < its_tiles && begins <= of));
+        if (count == 0) break;
+        u->tile = t0 + count - 1, u->chunk = of - lane_value(begins, count - 1);
+        if (count < 64) break;
+      }
+      u->chunks = uniform((int)(1 + (its_x + (uint32_t)u->tile) / m));
       return true;
     }
     before += lane_value(upto, 63);
@@ -301,7 +339,7 @@ struct Job {
 enum Mode { kWhole, kSplit, kOwn, kPrefix };
 
 // Fills a job from the block index; false if the block has nothing to do.
-template <Mode MODE, int ROWS, int KT, int GRAIN>
+template <Mode MODE, int ROWS, int KT, int GRAIN, int CHUNK>
 __device__ __forceinline__ bool find_job(const AttnArgs& a, int unit, Job* j) {
   j->prefix = j->own = Keys{a.prefix_pages, 0, -1};
   j->sequence = 0, j->first = unit, j->chunk = 0, j->chunks = 1;
@@ -329,7 +367,7 @@ __device__ __forceinline__ bool find_job(const AttnArgs& a, int unit, Job* j) {
     if (j->row0 < 0) return false;
   } else {
     Unit u;
-    if (!find_unit(a, unit, ROWS, GRAIN, shared, &u)) return false;
+    if (!find_unit<ROWS, CHUNK>(a, unit, shared, &u)) return false;
     s = Sequence{uniform(u.seq.start), uniform(u.seq.n), uniform(u.seq.len)};
     b = uniform(u.b), j->chunk = uniform(u.chunk), j->chunks = uniform(u.chunks);
     j->row0 = uniform(u.tile) * ROWS;
@@ -538,7 +576,7 @@ struct Joined {
 
 template <int D>
 struct Few {
-  static constexpr int kWaves = 4, kTile = 16, kStage = 2 * kTile * 2 * D, kGrain = kTile * kWaves;
+  static constexpr int kWaves = 4, kTile = 16, kStage = 2 * kTile * 2 * D, kGrain = kTile * kWaves, kChunk = 2 * kGrain;
   static constexpr int kRings = kWaves * 2 * kStage, kMerge = kWaves * kFewRows * (D + 2) * 4 + 64 * kWaves * 24;
   static constexpr int kLds = kRings > kMerge ? kRings : kMerge;  // NonFinite comes after
 };
@@ -553,7 +591,7 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a, int block, uint8_t
   const int unit = (int)((uint32_t)block / (uint32_t)a.kv_heads), head = block - unit * a.kv_heads;
   if (MODE == kOwn && unit == 0) zero_loose_tokens<D>(a, head, 64 * W);
   Job found;
-  if (!find_job<MODE, kFewRows, KT, Few<D>::kGrain>(a, unit, &found)) return;
+  if (!find_job<MODE, kFewRows, KT, Few<D>::kGrain, Few<D>::kChunk>(a, unit, &found)) return;
   const Job j = uniform(found);
   constexpr bool PREFIX = MODE == kPrefix;
   const Keys run = PREFIX ? j.prefix : j.own;
@@ -782,7 +820,12 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a, int block, uint8_t
 // ---------------------------------------------------------------------------
 template <int D>
 struct Many {
-  static constexpr int kTile = D == 256 ? 32 : 64, kGrain = 64;
+  // A chunk's partial results, 4 D bytes a row, have to be worth its keys. With
+  // 256, 384, 640 and 896 keys at least: 64 queries of 32 heads over 4000 keys
+  // 33, 29, 29 and 31 us; 4 sequences of 200 queries of 16 heads of 256 over 1000
+  // keys 55, 52, 44 and 44; prompts of 1024 tokens of those heads 46, 37, 39 and
+  // 46, of 1500 tokens of 32 heads of 128 51, 51, 48 and 46.
+  static constexpr int kTile = D == 256 ? 32 : 64, kGrain = 64, kChunk = 640;
   static constexpr int kLds = 2 * 2 * kTile * 2 * D;  // two stages; NonFinite comes after
 };
 
@@ -807,7 +850,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a, int block, uint8_
   const int group = a.group, li = lane & 31, half = lane >> 5;
   if (MODE != kPrefix && unit == 0) zero_loose_tokens<D>(a, head, 256);
   Job found;
-  if (!find_job<MODE, kManyRows, KT, Many<D>::kGrain>(a, unit, &found)) return;
+  if (!find_job<MODE, kManyRows, KT, Many<D>::kGrain, Many<D>::kChunk>(a, unit, &found)) return;
   const Job j = uniform(found);
 
   const int row = min(wave * 32 + li, j.rows - 1);
@@ -1011,21 +1054,26 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a, int block, uint8_
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+    constexpr int AHEAD = D < 128 ? D / 32 : 4;  // 32-channel blocks whose loads are in flight: 64 registers at most
     for (int c = 0; c < j.chunks; ++c) {
       const float2 ml = load_device(ml_at(c));
-      const float2 f = join_factors(&top, ml.x);
-      total = joined(f, total, ml.y);
+      float2 f;
 #pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) {
-        float2 x[8];
+      for (int dt = 0; dt < D / 32; dt += AHEAD) {
+        float2 x[AHEAD][8];
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) x[e >> 1] = load_device(o_at(c, dt, e));
+        for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          o[dt][e] = joined(f, o[dt][e], x[e >> 1].x);
-          o[dt][e + 1] = joined(f, o[dt][e + 1], x[e >> 1].y);
-        }
-        __builtin_amdgcn_sched_barrier(0);  // one 32-channel block's loads in flight, for the sake of registers
+          for (int e = 0; e < 16; e += 2) x[u][e >> 1] = load_device(o_at(c, dt + u, e));
+        if (dt == 0) f = join_factors(&top, ml.x), total = joined(f, total, ml.y);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            o[dt + u][e] = joined(f, o[dt + u][e], x[u][e >> 1].x);
+            o[dt + u][e + 1] = joined(f, o[dt + u][e + 1], x[u][e >> 1].y);
+          }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     sum = total;
