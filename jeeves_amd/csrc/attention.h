@@ -108,6 +108,7 @@ struct AttnPlan {
   bool few_own, few_prefix;  // tiles of kFewRows rows instead of kManyRows
   bool split;                // the keys of a row tile may go to several workgroups
   int tiles;                 // at least the batch's row tiles
+  int at_once;               // workgroups of a head that the device holds at a time
   int cu_units;              // workgroups of a head that come to the device's CUs first, one a CU
   int own_units;             // tile slots, or with a split the most units (tile, key chunk) that there can be
   int prefix_tiles, prefix_splits;  // where the prefix is gone through apart, for all tokens' rows

@@ -226,9 +226,19 @@ __device__ __forceinline__ float wave_sum_f32(float v) {
 // does, as each tile begins one chunk more than its share.
 //
 // Tiles of few rows are cut alike within a sequence (what its last tile sees is
-// taken for all). Of many rows, tile t of a sequence has x = a + t, so that a
-// prompt's early tiles, which see little, are cut less, and up to 64 sequences
-// take the least of eight m from W / own_units on that fits.
+// taken for all), from kWorthSplit steps on, and into half a device of chunks
+// more than there are tiles where these fill it. Cutting what is near the
+// average, for up to twice the tiles, took 24.3 instead of 16.7 us for 64
+// sequences of 300 keys (32 heads of 128), 45 instead of 30 for 128, 48 instead
+// of 42 for 64 of 1000; cutting 500 keys 18.5 instead of 15.0 for 32 sequences,
+// but 10.0 instead of 10.9 for 4.
+//
+// Of many rows, tile t of a sequence has x = a + t, so that a prompt's early
+// tiles, which see little, are cut less, and up to 64 sequences take the least
+// of eight m from W / own_units on that fits. (A prompt of 2048 tokens of 16
+// heads of 256: 70 us, 90 with chunks alike; of 1500 tokens of 32 heads of 128
+// 42 us, 49 with up to twice as many units as the device holds.)
+constexpr uint32_t kWorthSplit = 32;
 struct Unit {
   int b, tile, chunk, chunks;  // sequence, row tile and chunk of the unit, chunks of the tile
   Sequence seq;
@@ -242,7 +252,7 @@ __device__ __forceinline__ uint32_t sum_below(uint32_t x, uint32_t m) {
 template <int ROWS, int CHUNK>
 __device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int shared, Unit* u) {
   constexpr bool MANY = ROWS == kManyRows;
-  const int lane = threadIdx.x & 63, batches = (a.batch + 63) >> 6, most = a.p.own_units;
+  const int lane = threadIdx.x & 63, batches = (a.batch + 63) >> 6;
   const uint32_t step = MANY ? max(16u, (uint32_t)(ROWS + a.group - 1) / (uint32_t)a.group) : 16;
   uint32_t weight = 0, m = 1;
   int all_tiles = 0, before = 0;
@@ -259,13 +269,14 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int share
     // x of the first tile, or of all
     const uint32_t x = MANY ? ((uint32_t)(shared + max(0, s.len - s.n)) + step - 1) / step : (uint32_t)max(shared + s.len - 1, 0) / step;
     const auto units = [&](uint32_t m) {
-      return (int)(MANY ? tiles + sum_below(x + tiles, m) - sum_below(x, m) : a.p.split ? tiles * (1 + x / m) : tiles);
+      return (int)(MANY ? tiles + sum_below(x + tiles, m) - sum_below(x, m) : a.p.split && x >= kWorthSplit ? tiles * (1 + x / m) : tiles);
     };
     if (i < batches) {
       weight += (uint32_t)lane_value(wave_scan((int)(tiles * x + (MANY ? tiles * (tiles - 1) / 2 : 0))), 63);
       all_tiles = min(all_tiles + lane_value(wave_scan((int)tiles), 63), (1 << 30) - 1);
       if (i + 1 < batches) continue;
       if (all_tiles > a.p.tiles) return false;  // starts that decrease
+      const int most = MANY ? a.p.own_units : min(a.p.own_units, max(a.p.at_once, all_tiles + a.p.at_once / 2));
       const uint32_t least = (CHUNK + step - 1) / step;
       m = max(least, weight / (uint32_t)max(1, most - all_tiles) + 1);
       if (MANY && batches == 1) {
@@ -288,7 +299,7 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int share
       u->b = base + l;
       u->seq = Sequence{lane_value(s.start, l), lane_value(s.n, l), lane_value(s.len, l)};
       if (!MANY) {
-        u->chunks = a.p.split ? uniform((int)(1 + its_x / m)) : 1;
+        u->chunks = a.p.split && its_x >= kWorthSplit ? uniform((int)(1 + its_x / m)) : 1;
         u->tile = uniform((int)((uint32_t)of / (uint32_t)u->chunks));
         u->chunk = of - u->tile * u->chunks;
         return true;
@@ -1196,27 +1207,35 @@ AttnPlan attention_plan(int64_t tokens, int64_t batch, int64_t q_heads, int64_t 
                         bool ragged, int cus) {
   AttnPlan p{};
   const int64_t group = q_heads / kv_heads, all_rows = tokens * group;
+  // 16 sequences over 1000 keys, 8 heads of 4 query heads each: of 4 queries 21.5
+  // us in tiles of few rows and 22.5 of many, of 8 queries 21.6 and 22.9, of 16
+  // 36 and 24; one query of 2000 keys 11 and 21.
   p.few_own = all_rows <= batch * kFewRows;
   const int64_t rows = p.few_own ? kFewRows : kManyRows;
   const int64_t tiles = !ragged && group <= rows ? batch : all_rows / rows + batch;
   // units that the device holds at a time: by LDS, two workgroups a CU of the
   // many-row kernel, 4, 2 or 1 of the few-row kernel
   const int64_t at_once = cus * (p.few_own ? 256 / dim : 2) / kv_heads;
-  // Many-row tiles that fill the device stay whole. Otherwise the keys are cut
-  // for as many units as it holds, or for a second chunk of the longer
-  // sequences where the tiles alone come near that.
+  // Many-row tiles that fill the device stay whole: cutting them too, a prompt
+  // of 2048 tokens (32 heads of 128) takes 73 us instead of 56, 16 sequences of
+  // 128 queries over 1000 keys 77 instead of 51.
   p.split = p.few_own || tiles < at_once;
+  p.at_once = (int)std::max<int64_t>(1, at_once);
   p.cu_units = (int)(cus / kv_heads);
   p.tiles = (int)tiles;
-  p.own_units = (int)(p.split ? std::max<int64_t>(at_once, 2 * tiles) : tiles);
+  p.own_units = (int)(!p.split ? tiles : p.few_own ? std::max<int64_t>(at_once, tiles + at_once / 2) : at_once);
   // chunks that are not joined in a launch of their own are counted in
   const bool counted = p.split && !(p.few_own && prefix_len > 0);
   if (counted && p.own_units * kv_heads > kAttnCounters) p.split = false, p.own_units = (int)tiles;
   if (p.few_own && prefix_len > 0) {
+    // 16 rows over 1000 keys take 10.8 us in tiles of few rows, 12.7 of many; at
+    // 32 rows and 64 over 8192 the two differ by 2 us at most, either way.
     p.few_prefix = all_rows <= kFewRows;
     const int64_t prows = p.few_prefix ? kFewRows : kManyRows;
     p.prefix_tiles = (int)((all_rows + prows - 1) / prows);
-    // one workgroup a CU, of 256 keys at least: each writes its rows' results in 32 bits
+    // one workgroup a CU, of 256 keys at least: each writes its rows' results in
+    // 32 bits (two a CU: 37 us instead of 31 for 64 sequences over 8192 keys; 128
+    // keys: 24.7 instead of 19.2 for 32 over 4096, 14.0 instead of 15.9 over 1024)
     const int64_t share = std::max<int64_t>(1, cus / (kv_heads * p.prefix_tiles));
     p.prefix_splits = (int)std::min(share, (prefix_len + 255) / 256);
   }
