@@ -1228,9 +1228,9 @@ AttnPlan attention_plan(int64_t tokens, int64_t batch, int64_t q_heads, int64_t 
   const bool counted = p.split && !(p.few_own && prefix_len > 0);
   if (counted && p.own_units * kv_heads > kAttnCounters) p.split = false, p.own_units = (int)tiles;
   if (p.few_own && prefix_len > 0) {
-    // 16 rows over 1000 keys take 10.8 us in tiles of few rows, 12.7 of many; at
-    // 32 rows and 64 over 8192 the two differ by 2 us at most, either way.
-    p.few_prefix = all_rows <= kFewRows;
+    // in tiles of few rows and of many: 16 rows over 1000 keys 10.8 and 12.7 us, 32
+    // rows 10.9 and 12.9, 32 over 8192 16.6 and 18.4; 64 rows 19.8 and 20.1
+    p.few_prefix = all_rows <= 2 * kFewRows;
     const int64_t prows = p.few_prefix ? kFewRows : kManyRows;
     p.prefix_tiles = (int)((all_rows + prows - 1) / prows);
     // one workgroup a CU, of 256 keys at least: each writes its rows' results in

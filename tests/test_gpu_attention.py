@@ -332,6 +332,13 @@ def test_decode_with_prefix(dim, heads, prefix, batch):
           torch.bfloat16).check()
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [16, 17, 31, 32, 33])
+def test_prefix_tiles_of_few_and_many_rows(dim, rows):
+    """The rows of all heads of a group at and beside the tiles' sizes."""
+    Batch(26, [(b * 53) % 700 for b in range(rows)], prefix=1100, heads=(2, 2), dim=dim).check()
+
+
 @pytest.mark.parametrize("dim,heads", [(64, (6, 2)), (128, (8, 2)), (128, (3, 3)), (256, (8, 2))])
 @pytest.mark.parametrize("prefix", [0, 47, 700])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
