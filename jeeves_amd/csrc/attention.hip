@@ -8,12 +8,13 @@
 // outputs scaled by 2^(r - r') when r moves to r'. r only has to stay within
 // 2^8 of the largest weight, so it moves when a score exceeds it by 8, not at
 // every new maximum; until then a step needs no exchange between lanes and no
-// rescaling. Each row's reference moves by its own scores alone, so a row's
-// bits do not depend on the rows beside it. Scores, weights' sums and outputs are fp32; the weights are
-// rounded to the 16-bit type for the product with V (a relative 2^-9 or 2^-12
-// at most for bf16 and fp16, of mixed signs); their sum is that of the unrounded
-// ones. fp16 weights are 2^7 larger, up to 2^15, so that those that many keys
-// share stay normal numbers.
+// rescaling. Each row's reference moves by its own scores alone, so a row's bits
+// do not depend on the rows beside it. Scores, weights' sums and outputs are
+// fp32; the weights are rounded to the 16-bit type for the product with V (a
+// relative 2^-9 or 2^-12 at most for bf16 and fp16, of mixed signs). Their sum
+// is that of the unrounded ones in tiles of few rows and of the rounded ones, by
+// one instruction a pair, in tiles of many. fp16 weights are 2^7 larger, up to
+// 2^15, so that those that many keys share stay normal numbers.
 //
 // Both products run on MFMA with the keys on the A side: S^T = K Q^T leaves
 // each lane the scores of one query row, and the score tile's registers are,
@@ -267,9 +268,10 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int share
     }
     const uint32_t tiles = (uint32_t)(s.n * a.group + ROWS - 1) / (uint32_t)ROWS;
     // x of the first tile, or of all
-    const uint32_t x = MANY ? ((uint32_t)(shared + max(0, s.len - s.n)) + step - 1) / step : (uint32_t)max(shared + s.len - 1, 0) / step;
+    const uint32_t x = (MANY ? (uint32_t)(shared + max(0, s.len - s.n)) + step - 1 : (uint32_t)max(shared + s.len - 1, 0)) / step;
     const auto units = [&](uint32_t m) {
-      return (int)(MANY ? tiles + sum_below(x + tiles, m) - sum_below(x, m) : a.p.split && x >= kWorthSplit ? tiles * (1 + x / m) : tiles);
+      if (MANY) return (int)(tiles + sum_below(x + tiles, m) - sum_below(x, m));
+      return (int)(a.p.split && x >= kWorthSplit ? tiles * (1 + x / m) : tiles);
     };
     if (i < batches) {
       weight += (uint32_t)lane_value(wave_scan((int)(tiles * x + (MANY ? tiles * (tiles - 1) / 2 : 0))), 63);
@@ -561,6 +563,11 @@ __device__ __forceinline__ float with_non_finite(float o, const NonFinite<D>& n,
 // tiles of its own through its own ring of two stages, with no barrier, and
 // the waves' results meet in LDS at the end. 16x16 MFMA; a lane holds row
 // lane % 16 and keys 4 (lane / 16) + 0..3 of a tile.
+//
+// 4 sequences of 32000 to 59000 keys (4 heads of 256, 719 MB) take 134 us, 5.4
+// TB/s; a ragged batch of 64 (8 heads of 128, 124 MB) 29, 4.3 TB/s: a workgroup
+// has about 5 us of finding its unit, the first copies and the join beside its
+// keys. One sequence of 517 keys takes 9.5 us, a launch and that chain.
 // ---------------------------------------------------------------------------
 // Partial results that a thread has in flight when it joins them.
 constexpr int kJoinAhead = 8;
@@ -825,9 +832,20 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a, int block, uint8_t
 
 // ---------------------------------------------------------------------------
 // Many rows: tiles of 128, four waves of 32 rows that share the key tiles.
-// MFMA-bound for long prompts. 32x32x16 MFMA; a lane holds row lane % 32 and
-// keys 8 i + 4 (lane / 32) + 0..3. Two stages: while a tile is multiplied the
-// next one's copies are in flight; one barrier a tile.
+// 32x32x16 MFMA; a lane holds row lane % 32 and keys 8 i + 4 (lane / 32) + 0..3.
+// Two stages: while a tile is multiplied the next one's copies are in flight;
+// one barrier a tile. The next 16 keys' weights are worked out between the
+// products of the ones before, which hides the exponentials (8% of the time
+// without that).
+//
+// Prompts of 8192 tokens take 535 us with 32 heads of 128 (1030 TFLOP/s; a large
+// bf16 library product reaches 1197), 505 with 16 of 256 (1090) and 300 with 32
+// of 64 (915). Nothing alone bounds it: of a prompt's time 25% go without the
+// first product, 25% without the second, 12% without the copies; a wave's 32 rows
+// make LDS deliver as many bytes as MFMA takes cycles. Eight waves a workgroup
+// (108 instead of 85 us for 16 sequences over a prefix of 2000) and 32-key tiles
+// at three waves a SIMD (even) were no better. Short prompts wait for HBM beside
+// it: 16 of 512 tokens move 167 MB in 72 us.
 // ---------------------------------------------------------------------------
 template <int D>
 struct Many {
@@ -1117,7 +1135,9 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttnArgs a) {
 }
 
 // A decode batch with a prefix: shares of the prefix for all rows (the first
-// workgroups) and chunks of the sequences' own keys side by side.
+// workgroups) and chunks of the sequences' own keys side by side. 64 sequences
+// (32 heads of 128) over 8192 keys: 20 us, a share 16.6 of them for 8 key tiles,
+// and 5.3 of the join; in two launches, the own keys' after the prefix's, 6 more.
 template <class H, int D, bool FEW_PREFIX>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_shared_kernel(AttnArgs a) {
   constexpr int LDS = FEW_PREFIX || Few<D>::kLds > Many<D>::kLds ? Few<D>::kLds : Many<D>::kLds;
