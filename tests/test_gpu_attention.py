@@ -332,6 +332,12 @@ def test_decode_with_prefix(dim, heads, prefix, batch):
           torch.bfloat16).check()
 
 
+@pytest.mark.parametrize("queries", [None, [1, 40, 3]])
+@pytest.mark.parametrize("prefix", [0, 40])
+def test_more_key_heads_than_workgroups_at_a_time(queries, prefix):
+    Batch(27, [30, 100, 600], queries, prefix=prefix, heads=(600, 600), dim=64).check()
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("rows", [16, 17, 31, 32, 33])
 def test_prefix_tiles_of_few_and_many_rows(dim, rows):
