@@ -460,18 +460,18 @@ __device__ __forceinline__ void static_for(F&& f) {
 
 // The factors that bring a result with reference `top` and one with reference
 // `ref` to their common one, which becomes `top`. A part without keys has the
-// reference -inf and counts for nothing.
+// reference -inf and counts for nothing. One with a NaN score has the reference
+// NaN, which no later part takes away: fmaxf would drop it.
 __device__ __forceinline__ float2 join_factors(float* top, float ref) {
-  const float next = fmaxf(*top, ref);
+  const float next = __builtin_isunordered(*top, ref) ? __builtin_nanf("") : fmaxf(*top, ref);
   const float2 f{*top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(*top - next),
                  ref == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - next)};
   *top = next;
   return f;
 }
-// a f.x + b f.y, where a factor of 0 takes its value out whatever that is.
-__device__ __forceinline__ float joined(float2 f, float a, float b) {
-  return (f.x == 0.0f ? 0.0f : a * f.x) + (f.y == 0.0f ? 0.0f : b * f.y);
-}
+// a f.x + b f.y. The sums of a part without keys are 0; a NaN under a factor
+// that is 0 in 32 bits stays NaN, as it does under such a weight.
+__device__ __forceinline__ float joined(float2 f, float a, float b) { return a * f.x + b * f.y; }
 
 // Where the copies of a key tile come from. A wave copies rows of one aligned
 // group of 16 keys, which lies in one page: the page's id comes by a scalar

@@ -1,0 +1,117 @@
+"""paged_attention, qk_norm_rope and FP8Attention at unusual values and sizes.
+Oracles are in 64 bits or follow from the definition alone."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_attention import DEV, U, Batch, gen, new_cache, randn
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------
+# Rows that see a NaN score are NaN, all others keep their bits. Prefixes of 40
+# and 1100 keys are one and several shares; 6 sequences of 8 query heads go
+# through it in tiles of few rows (24 rows a key head), 16 query heads in tiles
+# of many (48). 4000 keys are cut into chunks.
+LENGTHS = [1, 16, 17, 48, 64, 4000]
+
+
+def check_nan_rows(b, clean, rows):
+    """rows [tokens] or [tokens, heads]: those that have to be NaN in every channel; the others are as in clean."""
+    out = b.run()
+    rows = rows if rows.dim() == 2 else rows[:, None].expand(out.shape[:2])
+    assert out[rows].isnan().all(), (~out.isnan().all(-1) & rows).nonzero().tolist()
+    assert torch.equal(out[~rows], clean[~rows])
+
+
+@pytest.mark.parametrize("prefix", [0, 40, 1100])
+@pytest.mark.parametrize("heads", [(8, 2), (16, 2)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_a_nan_query_is_nan_at_every_length(prefix, heads, dim):
+    b = Batch(40, LENGTHS, prefix=prefix, heads=heads, dim=dim)
+    clean = b.check()
+    for i in range(len(LENGTHS)):
+        kept = b.q[i, 3].clone()
+        b.q[i, 3, 7] = math.nan
+        rows = torch.zeros(b.q.shape[:2], dtype=torch.bool, device=DEV)
+        rows[i, 3] = True
+        check_nan_rows(b, clean, rows)
+        b.q[i, 3] = kept
+
+
+# whole tiles; the keys of many-row tiles split; tiles of few rows, whole and cut
+RAGGED = [([300, 500, 400], [300, 520, 400], 0, (64, 32)), ([64], [4000], 0, (8, 2)), ([64, 40], [3000, 900], 700, (8, 2)),
+          ([3, 2, 4], [70, 3000, 9], 0, (8, 2)), ([3, 2, 4], [70, 3000, 9], 300, (8, 2))]
+
+
+@pytest.mark.parametrize("queries,lengths,prefix,heads", RAGGED)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_a_nan_query_of_many_is_nan(queries, lengths, prefix, heads, dim):
+    b = Batch(41, lengths, queries, prefix=prefix, heads=heads, dim=dim)
+    clean = b.check()
+    for token in (0, queries[0] - 1, sum(queries) - 1):
+        kept = b.q[token, 1].clone()
+        b.q[token, 1, dim - 1] = math.nan
+        rows = torch.zeros(b.q.shape[:2], dtype=torch.bool, device=DEV)
+        rows[token, 1] = True
+        check_nan_rows(b, clean, rows)
+        b.q[token, 1] = kept
+
+
+def sees_own(b, i, key):
+    """[tokens]: the tokens that see own key `key` of sequence i."""
+    at = sum(b.queries[:i])
+    n, length = b.queries[i], b.lengths[i]
+    rows = torch.zeros(b.q.shape[0], dtype=torch.bool, device=DEV)
+    rows[at:at + n] = key <= length - n + torch.arange(n, device=DEV)
+    return rows
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("queries,lengths,prefix,heads", [(None, [100, 64, 4000], 0, (8, 2)), (None, [100, 64, 4000], 40, (8, 2)),
+                                                          (None, [100, 64, 4000], 1100, (16, 1)), *RAGGED])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_a_key_that_is_not_finite_reaches_every_row_that_sees_it(queries, lengths, prefix, heads, dim, value):
+    """In the first, a middle and the last wave, chunk and prefix share. Queries are positive in the channel, so that an
+    infinite key gives an infinite score, whose softmax is NaN."""
+    b = Batch(42, lengths, queries, prefix=prefix, heads=heads, dim=dim)
+    b.q[..., 3] = b.q[..., 3].abs() + 0.5
+    clean = b.check()
+    for i, length in enumerate(lengths):
+        for key in sorted({0, min(17, length - 1), min(33, length - 1), length // 2, length - 1}):
+            at = (int(b.table[i, key // b.page]), slice(None), key % b.page, 3)
+            kept = b.cache.k[at].clone()
+            b.cache.k[at] = value
+            check_nan_rows(b, clean, sees_own(b, i, key))
+            b.cache.k[at] = kept
+    for key in sorted({0, prefix // 2, prefix - 1}) if prefix else []:
+        at = (int(b.prefix_pages[key // b.page]), slice(None), key % b.page, 3)
+        kept = b.cache.k[at].clone()
+        b.cache.k[at] = value
+        check_nan_rows(b, clean, torch.ones(b.q.shape[0], dtype=torch.bool, device=DEV))
+        b.cache.k[at] = kept
+
+
+@pytest.mark.parametrize("queries,lengths,prefix,low", [
+    (None, [64, 64], 0, (0, 16)), (None, [64, 64], 0, (32, 48)), (None, [4000, 2500], 0, (0, 2000)), (None, [40, 40], 1100, (0, 608)),
+    (None, [40, 40], 1100, (1008, 1088)), ([64], [4000], 0, (0, 2000)), ([64], [4000], 0, (2000, 3008))])
+def test_a_nan_value_under_a_weight_of_zero(queries, lengths, prefix, low):
+    """Keys whose weights are 0 in 32 bits, one of them with a NaN value: 0 * NaN, so the channel is NaN, also where these
+    keys are all that a wave, a chunk or a share of the prefix has."""
+    b = Batch(43, lengths, queries, prefix=prefix)
+    b.q.fill_(4.0)
+    b.cache.k.fill_(0.0)
+    pages = (b.prefix_pages if prefix else b.table[0])[low[0] // 16:low[1] // 16].long()
+    clean = b.run()
+    b.cache.k[pages] = -8.0  # scores of -362: e^-362 is no number of 32 bits
+    b.cache.v[pages[-1], :, 3, 5] = math.nan
+    out = b.run()
+    rows = torch.ones(b.q.shape[0], dtype=torch.bool, device=DEV) if prefix else sees_own(b, 0, low[1] - 13)
+    assert out[rows][..., 5].isnan().all()
+    others = [c for c in range(b.q.shape[2]) if c != 5]
+    assert out[..., others].isfinite().all() and torch.equal(out[~rows], clean[~rows])
