@@ -32,9 +32,9 @@ extern "C" {
  * i + rotary / 2 (i < rotary / 2) are turned by the angle of the token's
  * position: fp32 throughout, rounded once.
  * rope: float32 [n_pos, rotary], each position's rotary / 2 cosines, then its
- * sines, 16-byte aligned (NULL: no rotation); rotary a multiple of 16 up to
- * dim. pos: int32 [tokens], int64 with pos64. A token whose position the table
- * does not have comes out as NaN. The role of _rotary
+ * sines, 16-byte aligned, n_pos at least 1 (NULL: no rotation); rotary a
+ * multiple of 16 up to dim. pos: int32 [tokens], int64 with pos64. A token whose
+ * position the table does not have comes out as NaN. The role of _rotary
  * (model/triton_kernels.py:54) and of the q and k norms before it.
  */
 int jv_norm_rope(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs, const float* rope,

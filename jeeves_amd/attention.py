@@ -123,8 +123,10 @@ def _rope_operands(rope: torch.Tensor | None, positions: torch.Tensor | None, to
     if rope is None:
         return _NO_ROPE
     shape = rope.shape
-    if rope.dtype is not torch.float32 or len(shape) != 2 or rope.get_device() != index or shape[1] & 15 or not 0 < shape[1] <= dim:
-        _refuse("rope", rope, f"float32 [positions, a multiple of 16 channels up to {dim}] on HIP device {index}")
+    # an empty table has no address, which would mean no rotation
+    if (rope.dtype is not torch.float32 or len(shape) != 2 or rope.get_device() != index or not shape[0] or shape[1] & 15 or
+            not 0 < shape[1] <= dim):
+        _refuse("rope", rope, f"float32 [positions (1 at least), a multiple of 16 channels up to {dim}] on HIP device {index}")
     if positions is None:
         raise ValueError("the rotation needs the tokens' positions")
     if not rope.is_contiguous() or rope.data_ptr() & 15:

@@ -38,7 +38,8 @@ int check_rope(const float* rope, int64_t n_pos, int64_t rotary, const void* pos
   if (!rope) return JV_OK;
   if (rotary <= 0 || rotary % 16 || rotary > dim)
     return fail(JV_ERR_VALUE, "the rotation takes a multiple of 16 channels up to %lld, got %lld", (long long)dim, (long long)rotary);
-  if (n_pos < 0 || !pos || !aligned16(rope)) return fail(JV_ERR_VALUE, "the rotation needs positions and a 16-byte aligned table");
+  if (n_pos < 1 || !pos || !aligned16(rope))
+    return fail(JV_ERR_VALUE, "the rotation needs positions and a 16-byte aligned table of one position at least");
   return JV_OK;
 }
 

@@ -72,3 +72,13 @@ def test_no_tokens_is_a_call_that_succeeds(product_lib):
     assert norm_rope(product_lib, tokens=0, q=None, k=None) == _lib.JV_OK
     assert append(product_lib, tokens=0, k=None, v=None, slots=None) == _lib.JV_OK
     assert attention(product_lib, tokens=0, q=None, out=None, batch=0) == _lib.JV_OK
+
+
+@pytest.mark.parametrize("n_pos", [0, -7])
+def test_rotation_needs_a_position(product_lib, n_pos):
+    """A position outside the table reads the first one's angles, which there have to be."""
+    assert norm_rope(product_lib, n_pos=n_pos, tokens=0) == _lib.JV_ERR_VALUE
+    assert b"one position" in product_lib.jv_fp8_last_error()
+    L = product_lib
+    assert L.jv_append_kv(P, 256, 128, P, 256, 128, P, 1, P, P, 4, 16, P, n_pos, 64, P, 0, None, 1e-6, None, 0, 0, None, None, 8, 0, 2,
+                          128, 0, None) == _lib.JV_ERR_VALUE

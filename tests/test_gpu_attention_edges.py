@@ -115,3 +115,19 @@ def test_a_nan_value_under_a_weight_of_zero(queries, lengths, prefix, low):
     assert out[rows][..., 5].isnan().all()
     others = [c for c in range(b.q.shape[2]) if c != 5]
     assert out[..., others].isfinite().all() and torch.equal(out[~rows], clean[~rows])
+
+
+# ---------------------------------------------------------------------------
+# index tensors
+# ---------------------------------------------------------------------------
+def test_rotation_needs_a_table():
+    from jeeves_amd.attention import append_kv, qk_norm_rope, rope_table
+
+    g = gen(50)
+    q, k, pos = randn(g, 2, 4, 128), randn(g, 2, 2, 128), torch.zeros(2, dtype=torch.int32, device=DEV)
+    cache = new_cache(g, 2, 2, 16, 128)
+    for rope in (rope_table(8, 64)[:0], rope_table(0, 64)):
+        with pytest.raises(ValueError):
+            qk_norm_rope(q, k, rope, pos)
+        with pytest.raises(ValueError):
+            append_kv(cache, k, k, pos, rope=rope, positions=pos)
