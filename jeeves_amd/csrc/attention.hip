@@ -33,6 +33,27 @@ namespace jv {
 
 constexpr float kRescaleAt = 8.0f;
 
+// Exponents are one FMA, s scale - r, of a reference r that was rounded as s
+// scale was: from 2^20 on what the rounding took from r would show in the
+// weights (2^24 and more of it passes what fp16 holds, 2^31 fp32). Scores of
+// such rows have r taken off their rounded product first, at every tile: their
+// wave's limit lets every tile in where references are moved. `sub`: what the
+// FMA takes off; s: N registers V of scores. Returns the wave's new limit.
+constexpr float kRoundAt = 1048576.0f;
+template <class H, int N, class V>
+__device__ __forceinline__ float moved_to(float ref, float scale, float* sub, V* s) {
+  *sub = ref == -__builtin_inff() ? 0.0f : ref - H::kShift;
+  const bool large = fabsf(ref) >= kRoundAt && ref != -__builtin_inff();
+  if (!__any(large)) return ref + kRescaleAt;
+  const float inv = 1.0f / scale;
+#pragma unroll
+  for (int b = 0; b < N; ++b)
+#pragma unroll
+    for (int e = 0; e < (int)(sizeof(V) / 4); ++e) s[b][e] = large ? (s[b][e] * scale - *sub) * inv : s[b][e];
+  if (large) *sub = 0.0f;
+  return -__builtin_inff();
+}
+
 __device__ __forceinline__ void load_lds16(const uint8_t* src, uint8_t* dst_wave_base) {
   typedef __attribute__((address_space(3))) void lds_void;
   typedef __attribute__((address_space(1))) void global_void;
@@ -649,6 +670,7 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a, int block, uint8_t
 #pragma unroll
   for (int dt = 0; dt < D / 16; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   float ref = -__builtin_inff(), sum = 0.0f;
+  float limit = ref, sub = 0.0f;  // what moves the reference, what is taken off an exponent
   lds_barrier();  // `bad` is set up
   Group next{};
   if (n_tiles > 0) {
@@ -681,7 +703,7 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a, int block, uint8_t
         if (key0 + quarter * 4 + e > sees) s[e] = -__builtin_inff();
     }
     float top = fmaxf(fmaxf(s.x, s.y), fmaxf(s.z, s.w));
-    if (__any(top * a.scale_log2 > ref + kRescaleAt)) {
+    if (__any(top * a.scale_log2 > limit)) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       const float next = top * a.scale_log2 > ref + kRescaleAt ? top * a.scale_log2 : ref;
@@ -690,8 +712,8 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a, int block, uint8_t
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt) o[dt] *= f;
       ref = next;
+      limit = moved_to<H, 1>(ref, a.scale_log2, &sub, &s);
     }
-    const float sub = ref == -__builtin_inff() ? 0.0f : ref - H::kShift;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.scale_log2, -sub));
@@ -930,6 +952,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a, int block, uint8_
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
   float ref = -__builtin_inff(), sum = 0.0f;
+  float limit = ref, sub = 0.0f;  // what moves the reference, what is taken off an exponent
   Group next{};
   if (j.tiles > 0) {
     issue(0, group_of(0));
@@ -995,7 +1018,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a, int block, uint8_
     for (int b = 0; b < SUB; ++b)
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, s[b][e]);
-    if (__any(top * a.scale_log2 > ref + kRescaleAt)) {
+    if (__any(top * a.scale_log2 > limit)) {
       top = fmaxf(top, __shfl_xor(top, 32));
       const float next = top * a.scale_log2 > ref + kRescaleAt ? top * a.scale_log2 : ref;
       const float f = ref == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ref - next);
@@ -1003,8 +1026,8 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a, int block, uint8_
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) o[dt] *= f;
       ref = next;
+      limit = moved_to<H, SUB>(ref, a.scale_log2, &sub, s);
     }
-    const float sub = ref == -__builtin_inff() ? 0.0f : ref - H::kShift;
     // The weights of 16 keys, as the B operand of their step.
     const auto weights = [&](int ks) {
       i32x4 p;

@@ -118,6 +118,37 @@ def test_a_nan_value_under_a_weight_of_zero(queries, lengths, prefix, low):
 
 
 # ---------------------------------------------------------------------------
+# weights
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("queries,lengths,prefix", [(None, [600, 333, 4000, 7], 0), (None, [600, 333, 40, 7], 1100), ([2, 3], [600, 333], 0),
+                                                    ([300, 400], [600, 433], 0), ([64], [4000], 100)])
+@pytest.mark.parametrize("size", [2048.0, 8192.0])
+def test_scores_past_32_bits_of_whole_numbers(queries, lengths, prefix, dtype, size):
+    """Finite queries and keys whose scores reach 2^26 to 2^31: the largest takes all of the softmax, so its value comes
+    out as it is. Rows whose two largest scores are closer than 32-bit sums tell apart (each is off by 2^-17 |q| |k| at
+    most for 128 products) are left out."""
+    b = Batch(47, lengths, queries, prefix=prefix, heads=(8, 2), dim=128, dtype=dtype)
+    b.q.mul_(size)
+    b.cache.k.mul_(size)
+    assert b.q.isfinite().all() and b.cache.k.isfinite().all()
+    out, at, left_out = b.run(scale=1.0), 0, 0
+    for i, (n, length) in enumerate(zip(b.queries, lengths)):
+        k, v = b.keys(i, b.cache.k), b.keys(i, b.cache.v)
+        unseen = torch.arange(prefix + length, device=DEV)[None] > prefix + length - n + torch.arange(n, device=DEV)[:, None]
+        for h in range(8):
+            q = b.q[at:at + n, h].double()
+            score = (q @ k[h // 4].t()).masked_fill(unseen, -math.inf)
+            top = torch.cat([score, torch.full((n, 1), -math.inf, dtype=torch.float64, device=DEV)], 1).topk(2, 1)
+            clear = top.values[:, 0] - top.values[:, 1] > 2.0 ** -14 * q.norm(dim=1) * k[h // 4].norm(dim=1).max() + 200
+            got, want = out[at:at + n, h], v[h // 4][top.indices[:, 0]].to(dtype)
+            assert torch.equal(got[clear], want[clear]), (i, h, (got != want).any(1).sum().item())
+            left_out += int((~clear).sum())
+        at += n
+    assert left_out <= 0.05 * at * 8
+
+
+# ---------------------------------------------------------------------------
 # index tensors
 # ---------------------------------------------------------------------------
 def test_rotation_needs_a_table():
