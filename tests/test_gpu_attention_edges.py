@@ -149,6 +149,23 @@ def test_scores_past_32_bits_of_whole_numbers(queries, lengths, prefix, dtype, s
 
 
 # ---------------------------------------------------------------------------
+# norm
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("exponent", [-62, -64, -66, -30, 30])
+def test_norm_of_tiny_and_large_rows(dim, exponent):
+    """Without eps, also where the mean square is below the normal numbers of 32 bits: rows of 2^-66 have squares of
+    2^-132, on a grid of 2^-149, so the mean and its root are off by 2^-17 or less (2^-18 and a half below it)."""
+    from jeeves_amd.attention import qk_norm_rope
+
+    x = randn(gen(48), 33, 3, dim) * 2.0 ** exponent
+    w = torch.ones(dim, device=DEV)
+    y = x.double() / x.double().square().mean(-1, keepdim=True).sqrt()
+    for out in qk_norm_rope(x, x, None, None, q_weight=w, k_weight=w, eps=0.0):
+        assert ((out.double() - y).abs() <= (2 * U[x.dtype] + 2.0 ** -14) * y.abs() + 2.0 ** -20).all()
+
+
+# ---------------------------------------------------------------------------
 # index tensors
 # ---------------------------------------------------------------------------
 def test_rotation_needs_a_table():
