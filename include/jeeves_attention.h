@@ -55,6 +55,14 @@ int jv_append_kv(const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64
                  int64_t q_hs, const float* q_weight, void* q_out, int64_t q_heads, int64_t tokens, int64_t kv_heads,
                  int64_t dim, int fp16, void* stream);
 
+/*
+ * int64 page tables, lengths or starts [rows, cols] as the contiguous int32
+ * that jv_paged_attention takes, values past 32 bits held at their ends.
+ * Strides in elements; fewer than 2^31 values.
+ */
+int jv_narrow_indices(const int64_t* src, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride, int32_t* dst,
+                      void* stream);
+
 #define JV_ATTENTION_COUNTERS 65536
 
 /* Bytes of workspace jv_paged_attention needs for these sizes on the current

@@ -228,7 +228,12 @@ def _int32(name: str, t: torch.Tensor, shape: tuple, index: int) -> torch.Tensor
     if t.dtype not in _WIDE or t.shape != shape or t.get_device() != index:
         _refuse(name, t, f"int32 or int64 {list(shape)} on HIP device {index}")
     if t.dtype is not torch.int32:
-        t = t.to(torch.int32)
+        rows, columns = shape if len(shape) == 2 else (1, shape[0])
+        out = torch.empty(shape, dtype=torch.int32, device=t.device)
+        with _on(index):
+            _lib.check(_lib.lib().jv_narrow_indices(t.data_ptr(), rows, columns, t.stride(0), t.stride(-1), out.data_ptr(),
+                                                    torch._C._cuda_getCurrentRawStream(index)))
+        return out
     return t if t.stride(-1) == 1 or shape[-1] < 2 else t.contiguous()
 
 

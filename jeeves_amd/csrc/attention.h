@@ -90,6 +90,10 @@ struct RopeArgs {
 
 hipError_t norm_rope(const RopeArgs& a, int dim, bool fp16, hipStream_t stream);
 
+// int64 indices [rows, cols] into contiguous int32, held in range (rope.hip).
+hipError_t narrow_indices(const int64_t* src, int rows, int cols, int64_t row_stride, int64_t col_stride, int32_t* dst,
+                          hipStream_t stream);
+
 // ---------------------------------------------------------------------------
 // Attention (attention.hip).
 // ---------------------------------------------------------------------------

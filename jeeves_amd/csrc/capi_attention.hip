@@ -123,6 +123,16 @@ int jv_append_kv(const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64
   return hip_status(jv::norm_rope(a, (int)dim, fp16 != 0, (hipStream_t)stream), "cache append launch");
 }
 
+int jv_narrow_indices(const int64_t* src, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride, int32_t* dst,
+                      void* stream) {
+  if (rows < 0 || cols < 0 || (cols > 0 && rows > INT32_MAX / cols))
+    return fail(JV_ERR_VALUE, "bad sizes: %lld rows of %lld indices", (long long)rows, (long long)cols);
+  if (rows == 0 || cols == 0) return JV_OK;
+  if (!src || !dst) return fail(JV_ERR_VALUE, "the indices or their output are missing");
+  return hip_status(jv::narrow_indices(src, (int)rows, (int)cols, row_stride, col_stride, dst, (hipStream_t)stream),
+                    "index launch");
+}
+
 int64_t jv_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
                                            int64_t prefix_len, int ragged) {
   if (check_batch(tokens, batch, q_heads, kv_heads, dim, prefix_len)) return -1;

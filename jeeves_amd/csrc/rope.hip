@@ -127,6 +127,22 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(RopeArgs a, uint32_t q_b
     if (keep && h0 + i < heads) *reinterpret_cast<uint4*>(dst + (h0 + i) * dst_hs) = x[i];
 }
 
+// A few thousand values at most: a launch's time.
+__global__ __launch_bounds__(256) void narrow_kernel(const int64_t* src, uint32_t n, uint32_t cols, int64_t row_stride,
+                                                     int64_t col_stride, int32_t* dst) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int64_t v = src[(int64_t)(i / cols) * row_stride + (int64_t)(i % cols) * col_stride];
+  dst[i] = (int32_t)(v < INT32_MIN ? INT32_MIN : v > INT32_MAX ? INT32_MAX : v);
+}
+
+hipError_t narrow_indices(const int64_t* src, int rows, int cols, int64_t row_stride, int64_t col_stride, int32_t* dst,
+                          hipStream_t stream) {
+  const uint32_t n = (uint32_t)rows * (uint32_t)cols;
+  narrow_kernel<<<(n + 255) / 256, 256, 0, stream>>>(src, n, (uint32_t)cols, row_stride, col_stride, dst);
+  return hipGetLastError();
+}
+
 template <class H, int D>
 static void launch_norm_rope(const RopeArgs& a, hipStream_t stream) {
   const auto blocks = [](int heads) { return (uint32_t)((heads + kHeads - 1) / kHeads); };

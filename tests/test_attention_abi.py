@@ -82,3 +82,11 @@ def test_rotation_needs_a_position(product_lib, n_pos):
     L = product_lib
     assert L.jv_append_kv(P, 256, 128, P, 256, 128, P, 1, P, P, 4, 16, P, n_pos, 64, P, 0, None, 1e-6, None, 0, 0, None, None, 8, 0, 2,
                           128, 0, None) == _lib.JV_ERR_VALUE
+
+
+def test_narrowing_refuses(product_lib):
+    narrow = product_lib.jv_narrow_indices
+    for rows, cols, src, dst in ((-1, 3, P, P), (3, -1, P, P), (1 << 16, 1 << 15, P, P), (2, 3, None, P), (2, 3, P, None)):
+        assert narrow(src, rows, cols, cols, 1, dst, None) == _lib.JV_ERR_VALUE
+    assert narrow(None, 0, 3, 3, 1, None, None) == _lib.JV_OK
+    assert narrow(None, 3, 0, 0, 1, None, None) == _lib.JV_OK

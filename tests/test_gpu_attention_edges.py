@@ -168,6 +168,28 @@ def test_norm_of_tiny_and_large_rows(dim, exponent):
 # ---------------------------------------------------------------------------
 # index tensors
 # ---------------------------------------------------------------------------
+def test_wide_indices_are_held_in_range_before_they_are_narrowed():
+    from jeeves_amd.attention import paged_attention
+
+    b = Batch(49, [70, 5, 33], [4, 5, 6], heads=(8, 2))
+    pages = b.cache.pages
+    far = torch.tensor([[-2 ** 40, 2 ** 32 + 1, 0, 3], [1, 2 ** 62, 3, 2], [2 ** 31, -1, 2, -2 ** 32 + 1]], device=DEV)
+    held = far.clamp(0, pages - 1).to(torch.int32)
+    lengths = torch.tensor([2 ** 32 + 3, -2 ** 33 + 20, 40], device=DEV)
+    starts = torch.tensor([0, 4, 9, 2 ** 32 + 3], device=DEV)
+    out = paged_attention(b.q, b.cache, far, lengths, query_starts=starts)
+    same = paged_attention(b.q, b.cache, held, torch.tensor([64, 0, 40], dtype=torch.int32, device=DEV), query_starts=b.starts)
+    assert torch.equal(out, same)
+    out = paged_attention(b.q, b.cache, b.table, b.device_lengths, query_starts=b.starts, prefix_pages=far[0], prefix_length=40)
+    same = paged_attention(b.q, b.cache, b.table, b.device_lengths, query_starts=b.starts, prefix_pages=held[0], prefix_length=40)
+    assert torch.equal(out, same)
+    strided = torch.stack([far, far + 1], 2)[..., 0]
+    lengths = torch.stack([b.device_lengths.long()] * 3, 1)[:, 1]
+    assert not strided.is_contiguous() and not lengths.is_contiguous()
+    assert torch.equal(paged_attention(b.q, b.cache, strided, lengths, query_starts=b.starts),
+                       paged_attention(b.q, b.cache, held, b.device_lengths, query_starts=b.starts))
+
+
 def test_rotation_needs_a_table():
     from jeeves_amd.attention import append_kv, qk_norm_rope, rope_table
 
