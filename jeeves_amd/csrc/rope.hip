@@ -105,11 +105,11 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(RopeArgs a, uint32_t q_b
         // the hardware's 1 / sqrt, which takes a subnormal m for 0 (so those go
         // through it scaled), and one Newton step (none where m is 0, inf or NaN)
         const bool tiny = m < 0x1p-100f;
-        m *= tiny ? 0x1p64f : 1.0f;
+        m *= tiny ? 0x1p60f : 1.0f;
         r = __builtin_amdgcn_rsqf(m);
         const float n = r * __builtin_fmaf(-0.5f * m * r, r, 1.5f);
         if (m > 0.0f && m < __builtin_inff()) r = n;
-        r *= tiny ? 0x1p32f : 1.0f;
+        r *= tiny ? 0x1p30f : 1.0f;
       }
       // a position that the table does not have: no angle, so no row
       if (bad) r = __builtin_nanf("");
