@@ -257,8 +257,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     A token that sees no key, or that belongs to no sequence, comes out as 0.
     Keys that a token does not see have no effect on it, even infinite or NaN
     ones; nor has what the table holds past a sequence's length, nor the other
-    sequences. The sums are in 32 bits; the softmax's weights are rounded to
-    the 16-bit type for the product with the values.
+    sequences. The sums are in 32 bits; where many query rows go through the same
+    keys (prompts, a prefix that many sequences share) the softmax's weights
+    are rounded to the 16-bit type for the product with the values, and their
+    sum is of the rounded ones.
 
     As a split-K GEMM of ``jeeves_amd.fp8`` does, a call whose keys are split
     over workgroups counts them in on the stream's tile counters, so run one on

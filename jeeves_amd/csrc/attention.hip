@@ -10,11 +10,14 @@
 // every new maximum; until then a step needs no exchange between lanes and no
 // rescaling. Each row's reference moves by its own scores alone, so a row's bits
 // do not depend on the rows beside it. Scores, weights' sums and outputs are
-// fp32; the weights are rounded to the 16-bit type for the product with V (a
-// relative 2^-9 or 2^-12 at most for bf16 and fp16, of mixed signs). Their sum
-// is that of the unrounded ones in tiles of few rows and of the rounded ones, by
-// one instruction a pair, in tiles of many. fp16 weights are 2^7 larger, up to
-// 2^15, so that those that many keys share stay normal numbers.
+// fp32; the product with V takes 16-bit weights. In tiles of few rows, where HBM
+// leaves MFMA idle, what the rounding leaves of a weight goes through a second
+// product (so weights are kept to 2^-16 or 2^-22; 29.1 and 28.8 us with and
+// without for the ragged 64 below, 133.5 both for the long ones). In tiles of
+// many rows, where MFMA is half the time, weights are rounded (a relative 2^-8
+// or 2^-11 at most for bf16 and fp16, of mixed signs) and their sum is that of
+// the rounded ones, by one instruction a pair. fp16 weights are 2^7 larger, up
+// to 2^15, so that those that many keys share stay normal numbers.
 //
 // Both products run on MFMA with the keys on the A side: S^T = K Q^T leaves
 // each lane the scores of one query row, and the score tile's registers are,
@@ -720,8 +723,10 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a, int block, uint8_t
       sum += s[e];
     }
     asm volatile("" : "+v"(sum));  // added up here, not after the weights' last use
+    // what the 16-bit weights leave goes through the product as well
     const uint2 pw{H::pack(s.x, s.y), H::pack(s.z, s.w)};
-    const s16x4 pb = __builtin_bit_cast(s16x4, pw);
+    const uint2 rest{H::pack(s.x - H::lo(pw.x), s.y - H::hi(pw.x)), H::pack(s.z - H::lo(pw.y), s.w - H::hi(pw.y))};
+    const s16x4 pb = __builtin_bit_cast(s16x4, pw), pr = __builtin_bit_cast(s16x4, rest);
     if (t + 1 < n_tiles) wait_vmem_below<2 * COPIES>();
     else wait_vmem_below<0>();
     __builtin_amdgcn_sched_barrier(0);
@@ -746,6 +751,8 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a, int block, uint8_t
 #pragma unroll
       for (int dt = 0; dt < AHEAD; dt += 4) lds_read_tr4<256>(at[dt], at[dt + 1], at[dt + 2], at[dt + 3], v + 8 + dt);
     }
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) o[dt] = H::mfma16k16(v[dt], pr, o[dt]);
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) o[dt] = H::mfma16k16(v[dt], pb, o[dt]);
   }

@@ -121,6 +121,39 @@ def test_a_nan_value_under_a_weight_of_zero(queries, lengths, prefix, low):
 # weights
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("queries,lengths,prefix", [
+    (None, [1, 2, 5, 17, 100, 1000, 5000], 0), (None, [1, 2, 5, 17, 100, 1000, 0], 50), (None, [1 + 9 * i for i in range(40)], 1100),
+    ([3, 2, 4], [70, 3000, 9], 0), ([64, 90], [3000, 90], 0), ([700, 800], [700, 810], 90)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_weights_add_to_one(queries, lengths, prefix, dim, dtype):
+    """Values that are the same for all keys come out as they are: sum(w) v / sum(w), with both sums in 32 bits of the
+    same weights, is v within 2^-14, which rounds to v, a number of the type."""
+    b = Batch(44, lengths, queries, prefix=prefix, dim=dim, dtype=dtype)
+    v = randn(gen(45), 1, b.cache.kv_heads, 1, dim, dtype=dtype)
+    b.cache.v.copy_(v.expand_as(b.cache.v))
+    out = b.run()
+    want = v[0, :, 0].repeat_interleave(b.q.shape[1] // b.cache.kv_heads, 0).expand_as(out).clone()
+    for i, length in enumerate(lengths):
+        if length == 0 and prefix == 0:
+            want[i] = 0
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("prefix", [0, 1, 9])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_weights_of_few_row_tiles_keep_more_than_16_bits(prefix, dim, dtype):
+    """Weights that go into the product as the sum of two 16-bit numbers are off by 2 u^2 at most, so all but the output's
+    rounding is that of the scores: 2 u |o| + (2^-14 + 4 u^2) m, m the softmax-weighted mean of |v|."""
+    b = Batch(46, [1 + i for i in range(30)], prefix=prefix, heads=(4, 4), dim=dim, dtype=dtype)
+    out = b.run().double()
+    exact, mag = b.exact()
+    u = U[dtype]
+    bound = 2 * u * exact.abs() + (2.0 ** -14 + 4 * u * u) * mag + (2.0 ** -25 if dtype == torch.float16 else 0)
+    assert ((out - exact).abs() <= bound).all(), ((out - exact).abs() / bound).max().item()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("queries,lengths,prefix", [(None, [600, 333, 4000, 7], 0), (None, [600, 333, 40, 7], 1100), ([2, 3], [600, 333], 0),
                                                     ([300, 400], [600, 433], 0), ([64], [4000], 100)])
 @pytest.mark.parametrize("size", [2048.0, 8192.0])
