@@ -72,8 +72,8 @@ int64_t jv_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_
 
 /*
  * Attention of a batch over the cache. Sequence b has the tokens starts[b] ..
- * starts[b + 1] - 1 of q (starts: int32 [batch + 1], not decreasing from 0; NULL: one
- * token each, tokens = batch) and lengths[b] own keys (int32), which lie in
+ * starts[b + 1] - 1 of q (starts: int32 [batch + 1], not decreasing, from 0 to
+ * tokens; NULL: one token each, tokens = batch) and lengths[b] own keys (int32), which lie in
  * the pages table[b * table_stride ..] in order; its token i of n sees the own
  * keys up to lengths[b] - n + i, and the first prefix_len keys of the pages
  * prefix_pages, which the whole batch shares (prefix_len 0: none). Query head h

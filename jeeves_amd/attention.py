@@ -246,8 +246,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     Sequence b of the batch owns the first ``lengths[b]`` keys of the pages
     ``page_table[b]`` ([batch, columns]); its queries are the tokens
     ``query_starts[b]`` to ``query_starts[b + 1] - 1`` ([batch + 1], not
-    decreasing from 0; None: one token each), the last of them at its last key:
-    query i of n sees the own keys up to ``lengths[b] - n + i``. With
+    decreasing, from 0 to tokens; None: one token each), the last of them at
+    its last key: query i of n sees the own keys up to ``lengths[b] - n + i``. With
     ``prefix_length`` all queries of the batch also see that many keys of
     ``prefix_pages``, which come before all own ones; where each sequence has
     few queries they are read once for the batch, not once for each sequence.

@@ -596,11 +596,13 @@ __device__ __forceinline__ float with_non_finite(float o, const NonFinite<D>& n,
 // Partial results that a thread has in flight when it joins them.
 constexpr int kJoinAhead = 8;
 
-// Tokens that belong to no sequence come out as 0: those past the last start.
+// Tokens that belong to no sequence come out as 0: those before the first start
+// and past the last.
 template <int D>
 __device__ __forceinline__ void zero_loose_tokens(const AttnArgs& a, int head, int threads) {
-  const int end = a.starts ? clamped(read_only(a.starts, a.batch), 0, a.tokens) : a.tokens;
-  for (int t = end; t < a.tokens; ++t)
+  if (!a.starts) return;
+  const int first = clamped(read_only(a.starts, 0), 0, a.tokens), end = clamped(read_only(a.starts, a.batch), first, a.tokens);
+  for (int t = first > 0 ? 0 : end; t < a.tokens; t = t + 1 == first ? end : t + 1)
     for (int i = threadIdx.x; i < a.group * D; i += threads) a.out[((int64_t)t * a.q_heads + head * a.group) * D + i] = 0;
 }
 

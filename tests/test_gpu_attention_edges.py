@@ -234,3 +234,22 @@ def test_rotation_needs_a_table():
             qk_norm_rope(q, k, rope, pos)
         with pytest.raises(ValueError):
             append_kv(cache, k, k, pos, rope=rope, positions=pos)
+
+
+# ---------------------------------------------------------------------------
+# tokens of no sequence
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("queries,heads,prefix", [([3, 4], (8, 2), 0), ([3, 4], (8, 2), 50), ([300, 500, 400], (64, 32), 0), ([64], (8, 2), 0)])
+def test_tokens_before_the_first_sequence_are_zero(queries, heads, prefix):
+    from jeeves_amd.attention import paged_attention
+
+    b = Batch(51, [n + 900 for n in queries], queries, heads=heads, prefix=prefix)
+    one = torch.ones(1, *b.q.shape[1:], dtype=b.dtype, device=DEV)
+    padded = torch.cat([one.expand(5, -1, -1), b.q, one.expand(3, -1, -1)])
+    dirty = [torch.full_like(padded, math.nan) for _ in range(8)]  # what the output's memory may have held before
+    del dirty
+    out = paged_attention(padded, b.cache, b.table, b.device_lengths, query_starts=b.starts + 5,
+                          prefix_pages=b.prefix_pages if prefix else None, prefix_length=prefix)
+    assert (out[:5] == 0).all() and (out[-3:] == 0).all()
+    exact, mag = b.exact()
+    assert ((out[5:-3].double() - exact).abs() <= 2 * U[b.dtype] * (exact.abs() + mag) + 2.0 ** -14 * mag).all()
