@@ -253,3 +253,39 @@ def test_tokens_before_the_first_sequence_are_zero(queries, heads, prefix):
     assert (out[:5] == 0).all() and (out[-3:] == 0).all()
     exact, mag = b.exact()
     assert ((out[5:-3].double() - exact).abs() <= 2 * U[b.dtype] * (exact.abs() + mag) + 2.0 ** -14 * mag).all()
+
+
+def device_time(f):
+    """Best time of a call in us on the device: ten runs of four in a graph."""
+    s = torch.cuda.Stream()
+    times = []
+    with torch.cuda.stream(s):
+        f()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            for _ in range(4):
+                f()
+        for _ in range(10):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record(s)
+            graph.replay()
+            b.record(s)
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b) * 250)
+    return min(times)
+
+
+@pytest.mark.parametrize("queries,heads", [([100], (32, 8)), ([10] * 64, (8, 8)), ([1500, 600], (32, 8))])
+def test_padding_costs_no_more_than_filling_the_output(queries, heads):
+    """A batch padded to 16384 tokens: four times the call without the padding and the fill of the output, and 30 us, are
+    margin enough for tokens cleared by all workgroups and not for tokens cleared by one a head, 1800 us."""
+    from jeeves_amd.attention import paged_attention
+
+    b = Batch(53, queries, queries, heads=heads)
+    padded = torch.zeros(16384, *b.q.shape[1:], dtype=b.dtype, device=DEV)
+    padded[:b.q.shape[0]] = b.q
+    fill = torch.empty_like(padded)
+    limit = 4 * (device_time(b.run) + device_time(fill.zero_)) + 30
+    took = device_time(lambda: paged_attention(padded, b.cache, b.table, b.device_lengths, query_starts=b.starts))
+    assert took <= limit, (took, limit)
