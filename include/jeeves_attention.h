@@ -14,7 +14,8 @@
  * The cache is two contiguous arrays [pages, kv_heads, page_size, dim], the
  * page size a power of two from 16 to 1024. Token `offset` of page `page` is
  * slot page * page_size + offset. A call takes less than 2^28 rows (tokens times
- * heads of q, k and v) and queries that can see up to 2^30 keys.
+ * heads of q, k and v) and queries that can see up to 2^30 keys, in all fewer
+ * than 2^35 for the row tiles of a call that splits its keys over workgroups.
  */
 #ifndef JEEVES_ATTENTION_H
 #define JEEVES_ATTENTION_H

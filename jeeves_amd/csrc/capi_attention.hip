@@ -155,8 +155,7 @@ int jv_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k_
   if (!starts && tokens != batch)
     return fail(JV_ERR_VALUE, "without query starts each of the %lld sequences has one token, got %lld", (long long)batch,
                 (long long)tokens);
-  if (table_cols < 0 || table_stride < 0 || table_cols > kMaxKeys / page_size || table_cols * page_size + prefix_len > kMaxKeys ||
-      (batch + tokens * (q_heads / kv_heads) / 16) * ((table_cols * page_size + prefix_len) / 16 + 1) > INT32_MAX)
+  if (table_cols < 0 || table_stride < 0 || table_cols > kMaxKeys / page_size || table_cols * page_size + prefix_len > kMaxKeys)
     return fail(JV_ERR_VALUE, "page table of %lld columns for a batch of %lld is too large", (long long)table_cols, (long long)batch);
   if (tokens == 0) return JV_OK;
   if (batch == 0) return fail(JV_ERR_VALUE, "%lld tokens of no sequence", (long long)tokens);
@@ -171,6 +170,9 @@ int jv_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k_
   const int64_t need = jv::attention_workspace(a.p, batch, kv_heads, dim);
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
     return fail(JV_ERR_VALUE, "workspace needs %lld bytes, 256-byte aligned", (long long)need);
+  // where keys are split, the 32-bit sum of the tiles' keys in steps of 16 and more
+  if (a.p.split && a.p.tiles * ((table_cols * page_size + prefix_len) / 16 + 1 + a.p.tiles) > INT32_MAX)
+    return fail(JV_ERR_VALUE, "page table of %lld columns for a batch of %lld is too large", (long long)table_cols, (long long)batch);
   const int64_t units = (int64_t)a.p.own_units * kv_heads, shares = (int64_t)a.p.prefix_tiles * a.p.prefix_splits * kv_heads;
   if (units + shares >= int64_t(1) << 24 || (shares && tokens * q_heads >= int64_t(1) << 26))
     return fail(JV_ERR_VALUE, "too many rows for one call: %lld tokens, %lld heads", (long long)tokens, (long long)q_heads);

@@ -90,3 +90,10 @@ def test_narrowing_refuses(product_lib):
         assert narrow(src, rows, cols, cols, 1, dst, None) == _lib.JV_ERR_VALUE
     assert narrow(None, 0, 3, 3, 1, None, None) == _lib.JV_OK
     assert narrow(None, 3, 0, 0, 1, None, None) == _lib.JV_OK
+
+
+@pytest.mark.parametrize("tokens,columns", [(1 << 20, 1 << 16), (300000, 18750), (32768, 1 << 18)])
+def test_long_prompts_are_not_refused_for_their_table(product_lib, tokens, columns):
+    """Prompts whose row tiles stay whole add no keys up: such a call gets as far as the missing lengths."""
+    assert attention(product_lib, tokens=tokens, batch=1, columns=columns, q_heads=32, kv_heads=4, lengths=None) == _lib.JV_ERR_VALUE
+    assert b"lengths" in product_lib.jv_fp8_last_error()

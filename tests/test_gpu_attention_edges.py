@@ -223,6 +223,28 @@ def test_wide_indices_are_held_in_range_before_they_are_narrowed():
                        paged_attention(b.q, b.cache, held, b.device_lengths, query_starts=b.starts))
 
 
+def test_a_long_prompt_under_a_wide_table():
+    """32768 queries of 16 rows each in a table of 2^20 keys: 2^31 tiles times steps of 16 keys, of which none are added up."""
+    from jeeves_amd.attention import paged_attention
+
+    n, length, dim, page = 32768, 33000, 64, 16
+    g = gen(54)
+    cache = new_cache(g, 2100, 1, page, dim)
+    q = randn(g, n, 16, dim)
+    table = torch.zeros(1, 65536, dtype=torch.int32, device=DEV)
+    table[0, :2063] = torch.randperm(2100, generator=g, device=DEV)[:2063]
+    out = paged_attention(q, cache, table, torch.tensor([length], dtype=torch.int32, device=DEV),
+                          query_starts=torch.tensor([0, n], dtype=torch.int32, device=DEV))
+    ids = table[0, :2063].long()
+    k, v = (x[ids, 0].flatten(0, 1)[:length].double() for x in (cache.k, cache.v))
+    rows = torch.tensor([0, 1, 127, 128, 9999, 20000, 32000, n - 1], device=DEV)
+    score = (q[rows].double() @ k.t()) * dim ** -0.5
+    score.masked_fill_(torch.arange(length, device=DEV) > (length - n + rows)[:, None, None], -math.inf)
+    p = torch.softmax(score, -1)
+    exact, mag = p @ v, p @ v.abs()
+    assert ((out[rows].double() - exact).abs() <= 2 * U[out.dtype] * (exact.abs() + mag) + 2.0 ** -14 * mag).all()
+
+
 def test_rotation_needs_a_table():
     from jeeves_amd.attention import append_kv, qk_norm_rope, rope_table
 
