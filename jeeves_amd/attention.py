@@ -334,9 +334,9 @@ class FP8Attention(nn.Module):
         ``paged_attention``'s."""
         tokens, q_size, kv_size = x.shape[0], self.q_heads * self.head_dim, self.kv_heads * self.head_dim
         q, k, v = self.qkv(x).split([q_size, kv_size, kv_size], 1)
-        q = append_kv(cache, k.view(tokens, self.kv_heads, -1), v.view(tokens, self.kv_heads, -1), slots, rope=rope,
-                      positions=positions, k_weight=self.k_weight, q=q.view(tokens, self.q_heads, -1), q_weight=self.q_weight,
-                      eps=self.eps)
+        q = append_kv(cache, k.view(tokens, self.kv_heads, self.head_dim), v.view(tokens, self.kv_heads, self.head_dim), slots,
+                      rope=rope, positions=positions, k_weight=self.k_weight, q=q.view(tokens, self.q_heads, self.head_dim),
+                      q_weight=self.q_weight, eps=self.eps)
         y = paged_attention(q, cache, page_table, lengths, query_starts=query_starts, prefix_pages=prefix_pages,
                             prefix_length=prefix_length)
         return self.o(y.view(tokens, q_size))

@@ -311,3 +311,29 @@ def test_padding_costs_no_more_than_filling_the_output(queries, heads):
     limit = 4 * (device_time(b.run) + device_time(fill.zero_)) + 30
     took = device_time(lambda: paged_attention(padded, b.cache, b.table, b.device_lengths, query_starts=b.starts))
     assert took <= limit, (took, limit)
+
+
+# ---------------------------------------------------------------------------
+# the block
+# ---------------------------------------------------------------------------
+def block_of(g, hidden=1024, hq=8, hk=2, dim=128):
+    from jeeves_amd import FP8Linear
+    from jeeves_amd.attention import FP8Attention
+
+    parts = [FP8Linear(hidden, n * dim, device=DEV) for n in (hq, hk, hk)]
+    o = FP8Linear(hq * dim, hidden, device=DEV)
+    for m in (*parts, o):
+        m.load_weight(randn(g, m.out_features, m.in_features) * 0.03)
+    return FP8Attention(FP8Linear.concatenated(parts), o, hq, hk)
+
+
+def test_attention_block_of_no_tokens():
+    from jeeves_amd.attention import PagedKVCache
+
+    block = block_of(gen(52))
+    cache = PagedKVCache.allocate(4, 2, 16, 128)
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    x = torch.empty(0, 1024, dtype=torch.bfloat16, device=DEV)
+    assert block(x, cache, none, none.view(0, 3), none).shape == (0, 1024)
+    starts = torch.zeros(3, dtype=torch.int32, device=DEV)
+    assert block(x, cache, none, torch.zeros(2, 3, dtype=torch.int32, device=DEV), starts[:2], query_starts=starts).shape == (0, 1024)
