@@ -70,6 +70,9 @@ int jv_narrow_indices(const int64_t* src, int64_t rows, int64_t cols, int64_t ro
  * device (0: none); -1 if it cannot be queried or the sizes are refused. */
 int64_t jv_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
                                            int64_t prefix_len, int ragged);
+/* Counters that it needs (0: none, they may be NULL); -1 as above. */
+int64_t jv_paged_attention_counters_needed(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                                           int64_t prefix_len, int ragged);
 
 /*
  * Attention of a batch over the cache. Sequence b has the tokens starts[b] ..

@@ -59,6 +59,7 @@ SIGNATURES: dict[str, tuple] = {
                              c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p]),
     "jv_narrow_indices": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
     "jv_paged_attention_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int]),
+    "jv_paged_attention_counters_needed": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int]),
     "jv_paged_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                    c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_float, c_void_p, c_int64, c_int64, c_int64,
                                    c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),

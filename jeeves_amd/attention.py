@@ -216,12 +216,14 @@ def append_kv(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, slots: torc
 
 
 @lru_cache(maxsize=4096)
-def _workspace(index: int, tokens: int, batch: int, q_heads: int, kv_heads: int, dim: int, prefix: int, ragged: bool) -> int:
-    """Workspace bytes for these sizes on a device, which is current; 0: none, and no counters."""
-    n = _lib.lib().jv_paged_attention_workspace_bytes(tokens, batch, q_heads, kv_heads, dim, prefix, ragged)
-    if n < 0:
+def _plan(index: int, tokens: int, batch: int, q_heads: int, kv_heads: int, dim: int, prefix: int, ragged: bool) -> tuple[int, int]:
+    """(workspace bytes, counters) for these sizes on a device, which is current."""
+    L = _lib.lib()
+    sizes = (L.jv_paged_attention_workspace_bytes(tokens, batch, q_heads, kv_heads, dim, prefix, ragged),
+             L.jv_paged_attention_counters_needed(tokens, batch, q_heads, kv_heads, dim, prefix, ragged))
+    if min(sizes) < 0:
         raise ValueError(f"the attention does not take {tokens} tokens of {batch} sequences, {q_heads} and {kv_heads} heads")
-    return n
+    return sizes
 
 
 def _int32(name: str, t: torch.Tensor, shape: tuple, index: int) -> torch.Tensor:
@@ -264,7 +266,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
 
     As a split-K GEMM of ``jeeves_amd.fp8`` does, a call whose keys are split
     over workgroups counts them in on the stream's tile counters, so run one on
-    a stream before capturing a graph on it.
+    a stream before capturing a graph on it. (Single tokens over a prefix need
+    none.)
     """
     dtype, index, tokens, dim = _first("q", q)
     cache.check(dtype, index, dim)
@@ -293,12 +296,13 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if tokens:
         with _on(index):
-            ws_bytes = _workspace(index, tokens, batch, q_heads, kv_heads, dim, prefix_length, query_starts is not None)
+            ws_bytes, counted = _plan(index, tokens, batch, q_heads, kv_heads, dim, prefix_length, query_starts is not None)
             ws_ptr, counters_ptr, n_counters = None, None, 0
             if ws_bytes:
                 ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-                counters = _stream_counters(q.device)
-                ws_ptr, counters_ptr, n_counters = ws.data_ptr(), counters.data_ptr(), TILE_COUNTER_SLOTS
+                ws_ptr = ws.data_ptr()
+            if counted:
+                counters_ptr, n_counters = _stream_counters(q.device).data_ptr(), TILE_COUNTER_SLOTS
             _lib.check(_lib.lib().jv_paged_attention(
                 q_ptr, q_ts, q_hs, cache.k.data_ptr(), cache.v.data_ptr(), cache.pages, cache.page_size, page_table.data_ptr(),
                 page_table.stride(0), columns, lengths.data_ptr(), starts_ptr, batch, prefix_ptr, prefix_length,

@@ -70,6 +70,11 @@ int check_batch(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads
   return JV_OK;
 }
 
+// Counters of a plan: one a unit and key head, where the last unit of a tile joins its parts.
+int64_t counters_of(const jv::AttnPlan& p, int64_t kv_heads) {
+  return p.split && !p.prefix_tiles ? p.own_units * kv_heads : 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -143,6 +148,15 @@ int64_t jv_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_
                                  kv_heads, dim);
 }
 
+int64_t jv_paged_attention_counters_needed(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                                           int64_t prefix_len, int ragged) {
+  if (check_batch(tokens, batch, q_heads, kv_heads, dim, prefix_len)) return -1;
+  if (tokens == 0 || batch == 0) return 0;
+  const int cus = jv::cu_count_of(-1);
+  if (cus <= 0) return -1;
+  return counters_of(jv::attention_plan(tokens, batch, q_heads, kv_heads, dim, prefix_len, ragged != 0, cus), kv_heads);
+}
+
 int jv_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k_pages, const void* v_pages, int64_t pages,
                        int64_t page_size, const int32_t* table, int64_t table_stride, int64_t table_cols,
                        const int32_t* lengths, const int32_t* starts, int64_t batch, const int32_t* prefix_pages,
@@ -176,8 +190,8 @@ int jv_paged_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k_
   const int64_t units = (int64_t)a.p.own_units * kv_heads, shares = (int64_t)a.p.prefix_tiles * a.p.prefix_splits * kv_heads;
   if (units + shares >= int64_t(1) << 24 || (shares && tokens * q_heads >= int64_t(1) << 26))
     return fail(JV_ERR_VALUE, "too many rows for one call: %lld tokens, %lld heads", (long long)tokens, (long long)q_heads);
-  if (a.p.split && !shares && (!counters || n_counters < units))
-    return fail(JV_ERR_VALUE, "%lld units exceed the %lld counters", (long long)units, (long long)n_counters);
+  if (const int64_t n = counters_of(a.p, kv_heads); n && (!counters || n_counters < n))
+    return fail(JV_ERR_VALUE, "%lld units exceed the %lld counters", (long long)n, (long long)n_counters);
   a.counters = counters;
   a.q = (const uint16_t*)q, a.q_ts = q_ts, a.q_hs = q_hs;
   a.k_pages = (const uint16_t*)k_pages, a.v_pages = (const uint16_t*)v_pages;

@@ -97,3 +97,9 @@ def test_long_prompts_are_not_refused_for_their_table(product_lib, tokens, colum
     """Prompts whose row tiles stay whole add no keys up: such a call gets as far as the missing lengths."""
     assert attention(product_lib, tokens=tokens, batch=1, columns=columns, q_heads=32, kv_heads=4, lengths=None) == _lib.JV_ERR_VALUE
     assert b"lengths" in product_lib.jv_fp8_last_error()
+
+
+def test_counters_of_refused_and_empty_calls(product_lib):
+    need = product_lib.jv_paged_attention_counters_needed
+    assert need(0, 3, 8, 2, 128, 0, 1) == 0 and need(4, 0, 8, 2, 128, 0, 1) == 0
+    assert need(4, 2, 7, 2, 128, 0, 1) == -1 and need(4, 2, 8, 2, 96, 0, 1) == -1 and need(4, 2, 8, 2, 128, -1, 1) == -1

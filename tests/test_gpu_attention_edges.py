@@ -314,6 +314,33 @@ def test_padding_costs_no_more_than_filling_the_output(queries, heads):
 
 
 # ---------------------------------------------------------------------------
+# capture
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("queries,lengths,prefix,heads", [(None, [70, 5, 200], 100, (8, 2)), (None, [70] * 40, 1100, (8, 2)),
+                                                          ([300, 500, 400], [300, 520, 400], 0, (64, 32))])
+def test_what_counts_nothing_is_captured_on_a_new_stream(queries, lengths, prefix, heads):
+    """Single tokens over a prefix, whose parts a launch of its own joins, and whole tiles: no counters to make first.
+    Replayed between eager work, with other queries."""
+    from jeeves_amd.fp8 import TILE_COUNTERS
+
+    b = Batch(55, lengths, queries, prefix=prefix, heads=heads)
+    b.run()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(64)]
+    s = next((s for s in streams if (torch.device("cuda", s.device_index), s.cuda_stream) not in TILE_COUNTERS), streams[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        out = b.run()
+    g = gen(56)
+    for _ in range(4):
+        b.q.copy_(randn(g, *b.q.shape))
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, b.run())
+        torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------------------
 # the block
 # ---------------------------------------------------------------------------
 def block_of(g, hidden=1024, hq=8, hk=2, dim=128):
