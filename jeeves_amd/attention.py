@@ -26,6 +26,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from .device import sm_count
 from .fp8 import _CURRENT, TILE_COUNTER_SLOTS, FP8Linear, _stream_counters
 
 HEAD_DIMS = (64, 128, 256)
@@ -329,6 +330,32 @@ class FP8Attention(nn.Module):
         for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
             self.register_buffer(name, None if w is None else w.detach().to(torch.float32))
         self.eps = eps
+
+    @torch.no_grad()
+    def warm(self) -> None:
+        """Runs the block's operators in each of their forms on empty sequences,
+        as ``jeeves_amd.fp8.warm`` runs its linears: kernels load and the
+        stream's counters exist before graph capture."""
+        device, dim, group = self.qkv.weight.device, self.head_dim, self.q_heads // self.kv_heads
+        cache = PagedKVCache.allocate(1, self.kv_heads, 16, dim, device=device)
+
+        def batch(sequences: int, queries: int, prefix: int) -> None:
+            tokens = sequences * queries
+            q = torch.zeros(tokens, self.q_heads, dim, dtype=torch.bfloat16, device=device)
+            none = torch.zeros(sequences, 1, dtype=torch.int32, device=device)
+            starts = torch.arange(0, tokens + 1, queries, dtype=torch.int32, device=device) if queries > 1 else None
+            paged_attention(q, cache, none, none[:, 0], query_starts=starts, prefix_pages=none[0] if prefix else None,
+                            prefix_length=prefix)
+
+        k = torch.zeros(1, self.kv_heads, dim, dtype=torch.bfloat16, device=device)
+        append_kv(cache, k, k, torch.full((1,), -1, dtype=torch.int32, device=device),
+                  q=torch.zeros(1, self.q_heads, dim, dtype=torch.bfloat16, device=device))
+        many = 16 // group + 1  # queries of more than 16 rows
+        batch(1, 1, 0)
+        batch(1, 1, 16)
+        batch(33, 1, 16)
+        batch(1, max(many, 2), 0)
+        batch(2 * sm_count(device) + 1, max(many, 2), 0)  # more row tiles than workgroups at a time: whole ones
 
     def forward(self, x: torch.Tensor, cache: PagedKVCache, slots: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, *,
                 rope: torch.Tensor | None = None, positions: torch.Tensor | None = None, query_starts: torch.Tensor | None = None,

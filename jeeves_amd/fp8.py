@@ -874,9 +874,14 @@ def load_view(model: str, drafter: str, block: int, device: torch.device):
 def warm(module: nn.Module) -> int:
     """``inference/fp8.py:194-203``: run every distinct (N, K) at ``WARM_ROWS``
     so each kernel variant has loaded and each stream's tile counters exist
-    before graph capture."""
+    before graph capture; attention blocks run their own operators. Returns the
+    number of distinct (N, K)."""
+    from .attention import FP8Attention  # which imports this module
+
     seen = set()
     for m in module.modules():
+        if isinstance(m, FP8Attention):
+            m.warm()
         if isinstance(m, FP8Linear) and (m.out_features, m.in_features) not in seen:
             seen.add((m.out_features, m.in_features))
             w = m.weight

@@ -364,3 +364,42 @@ def test_attention_block_of_no_tokens():
     assert block(x, cache, none, none.view(0, 3), none).shape == (0, 1024)
     starts = torch.zeros(3, dtype=torch.int32, device=DEV)
     assert block(x, cache, none, torch.zeros(2, 3, dtype=torch.int32, device=DEV), starts[:2], query_starts=starts).shape == (0, 1024)
+
+
+def test_warm_prepares_the_block_for_capture():
+    """warm(block) on a stream, then a step of single tokens, whose keys are split, captured on it; no linear of these
+    sizes counts."""
+    from jeeves_amd import warm
+    from jeeves_amd.attention import PagedKVCache
+    from jeeves_amd.fp8 import TILE_COUNTERS
+
+    g = gen(57)
+    block = block_of(g, 6144, 32, 8)
+    cache = PagedKVCache.allocate(12, 8, 16, 128)
+    x = randn(g, 3, 6144)
+    table = torch.arange(12, dtype=torch.int32, device=DEV).view(3, 4)
+    lengths = torch.tensor([1, 17, 64], dtype=torch.int32, device=DEV)
+    slots = table.gather(1, (lengths.long()[:, None] - 1) // 16)[:, 0] * 16 + (lengths - 1) % 16
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(64)]
+    s = next((s for s in streams if (torch.device("cuda", s.device_index), s.cuda_stream) not in TILE_COUNTERS), streams[0])
+    with torch.cuda.stream(s):
+        assert warm(block) == 2
+    torch.cuda.synchronize()
+    assert (cache.k == 0).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        out = block(x, cache, slots, table, lengths)
+    for _ in range(4):
+        x.copy_(randn(g, 3, 6144))
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, block(x, cache, slots, table, lengths))
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("hq,hk,dim", [(4, 4, 64), (32, 1, 64), (16, 4, 256)])
+def test_warm_of_other_head_layouts(hq, hk, dim):
+    block = block_of(gen(58), 256, hq, hk, dim)
+    block.warm()
+    torch.cuda.synchronize()
