@@ -84,7 +84,8 @@ int64_t jv_paged_attention_counters_needed(int64_t tokens, int64_t batch, int64_
  * reads kv head h / (q_heads / kv_heads). out [tokens, q_heads, dim],
  * contiguous, is the softmax-weighted sum of the values, scores times `scale`;
  * 0 where a token sees no key or belongs to no sequence. Keys that a token
- * does not see have no effect, whatever their values. Lengths are taken up to
+ * does not see have no effect, whatever their values; a NaN score that it sees
+ * makes its row NaN, a NaN value the channel. Lengths are taken up to
  * the table's width, page ids into the cache's range.
  * workspace: 256-byte aligned. counters: int32, JV_ATTENTION_COUNTERS of them
  * serve every call; zero before the first call and left at zero by each, one

@@ -260,7 +260,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     A token that sees no key, or that belongs to no sequence, comes out as 0.
     Keys that a token does not see have no effect on it, even infinite or NaN
     ones; nor has what the table holds past a sequence's length, nor the other
-    sequences. The sums are in 32 bits; where many query rows go through the same
+    sequences' keys (their lengths decide how keys are cut, which can change a
+    token's last bits). A NaN that it sees stays NaN. The sums are in 32 bits; where many query rows go through the same
     keys (prompts, a prefix that many sequences share) the softmax's weights
     are rounded to the 16-bit type for the product with the values, and their
     sum is of the rounded ones.
@@ -316,7 +317,9 @@ class FP8Attention(nn.Module):
     """An attention block over FP8 projections: the merged q/k/v projection
     (``FP8Linear.concatenated``, rows of all q heads, then k, then v), norms,
     rotation and append in one launch, the attention over the paged cache, and
-    the o projection."""
+    the o projection. A projection with other rows merged in, an output gate's
+    say, is not for it: split those off around ``append_kv`` and
+    ``paged_attention``."""
 
     def __init__(self, qkv: FP8Linear, o: FP8Linear, q_heads: int, kv_heads: int, q_weight: torch.Tensor | None = None,
                  k_weight: torch.Tensor | None = None, eps: float = 1e-6):

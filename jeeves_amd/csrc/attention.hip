@@ -234,12 +234,6 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 __device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
-__device__ __forceinline__ float wave_sum_f32(float v) {
-#pragma unroll
-  for (int s = 1; s < 64; s *= 2) v += __shfl_xor(v, s);
-  return v;
-}
-
 // Where keys are split over workgroups: the (sequence, row tile, key chunk) of
 // a unit, computed by each wave for itself, 64 sequences a step, from the
 // lengths on the device. `shared`: keys before the own ones that count too.
@@ -588,10 +582,11 @@ __device__ __forceinline__ float with_non_finite(float o, const NonFinite<D>& n,
 // the waves' results meet in LDS at the end. 16x16 MFMA; a lane holds row
 // lane % 16 and keys 4 (lane / 16) + 0..3 of a tile.
 //
-// 4 sequences of 32000 to 59000 keys (4 heads of 256, 719 MB) take 134 us, 5.4
-// TB/s; a ragged batch of 64 (8 heads of 128, 124 MB) 29, 4.3 TB/s: a workgroup
+// 4 sequences of 32000 to 59000 keys (4 heads of 256, 719 MB) take 128 us, 5.6
+// TB/s; a ragged batch of 64 (8 heads of 128, 124 MB) 31, 4.0 TB/s: a workgroup
 // has about 5 us of finding its unit, the first copies and the join beside its
-// keys. One sequence of 517 keys takes 9.5 us, a launch and that chain.
+// keys. One sequence of 517 keys takes 8.6 us, a launch and that chain. (Thirty
+// calls of a graph, their inputs in turn.)
 // ---------------------------------------------------------------------------
 // Partial results that a thread has in flight when it joins them.
 constexpr int kJoinAhead = 8;
@@ -881,14 +876,15 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a, int block, uint8_t
 // products of the ones before, which hides the exponentials (8% of the time
 // without that).
 //
-// Prompts of 8192 tokens take 535 us with 32 heads of 128 (1030 TFLOP/s; a large
-// bf16 library product reaches 1197), 505 with 16 of 256 (1090) and 300 with 32
-// of 64 (915). Nothing alone bounds it: of a prompt's time 25% go without the
-// first product, 25% without the second, 12% without the copies; a wave's 32 rows
-// make LDS deliver as many bytes as MFMA takes cycles. Eight waves a workgroup
-// (108 instead of 85 us for 16 sequences over a prefix of 2000) and 32-key tiles
-// at three waves a SIMD (even) were no better. Short prompts wait for HBM beside
-// it: 16 of 512 tokens move 167 MB in 72 us.
+// Prompts of 8192 tokens take 558 us with 32 heads of 128 (985 TFLOP/s; a large
+// bf16 library product reaches 1200 beside it), 535 with 16 of 256 (1025) and 326
+// with 32 of 64 (840), in thirty calls of a graph. Nothing alone bounds it: with
+// 32 heads of 128 MFMA is busy 48% of the time and LDS 24%, without conflicts, and
+// VALU instructions, the exponentials among them, take 30% at four cycles each; a
+// wave does one after the other but for what is laid between the products. Eight
+// waves a workgroup (108 instead of 85 us for 16 sequences over a prefix of 2000)
+// and 32-key tiles at three waves a SIMD (even) were no better. Short prompts wait
+// for HBM beside it: 16 of 512 tokens move 167 MB in 73 us.
 // ---------------------------------------------------------------------------
 template <int D>
 struct Many {
@@ -1182,8 +1178,9 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttnArgs a) {
 
 // A decode batch with a prefix: shares of the prefix for all rows (the first
 // workgroups) and chunks of the sequences' own keys side by side. 64 sequences
-// (32 heads of 128) over 8192 keys: 20 us, a share 16.6 of them for 8 key tiles,
-// and 5.3 of the join; in two launches, the own keys' after the prefix's, 6 more.
+// (32 heads of 128) over 8192 keys: 22 us, a share of 8 key tiles most of them, and
+// 6 of the join, which reads the 18 MB of parts that this kernel writes beside
+// the case's 48 MB; in two launches, the own keys' after the prefix's, 6 more.
 template <class H, int D, bool FEW_PREFIX>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_shared_kernel(AttnArgs a) {
   constexpr int LDS = FEW_PREFIX || Few<D>::kLds > Many<D>::kLds ? Few<D>::kLds : Many<D>::kLds;
