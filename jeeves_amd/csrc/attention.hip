@@ -16,7 +16,10 @@
 // without for the ragged 64 below, 133.5 both for the long ones). In tiles of
 // many rows, where MFMA is half the time, weights are rounded (a relative 2^-8
 // or 2^-11 at most for bf16 and fp16, of mixed signs) and their sum is that of
-// the rounded ones, by one instruction a pair. fp16 weights are 2^7 larger, up
+// the rounded ones, by one instruction a pair: a second product there takes 740
+// us instead of 532 for a prompt of 8192 tokens, 104 instead of 83 for questions
+// after a prefix, 32.3 instead of 30.6 for 64 tokens over a prefix of 8192, and
+// brings the relative error from 2.3e-3 to the 1.7e-3 of the output's rounding. fp16 weights are 2^7 larger, up
 // to 2^15, so that those that many keys share stay normal numbers.
 //
 // Both products run on MFMA with the keys on the A side: S^T = K Q^T leaves
