@@ -18,9 +18,10 @@
 // or 2^-11 at most for bf16 and fp16, of mixed signs) and their sum is that of
 // the rounded ones, by one instruction a pair: a second product there takes 740
 // us instead of 532 for a prompt of 8192 tokens, 104 instead of 83 for questions
-// after a prefix, 32.3 instead of 30.6 for 64 tokens over a prefix of 8192, and
-// brings the relative error from 2.3e-3 to the 1.7e-3 of the output's rounding. fp16 weights are 2^7 larger, up
-// to 2^15, so that those that many keys share stay normal numbers.
+// after a prefix, 32.3 instead of 30.6 for 64 tokens over a prefix of 8192, where
+// the output's own rounding is 1.7e-3 of the 2.3e-3 that bf16 outputs are off by.
+// fp16 weights are 2^7 larger, up to 2^15, so that those that many keys share
+// stay normal numbers.
 //
 // Both products run on MFMA with the keys on the A side: S^T = K Q^T leaves
 // each lane the scores of one query row, and the score tile's registers are,
