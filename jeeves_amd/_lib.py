@@ -15,7 +15,7 @@ LIB_PATH = Path(__file__).resolve().with_name("libjeeves_fp8.so")
 
 JV_OK, JV_ERR_VALUE, JV_ERR_RUNTIME, JV_ERR_HIP = 0, 1, 2, 3
 
-# name -> (restype, argtypes); mirrors include/jeeves_fp8.h and include/jeeves_attention.h
+# name -> (restype, argtypes); mirrors include/*.h
 SIGNATURES: dict[str, tuple] = {
     "jv_fp8_last_error": (c_char_p, []),
     "jv_device_cu_count": (c_int, [c_int]),
@@ -63,6 +63,18 @@ SIGNATURES: dict[str, tuple] = {
     "jv_paged_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                    c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_float, c_void_p, c_int64, c_int64, c_int64,
                                    c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    # include/jeeves_norm.h
+    "jv_block_norm": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_float,
+                              c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int,
+                              c_void_p]),
+    # include/jeeves_linear_attention.h
+    "jv_causal_conv": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                               c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p]),
+    "jv_linear_attention_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int]),
+    "jv_linear_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+                                    c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_float, c_void_p, c_int64, c_void_p,
+                                    c_void_p, c_void_p, c_int64, c_float, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                    c_int, c_void_p, c_int64, c_void_p]),
 }
 
 _lib = None

@@ -718,6 +718,22 @@ class FP8Linear(nn.Module):
             y = fp8_matmul(x2, w, scale, bias=self.bias, lora=self.lora, tiled=tiled)
         return y if len(shape) == 2 else y.view(*shape[:-1], self.out_features)
 
+    def takes_codes(self) -> bool:
+        """Whether ``forward_codes`` takes packed codes: per-token e4m3
+        activations, no LoRA (its x A^T needs x), rows that the packed layout
+        covers."""
+        return (self.activations == "fp8" and self.lora is None and self.in_features % BLOCK_K == 0
+                and self.in_features <= QUANT_MAX_PACKED_COLS)
+
+    def forward_codes(self, codes: torch.Tensor, scales: torch.Tensor, packed_rows: int | None = None) -> torch.Tensor:
+        """``forward`` on activations whose codes and scales another operator
+        has worked out (``add_norm``, ``gated_norm``): float8_e4m3fn [M, K], or
+        ``packed_rows=M`` rows in the packed order."""
+        if self.activations != "fp8" or self.lora is not None:
+            raise ValueError("codes go with per-token e4m3 activations and no LoRA adapter")
+        w, tiled = self.kernel_weight()
+        return fp8_matmul_quantized(codes, scales, w, self.scale, bias=self.bias, packed_rows=packed_rows, tiled=tiled)
+
 
 class FP8SwiGLU(nn.Module):
     """``SwiGLU`` (``model/model.py:574-584``) over FP8 projections: the gate
@@ -876,11 +892,12 @@ def warm(module: nn.Module) -> int:
     so each kernel variant has loaded and each stream's tile counters exist
     before graph capture; attention blocks run their own operators. Returns the
     number of distinct (N, K)."""
-    from .attention import FP8Attention  # which imports this module
+    from .attention import FP8Attention  # which import this module
+    from .linear_attention import FP8LinearAttention
 
     seen = set()
     for m in module.modules():
-        if isinstance(m, FP8Attention):
+        if isinstance(m, (FP8Attention, FP8LinearAttention)):
             m.warm()
         if isinstance(m, FP8Linear) and (m.out_features, m.in_features) not in seen:
             seen.add((m.out_features, m.in_features))
