@@ -79,6 +79,11 @@ __device__ __forceinline__ int32_t uniform_at(const int32_t* p, int i) {
   return *(constant_ptr)(uintptr_t)(p + __builtin_amdgcn_readfirstlane(i));
 }
 
+__device__ __forceinline__ float uniform_f32(const float* p, int i) {
+  typedef const __attribute__((address_space(4))) float* constant_ptr;
+  return *(constant_ptr)(uintptr_t)(p + __builtin_amdgcn_readfirstlane(i));
+}
+
 struct ConvArgs {
   const uint16_t* x;
   int64_t x_ts;

@@ -25,7 +25,6 @@
 namespace jv {
 
 constexpr int kStepCols = 32;  // columns of S that a workgroup of step_kernel has
-constexpr int kCols = 32;      // and one of scan_kernel
 
 template <class H>
 __device__ __forceinline__ float gate_at(const void* p, int wide16, int64_t i) {
@@ -33,8 +32,8 @@ __device__ __forceinline__ float gate_at(const void* p, int wide16, int64_t i) {
 }
 
 // log2 of a token's decay; what is below 2^-14400 is 0 by far.
-__device__ __forceinline__ double log2_decay(const LinearArgs& a, float z, int head) {
-  if (a.rate) z = -a.rate[head] * softplus(z + (a.decay_bias ? a.decay_bias[head] : 0.0f));
+__device__ __forceinline__ double log2_decay(float z, bool raw, float rate, float bias) {
+  if (raw) z = -rate * softplus(z + bias);
   const double g = (double)z * 1.4426950408889634;
   return g < -14400.0 ? -14400.0 : g;
 }
@@ -73,7 +72,9 @@ __global__ __launch_bounds__(256) void step_kernel(LinearArgs a, int v_dim, uint
   for (int i = 0; i < NR; ++i) kr[i] = H::lo(k[rg + 32 * i]), qr[i] = H::lo(q[rg + 32 * i]);
 #pragma unroll
   for (int i = 0; i < DK / 64; ++i) kl[i] = H::lo(k[lane + 64 * i]), ql[i] = H::lo(q[lane + 64 * i]);
-  const float decay = __builtin_amdgcn_exp2f((float)log2_decay(a, gate_at<H>(a.decay, a.gates16, seq * a.decay_ts + head), head));
+  const float rate = a.rate ? uniform_f32(a.rate, head) : 0.0f, bias = a.decay_bias ? uniform_f32(a.decay_bias, head) : 0.0f;
+  const float decay =
+      __builtin_amdgcn_exp2f((float)log2_decay(gate_at<H>(a.decay, a.gates16, seq * a.decay_ts + head), a.rate != nullptr, rate, bias));
   const float beta = a.beta ? beta_of(a, gate_at<H>(a.beta, a.gates16, seq * a.beta_ts + head)) : 1.0f;
   float kk = 0.0f, qq = 0.0f, qk = 0.0f;
 #pragma unroll
@@ -132,11 +133,11 @@ __global__ __launch_bounds__(256) void step_kernel(LinearArgs a, int v_dim, uint
 typedef short bits8 __attribute__((ext_vector_type(8)));
 
 // A chunk's data for a value head in the workspace, in fragments of 64 lanes
-// of 16 bytes: T [row tile][32 columns][3 parts], M [row tile][32 columns]
-// [2 parts], then the rows' factors.
+// of 16 bytes: T [lower fragment][3 parts], M [lower fragment][2 parts], then
+// the rows' factors.
 constexpr int kFragment = 1024;
-constexpr int kBytesT = 4 * 2 * 3 * kFragment, kBytesM = 4 * 2 * 2 * kFragment;
-enum { kFromK, kFromQ, kBeta, kToEnd, kEnd, kFactors };  // [kFactors][64] floats; kEnd: the whole chunk's decay
+constexpr int kBytesT = 6 * 3 * kFragment, kBytesM = 6 * 2 * kFragment;
+enum { kFromK, kFromQ, kBeta, kToEnd, kEnd, kFactors = 8 };  // [8][64] floats; kEnd: the whole chunk's decay
 constexpr int kBytesHead = kBytesT + kBytesM + kFactors * kChunk * 4;
 
 // K's transpose for a key head: [DK / 16][32 tokens] fragments.
@@ -154,14 +155,33 @@ __device__ __forceinline__ uint8_t* key_data(const LinearArgs& a, int chunk, int
          ((int64_t)chunk * a.k_heads + kh) * bytes_kt(k_dim);
 }
 
-// Two fp32 values as sums of bf16 ones: x = p0 + p1 + p2 to 24 bits.
+// Two fp32 values as sums of bf16 ones: x = p0 + p1 + p2 to 24 bits. What a
+// rounding leaves is exact in fp32: one v_dot2_f32_bf16 with (-1, 0) or (0, -1).
+// The pairs come from registers: as a constant the compiler writes the first
+// one as the operand -1.0, which the instruction takes for the second.
 template <int N>
 __device__ __forceinline__ void split2(float x, float y, uint32_t (&p)[N]) {
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  uint32_t low, high;
+  asm("s_mov_b32 %0, 0xbf80" : "=s"(low));
+  asm("s_mov_b32 %0, 0xbf800000" : "=s"(high));
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     p[i] = Bf16::pack(x, y);
-    x -= Bf16::lo(p[i]), y -= Bf16::hi(p[i]);
+    if (i + 1 < N) {
+      x = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair, p[i]), __builtin_bit_cast(pair, low), x, false);
+      y = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair, p[i]), __builtin_bit_cast(pair, high), y, false);
+    }
   }
+}
+
+// Two tiles' sums as a right operand's 32 rows.
+template <int N>
+__device__ __forceinline__ void split8(f32x4 x, f32x4 y, i32x4 (&f)[N]) {
+  uint32_t p[4][N];
+  split2<N>(x[0], x[1], p[0]), split2<N>(x[2], x[3], p[1]), split2<N>(y[0], y[1], p[2]), split2<N>(y[2], y[3], p[3]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] = i32x4{(int)p[0][i], (int)p[1][i], (int)p[2][i], (int)p[3][i]};
 }
 
 // A fragment of the tensors' type as bf16 ones whose sum it is.
@@ -187,17 +207,58 @@ struct Parts<Fp16> {
 
 __device__ __forceinline__ int clamp_to(int v, int hi) { return min(max(v, 0), hi); }
 
+// Inclusive sums over the wave by DPP moves: row_shr 1, 2, 4, 8 within the 16
+// lanes of a row (a shifted-out source adds 0), then row_bcast 15 and 31.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, false);
+  return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sums(double v) {
+  v = dpp_add<0x111, 0xf>(v), v = dpp_add<0x112, 0xf>(v), v = dpp_add<0x114, 0xf>(v), v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);
+  return dpp_add<0x143, 0xc>(v);
+}
+
+// The products' operands T and M go by a k order of their own: in 32 columns a
+// lane's 8 are 4 g .. 4 g + 3 and 16 + 4 g .., g = lane / 16, which is what the
+// four registers of two products' results hold. Row i of D and U then lies at
+// place(i).
+__device__ __forceinline__ int place_of(int i) { return (i & ~31) + ((i >> 2) & 3) * 8 + ((i >> 4) & 1) * 4 + (i & 3); }
+
+// S's rows in the tiles of its sums: a tile's rows 4 g .. 4 g + 3 are the lanes'
+// of group g, and two tiles hold 32 rows, 8 g .. 8 g + 7 a group, as the k of a
+// product with K or Q goes.
+__device__ __forceinline__ int state_row(int m, int g) { return 32 * (m >> 1) + 8 * g + 4 * (m & 1); }
+
+// The lower triangle's fragments: of row tile t the 32 columns x, x <= t / 2.
+__device__ __forceinline__ int fragment_of(int t, int x) { return x ? t + 2 : t; }
+
 template <class H, int DK, bool BETA>
-__global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a) {
-  constexpr int KS = DK / 32, kRow = 68, kRow16 = 72;
+__global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
+  constexpr int KS = DK / 32, kRow = 68, kRowK = DK + 8, kRowD = 20;
+  __shared__ __attribute__((aligned(16))) uint16_t krows[kChunk * kRowK];
   __shared__ __attribute__((aligned(16))) float tri[BETA ? kChunk * kRow : 4];
-  __shared__ __attribute__((aligned(16))) uint16_t m16[2][kChunk * kRow16];
-  __shared__ __attribute__((aligned(16))) uint16_t kt[DK * kRow16];
-  __shared__ double sum[kChunk];
-  __shared__ float rk[kChunk], rq[kChunk], betas[kChunk];
+  __shared__ __attribute__((aligned(16))) float diagonal[BETA ? 4 : 1][16 * kRowD];
+  __shared__ __attribute__((aligned(16))) double sum[kChunk];
+  __shared__ __attribute__((aligned(16))) float rk[kChunk], rq[kChunk], betas[kChunk];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int place = (int)(blockIdx.x / (uint32_t)a.v_heads), head = (int)(blockIdx.x % (uint32_t)a.v_heads), kh = head / a.group;
   const Batch& b = a.b;
+
+  // Tokens before the first sequence's and behind the last's come out as 0: of the batch's 64 from `place` x 64 on.
+  {
+    const int lo = clamp_to(uniform_at(b.starts, 0), b.tokens), hi = clamp_to(uniform_at(b.starts, b.batch), b.tokens);
+    const int at = place * kChunk, to = min(at + kChunk, b.tokens);
+    if (at < lo || to > hi)
+      for (int i = at * (v_dim / 8) + tid; i < to * (v_dim / 8); i += 256) {
+        const int t = i / (v_dim / 8);
+        if (t < lo || t >= hi)
+          *reinterpret_cast<uint4*>(a.out + ((int64_t)t * a.v_heads + head) * v_dim + i % (v_dim / 8) * 8) = uint4{0, 0, 0, 0};
+      }
+  }
 
   // the sequence whose chunk this is
   int count = 0;
@@ -215,218 +276,774 @@ __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a) {
   if (t0 < 0 || rows <= 0) return;
   const int first = start + t0;
 
-  const int r16 = lane & 15, k8 = (lane >> 4) * 8;
-  const auto fragment = [&](const uint16_t* p, int64_t ts, int64_t hs, int tile, int s) {
-    const int i = tile * 16 + r16;
-    const i32x4 v = *reinterpret_cast<const i32x4*>(p + (int64_t)(first + min(i, rows - 1)) * ts + kh * hs + s * 32 + k8);
-    return v & ((i - rows) >> 31);  // 0 behind the sequence's end
-  };
-  i32x4 kf[KS], qf[KS];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) kf[s] = fragment(a.k, a.k_ts, a.k_hs, wave, s), qf[s] = fragment(a.q, a.q_ts, a.q_hs, wave, s);
+  const int r16 = lane & 15, g = lane >> 4, k8 = g * 8;
+  float gate_d = 0.0f, gate_b = 0.0f, rate = 0.0f, bias = 0.0f;
   if (wave == 0) {
-    const int t = first + min(lane, rows - 1);
-    const bool real = lane < rows;
-    double g = real ? log2_decay(a, gate_at<H>(a.decay, a.gates16, t * a.decay_ts + head), head) : 0.0;
-#pragma unroll
-    for (int s = 1; s < 64; s *= 2) {
-      const double o = __shfl_up(g, s);
-      if (lane >= s) g += o;
+    const int64_t t = first + min(lane, rows - 1);
+    if (a.rate) rate = uniform_f32(a.rate, head), bias = a.decay_bias ? uniform_f32(a.decay_bias, head) : 0.0f;
+    if (a.gates16) {
+      const uint16_t d = reinterpret_cast<const uint16_t*>(a.decay)[t * a.decay_ts + head];
+      const uint16_t e = BETA ? reinterpret_cast<const uint16_t*>(a.beta)[t * a.beta_ts + head] : 0;
+      gate_d = H::lo(d), gate_b = H::lo(e);
+    } else {
+      gate_d = reinterpret_cast<const float*>(a.decay)[t * a.decay_ts + head];
+      if (BETA) gate_b = reinterpret_cast<const float*>(a.beta)[t * a.beta_ts + head];
     }
-    sum[lane] = g;
-    betas[lane] = !real ? 0.0f : BETA ? beta_of(a, gate_at<H>(a.beta, a.gates16, t * a.beta_ts + head)) : 1.0f;
   }
+  i32x4 kf[KS], qf[KS];
   {
+    const int i = wave * 16 + r16;
+    const int64_t t = first + min(i, rows - 1);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      kf[s] = *reinterpret_cast<const i32x4*>(a.k + t * a.k_ts + kh * a.k_hs + s * 32 + k8);
+      qf[s] = *reinterpret_cast<const i32x4*>(a.q + t * a.q_ts + kh * a.q_hs + s * 32 + k8);
+    }
+    if (wave == 0) {
+      const bool real = lane < rows;
+      const double d = wave_sums(real ? log2_decay(gate_d, a.rate != nullptr, rate, bias) : 0.0);
+      sum[lane] = d;
+      betas[lane] = !real ? 0.0f : !BETA ? 1.0f : a.rate ? sigmoid(gate_b) : gate_b;
+    }
+    if (rows < kChunk)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) kf[s] &= (i - rows) >> 31, qf[s] &= (i - rows) >> 31;  // 0 behind the sequence's end
     float sk = 0.0f, sq = 0.0f;
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+    for (int s = 0; s < KS; ++s) {
+      *reinterpret_cast<i32x4*>(&krows[i * kRowK + s * 32 + k8]) = kf[s];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float k0 = H::lo((uint32_t)kf[s][e]), k1 = H::hi((uint32_t)kf[s][e]);
         const float q0 = H::lo((uint32_t)qf[s][e]), q1 = H::hi((uint32_t)qf[s][e]);
         sk = __builtin_fmaf(k0, k0, __builtin_fmaf(k1, k1, sk)), sq = __builtin_fmaf(q0, q0, __builtin_fmaf(q1, q1, sq));
       }
-    sk += __shfl_xor(sk, 16), sk += __shfl_xor(sk, 32), sq += __shfl_xor(sq, 16), sq += __shfl_xor(sq, 32);
-    if (lane < 16) {
-      const bool norm = a.norm_eps > 0.0f;
-      rk[wave * 16 + lane] = norm ? inv_sqrt(sk + a.norm_eps) : 1.0f;
-      rq[wave * 16 + lane] = a.scale * (norm ? inv_sqrt(sq + a.norm_eps) : 1.0f);
     }
+    const bool norm = a.norm_eps > 0.0f;
+    if (norm) {
+      sk += __shfl_xor(sk, 16), sk += __shfl_xor(sk, 32), sq += __shfl_xor(sq, 16), sq += __shfl_xor(sq, 32);
+      sk = inv_sqrt(sk + a.norm_eps), sq = inv_sqrt(sq + a.norm_eps);
+    }
+    if (lane < 16) rk[i] = norm ? sk : 1.0f, rq[i] = a.scale * (norm ? sq : 1.0f);
   }
-  if (head % a.group == 0) {
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        kt[(s * 32 + k8 + e) * kRow16 + wave * 16 + r16] = (uint16_t)((uint32_t)kf[s][e >> 1] >> (16 * (e & 1)));
-  }
-  __syncthreads();
+  lds_barrier();
 
-  // A and M, 16 rows a wave, their column tiles up to the diagonal
+  // A and M transposed: a lane has row i of 16 w .. 16 w + 15 and of every
+  // column tile up to the diagonal the columns 4 g .. 4 g + 3.
+  uint8_t* out = head_data(a, place, head);
+  const int i = wave * 16 + r16;
+  const double sum_i = sum[i];
+  const float rk_i = rk[i], rq_i = rq[i], beta_i = betas[i];
+  uint2 mp[4][2];
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    if (t > (wave | 1)) break;
+    mp[t][0] = mp[t][1] = uint2{0u, 0u};
+    if (t > wave) continue;
     f32x4 kk = {0.0f, 0.0f, 0.0f, 0.0f}, qk = kk;
-    if (t <= wave) {
-      i32x4 kb[KS];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) kb[s] = fragment(a.k, a.k_ts, a.k_hs, t, s);
-#pragma unroll
-      for (int s = 0; s < KS; ++s) kk = H::mfma16(kf[s], kb[s], kk), qk = H::mfma16(qf[s], kb[s], qk);
+    for (int s = 0; s < KS; ++s) {
+      const i32x4 kb = *reinterpret_cast<const i32x4*>(&krows[(t * 16 + r16) * kRowK + s * 32 + k8]);
+      kk = H::mfma16(kb, kf[s], kk), qk = H::mfma16(kb, qf[s], qk);
     }
-    const int j = t * 16 + r16;
-    const double gj = sum[j];
-    const float rkj = rk[j];
+    const f32x4 rk_j = *reinterpret_cast<const f32x4*>(&rk[t * 16 + g * 4]);
+    f32x4 pull;
+    float m[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = wave * 16 + (lane >> 4) * 4 + r;
-      const float e = __builtin_amdgcn_exp2f((float)(sum[i] - gj)) * rkj;
-      if (BETA) tri[i * kRow + j] = j < i ? kk[r] * e * rk[i] * betas[i] : 0.0f;
-      uint32_t p[2];
-      split2<2>(j <= i ? qk[r] * e * rq[i] : 0.0f, 0.0f, p);
-      m16[0][i * kRow16 + j] = (uint16_t)p[0], m16[1][i * kRow16 + j] = (uint16_t)p[1];
+      const int j = t * 16 + g * 4 + r;
+      const float e = __builtin_amdgcn_exp2f((float)(sum_i - sum[j])) * rk_j[r];
+      const float x = kk[r] * e * rk_i * beta_i, y = qk[r] * e * rq_i;
+      pull[r] = j < i ? x : 0.0f, m[r] = j <= i ? y : 0.0f;
     }
+    if constexpr (BETA) *reinterpret_cast<f32x4*>(&tri[i * kRow + t * 16 + g * 4]) = pull;
+    uint32_t p[2][2];
+    split2<2>(m[0], m[1], p[0]), split2<2>(m[2], m[3], p[1]);
+    mp[t][0] = uint2{p[0][0], p[1][0]}, mp[t][1] = uint2{p[0][1], p[1][1]};
   }
-  uint8_t* out = head_data(a, place, head);
-  if (wave == 3) {
-    const double g = sum[lane], all = sum[kChunk - 1];
-    const float from = __builtin_amdgcn_exp2f((float)g);
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    if (s > wave >> 1) continue;
+    uint4* m = reinterpret_cast<uint4*>(out + kBytesT) + fragment_of(wave, s) * 2 * 64 + lane;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) m[p * 64] = uint4{mp[2 * s][p].x, mp[2 * s][p].y, mp[2 * s + 1][p].x, mp[2 * s + 1][p].y};
+  }
+  if (wave == 0) {
+    const double d = sum[lane], all = sum[kChunk - 1];
+    const float from = __builtin_amdgcn_exp2f((float)d);
     float* f = reinterpret_cast<float*>(out + kBytesT + kBytesM);
-    f[kFromK * kChunk + lane] = from * rk[lane], f[kFromQ * kChunk + lane] = from * rq[lane];
+    f[kFromK * kChunk + lane] = betas[lane] * from * rk[lane], f[kFromQ * kChunk + lane] = from * rq[lane];
     f[kBeta * kChunk + lane] = betas[lane];
-    f[kToEnd * kChunk + lane] = __builtin_amdgcn_exp2f((float)(all - g)) * rk[lane];
+    f[kToEnd * kChunk + lane] = __builtin_amdgcn_exp2f((float)(all - d)) * rk[lane];
     f[kEnd * kChunk + lane] = __builtin_amdgcn_exp2f((float)all);
-  }
-  __syncthreads();
-
-  if constexpr (BETA) {
-    if (wave == 0) {
-      // column `lane` of T by forward substitution
-      float x[kChunk];
-#pragma unroll
-      for (int i = 0; i < kChunk; ++i) {
-        float s[4] = {lane == i ? 1.0f : 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < i; j += 4) {
-          const float4 r = *reinterpret_cast<const float4*>(&tri[i * kRow + j]);
-          s[0] = __builtin_fmaf(-r.x, x[j], s[0]);
-          if (j + 1 < i) s[1] = __builtin_fmaf(-r.y, x[j + 1], s[1]);
-          if (j + 2 < i) s[2] = __builtin_fmaf(-r.z, x[j + 2], s[2]);
-          if (j + 3 < i) s[3] = __builtin_fmaf(-r.w, x[j + 3], s[3]);
-        }
-        x[i] = i < lane ? 0.0f : (s[0] + s[1]) + (s[2] + s[3]);
-      }
-#pragma unroll
-      for (int i = 0; i < kChunk; ++i) tri[i * kRow + lane] = x[i];
-    }
-    __syncthreads();
-  }
-  for (int s = 0; s <= wave >> 1; ++s) {
-    const int at = (wave * 16 + r16), col = s * 32 + k8;
-    i32x4* m = reinterpret_cast<i32x4*>(out + kBytesT) + (wave * 2 + s) * 2 * 64 + lane;
-#pragma unroll
-    for (int p = 0; p < 2; ++p) m[p * 64] = *reinterpret_cast<const i32x4*>(&m16[p][at * kRow16 + col]);
-    if constexpr (BETA) {
-      const float4 x = *reinterpret_cast<const float4*>(&tri[at * kRow + col]), y = *reinterpret_cast<const float4*>(&tri[at * kRow + col + 4]);
-      uint32_t p[4][3];
-      split2<3>(x.x, x.y, p[0]), split2<3>(x.z, x.w, p[1]), split2<3>(y.x, y.y, p[2]), split2<3>(y.z, y.w, p[3]);
-      i32x4* t = reinterpret_cast<i32x4*>(out) + (wave * 2 + s) * 3 * 64 + lane;
-#pragma unroll
-      for (int i = 0; i < 3; ++i) t[i * 64] = i32x4{(int)p[0][i], (int)p[1][i], (int)p[2][i], (int)p[3][i]};
-    }
   }
   if (head % a.group == 0) {
     i32x4* dst = reinterpret_cast<i32x4*>(key_data(a, place, kh, DK)) + lane;
-    for (int f = wave; f < DK / 16 * 2; f += 4)
-      dst[f * 64] = *reinterpret_cast<const i32x4*>(&kt[((f >> 1) * 16 + r16) * kRow16 + (f & 1) * 32 + k8]);
+    for (int f = wave; f < DK / 16 * 2; f += 4) {
+      const int row = state_row(f >> 1, r16 >> 2) + (r16 & 3);
+      i32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint16_t* p = &krows[((f & 1) * 32 + (e >> 1) * 16 + g * 4 + (e & 1) * 2) * kRowK + row];
+        v[e] = (int)(p[0] | (uint32_t)p[kRowK] << 16);
+      }
+      dst[f * 64] = v;
+    }
+  }
+
+  if constexpr (BETA) {
+    lds_barrier();
+    // T by blocks of 16 rows. Wave w inverts the diagonal block w by forward
+    // substitution, a column a lane (every 16 lanes the same), then works out
+    // T's block column w: T_iw = -T_ii sum_(w <= k < i) A_ik T_kw in fp32 MFMAs
+    // (16x16x4: a lane's A is row lane % 16, its B column lane % 16, k = lane /
+    // 16). Their k go by 4 g + s for the s-th of four, which is where a result's
+    // s-th register has its rows, so that a result is the next product's B as
+    // it is, and as its A the transpose: T_iw^T = -(..)^T T_ii^T has the four
+    // columns of a row in a lane.
+    f32x4 tb[4], tt[4];
+    {
+      const float* d = &tri[(wave * 16) * kRow + wave * 16];
+      float x[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        float s[2] = {r16 == c ? 1.0f : 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < c; j += 4) {
+          const float4 r = *reinterpret_cast<const float4*>(d + c * kRow + j);
+          s[0] = __builtin_fmaf(-r.x, x[j], s[0]);
+          if (j + 1 < c) s[1] = __builtin_fmaf(-r.y, x[j + 1], s[1]);
+          if (j + 2 < c) s[0] = __builtin_fmaf(-r.z, x[j + 2], s[0]);
+          if (j + 3 < c) s[1] = __builtin_fmaf(-r.w, x[j + 3], s[1]);
+        }
+        x[c] = c < r16 ? 0.0f : s[0] + s[1];
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        tb[0][r] = g == 0 ? x[r] : g == 1 ? x[4 + r] : g == 2 ? x[8 + r] : x[12 + r];
+        diagonal[wave][(g * 4 + r) * kRowD + r16] = tb[0][r];
+      }
+    }
+    lds_barrier();
+    tt[0] = *reinterpret_cast<const f32x4*>(&diagonal[wave][r16 * kRowD + g * 4]);
+#pragma unroll
+    for (int c = 1; c < 4; ++c) {
+      if (wave + c > 3) break;
+      f32x4 sums = {0.0f, 0.0f, 0.0f, 0.0f}, next = sums, turned = sums;
+#pragma unroll
+      for (int k = 0; k < c; ++k) {
+        const f32x4 l = *reinterpret_cast<const f32x4*>(&tri[((wave + c) * 16 + r16) * kRow + (wave + k) * 16 + g * 4]);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) sums = __builtin_amdgcn_mfma_f32_16x16x4f32(l[s], tb[k][s], sums, 0, 0, 0);
+      }
+      // rows behind a column's first one that is not finite must not reach those before it
+      int bad = 16;
+#pragma unroll
+      for (int r = 3; r >= 0; --r)
+        if (!(__builtin_fabsf(sums[r]) < __builtin_inff())) bad = g * 4 + r;
+      const bool spoilt = __ballot(bad < 16) != 0;
+      if (spoilt) {
+        bad = min(bad, __shfl_xor(bad, 16));
+        bad = min(bad, __shfl_xor(bad, 32));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (g * 4 + r >= bad) sums[r] = 0.0f;
+      }
+      const f32x4 l = *reinterpret_cast<const f32x4*>(&diagonal[wave + c][r16 * kRowD + g * 4]);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        next = __builtin_amdgcn_mfma_f32_16x16x4f32(l[s], sums[s], next, 0, 0, 0);
+        turned = __builtin_amdgcn_mfma_f32_16x16x4f32(sums[s], l[s], turned, 0, 0, 0);
+      }
+      tb[c] = -next, tt[c] = -turned;
+      if (spoilt) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (g * 4 + r >= bad) tb[c][r] = __builtin_nanf("");
+          if (r16 >= __shfl(bad, g * 4 + r)) tt[c][r] = __builtin_nanf("");
+        }
+      }
+    }
+    // half of each fragment: the wave's 16 columns
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int tile = wave + c;
+      if (tile > 3) break;
+      uint32_t p[2][3];
+      split2<3>(tt[c][0], tt[c][1], p[0]), split2<3>(tt[c][2], tt[c][3], p[1]);
+#pragma unroll
+      for (int x = 0; x < 3; ++x)
+        *reinterpret_cast<uint2*>(out + (fragment_of(tile, wave >> 1) * 3 + x) * kFragment + lane * 16 + (wave & 1) * 8) = uint2{p[0][x], p[1][x]};
+    }
+    if (wave & 1) {
+#pragma unroll
+      for (int x = 0; x < 3; ++x)
+        *reinterpret_cast<uint2*>(out + (fragment_of(wave - 1, wave >> 1) * 3 + x) * kFragment + lane * 16 + 8) = uint2{0u, 0u};
+    }
   }
 }
 
 __device__ __forceinline__ f32x4 mfma_bf16(i32x4 a, i32x4 b, f32x4 c) { return Bf16::mfma16(a, b, c); }
 
+// Waits out 16x16 MFMAs' results, which other instructions may not read for up
+// to 11 issue slots: ahead of a wave-uniform branch the compiler has left the
+// wait out (the listing's test follows every path).
+template <int N>
+__device__ __forceinline__ void settle(f32x4 (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(r[i]));
+  asm volatile("s_nop 7\n\ts_nop 2" : "+v"(r[N - 1]));
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(r[i]));
+}
+
 // A sequence's chunks one after the other, kCols columns of a head's state a
-// workgroup, wave w with the state's rows from w DK / 4 on and a chunk's rows
-// from 16 w on. Three exchanges through LDS a chunk: the state (as the right
-// operand of K S and Q S), the differences D = beta (V - e^G K S), and U.
-template <class H, int DK, bool BETA>
-__global__ __launch_bounds__(256) void scan_kernel(LinearArgs a, int v_dim, uint32_t col_blocks) {
+// workgroup, 16 a wave: a wave's columns of S, D and U are no other wave's, so
+// that what a product leaves in registers is the next one's right operand as
+// it lies there (the left operands have their k in that order), in two or three
+// bf16 parts. The left operands K, Q, T, M and K^T are the same for all waves:
+// they go through LDS, K and Q of the next chunk once this one's are read, the
+// others at its end. A wave has loaded its share of them into registers a
+// chunk's time before (copies straight into LDS are not used: the compiler
+// waits for all of those in flight at any read of LDS).
+//
+// What bounds it: the 182 MFMAs of a wave's chunk (DK 128), 2900 cycles, beside
+// 450 VALU instructions.
+//
+// A chunk whose U is not finite is gone through again: what lies behind a
+// column's first row that is not finite is left out, where it would reach the
+// rows before it as 0 times infinity, and comes out as NaN.
+template <class H, int DK, int NW, bool BETA>
+__global__ __launch_bounds__(64 * NW, NW / 4) void scan_kernel(LinearArgs a, int v_dim, uint32_t col_blocks) {
+  constexpr int kCols = 16 * NW, kRowO = kCols + 8;
+  constexpr int KS = DK / 32, MT = DK / 16, NP = Parts<H>::n;
+  // fragments of 1 KB: what the first half of a chunk reads, and the second
+  constexpr int kK = 0, kQ = BETA ? 4 * KS : 0, kKt = kQ + 4 * KS, kM = kKt + 2 * MT, kT = kM + 12, kF = kT + (BETA ? 18 : 0), kV = kF + 2;
+  constexpr int kVs = 2 * NW;  // V's fragments
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[(kV + kVs) * kFragment];
+  __shared__ __attribute__((aligned(16))) uint16_t ob[kChunk * kRowO];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // The hardware hands consecutive workgroups to the 8 XCDs in turn: those of
+  // one sequence and key head, which read the same operands, come to one.
+  const Batch& b = a.b;
+  const uint32_t unit_size = (uint32_t)a.group * col_blocks, round = blockIdx.x / (8 * unit_size), within = blockIdx.x % (8 * unit_size);
+  const uint32_t units = min((uint32_t)(b.batch * a.k_heads) - round * 8, 8u);
+  const uint32_t unit = round * 8 + within % units, inner = within / units, cb = inner % col_blocks;
+  const int kh = (int)(unit % (uint32_t)a.k_heads), seq = (int)(unit / (uint32_t)a.k_heads), head = kh * a.group + (int)(inner / col_blocks);
+  const int start = clamp_to(uniform_at(b.starts, seq), b.tokens), n = clamp_to(uniform_at(b.starts, seq + 1), b.tokens) - start;
+  if (n <= 0) return;
+  const int from = uniform_at(b.from, seq), to = uniform_at(b.slots, seq);
+  const int r16 = lane & 15, g = lane >> 4, r4 = g * 4, k8 = g * 8;
+  const int last = (n - 1) / kChunk, chunk0 = start / kChunk + seq;
+  const int64_t slot_size = (int64_t)DK * v_dim;
+  const int col = (int)cb * kCols + wave * 16 + r16;
+
+  // Chunk c's rows of K and Q as fragments [row tile][32 columns]; rows behind the end: the last one's. The wave's share is
+  // every (NW / 4)-th of a row tile's.
+  constexpr int kShare = 4 * KS / NW;
+  const int tile = wave & 3, x0 = wave >> 2;
+  i32x4 kq[2][kShare];
+  const auto load_kq = [&](int c) {
+    const int64_t t = start + c * kChunk + min(tile * 16 + r16, n - c * kChunk - 1);
+    const uint16_t *k = a.k + t * a.k_ts + kh * a.k_hs + x0 * 32 + k8, *q = a.q + t * a.q_ts + kh * a.q_hs + x0 * 32 + k8;
+#pragma unroll
+    for (int x = 0; x < kShare; ++x) {
+      if (BETA) kq[0][x] = *reinterpret_cast<const i32x4*>(k + x * (NW / 4) * 32);
+      kq[1][x] = *reinterpret_cast<const i32x4*>(q + x * (NW / 4) * 32);
+    }
+  };
+  const auto put = [&](int i, i32x4 v) { *reinterpret_cast<i32x4*>(lds + i * kFragment + lane * 16) = v; };
+  const auto put_kq = [&]() {
+#pragma unroll
+    for (int x = 0; x < kShare; ++x) {
+      if (BETA) put(kK + tile * KS + x * (NW / 4) + x0, kq[0][x]);
+      put(kQ + tile * KS + x * (NW / 4) + x0, kq[1][x]);
+    }
+  };
+  // Its other operands, every NW-th fragment of each kind a wave's (a kind's
+  // last one again where it has none), and V's rows [64][kCols].
+  constexpr int kKts = 2 * MT, kMs = 12, kTs = BETA ? 20 : 2;  // T's 18 and the factors' 2, in the order of LDS
+  constexpr int kNKt = (kKts + NW - 1) / NW, kNM = (kMs + NW - 1) / NW, kNT = (kTs + NW - 1) / NW;
+  i32x4 kt[kNKt], mt[kNM], tail[kNT], v8[2];
+  const auto load_rest = [&](int c) {
+    const i32x4* d = reinterpret_cast<const i32x4*>(head_data(a, chunk0 + c, head)) + lane;
+    const i32x4* k = reinterpret_cast<const i32x4*>(key_data(a, chunk0 + c, kh, DK)) + lane;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = ((i * NW + wave) * 64 + lane) * 8, row = at / kCols;
+      const int64_t t = start + c * kChunk + min(row, n - c * kChunk - 1);
+      v8[i] = *reinterpret_cast<const i32x4*>(a.v + t * a.v_ts + head * a.v_hs + cb * kCols + at % kCols);
+    }
+#pragma unroll
+    for (int i = 0; i < kNT; ++i) {
+      const int f = min(i * NW + wave, kTs - 1);
+      tail[i] = d[(f < kTs - 2 ? f : f - (kTs - 2) + (kBytesT + kBytesM) / kFragment) * 64];
+    }
+#pragma unroll
+    for (int i = 0; i < kNM; ++i) mt[i] = d[(kBytesT / kFragment + min(i * NW + wave, kMs - 1)) * 64];
+#pragma unroll
+    for (int i = 0; i < kNKt; ++i) kt[i] = k[min(i * NW + wave, kKts - 1) * 64];
+  };
+  const auto put_rest = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) put(kV + i * NW + wave, v8[i]);
+#pragma unroll
+    for (int i = 0; i < kNT; ++i) put(kT + min(i * NW + wave, kTs - 1), tail[i]);
+#pragma unroll
+    for (int i = 0; i < kNM; ++i) put(kM + min(i * NW + wave, kMs - 1), mt[i]);
+#pragma unroll
+    for (int i = 0; i < kNKt; ++i) put(kKt + min(i * NW + wave, kKts - 1), kt[i]);
+  };
+  const auto fragment = [&](int i) { return *reinterpret_cast<const i32x4*>(lds + i * kFragment + lane * 16); };
+  const auto factor = [&](int which, int t) {
+    return *reinterpret_cast<const f32x4*>(lds + kF * kFragment + (which * kChunk + t * 16 + r4) * 4);
+  };
+
+  load_kq(0);
+  __builtin_amdgcn_sched_barrier(0);
+  load_rest(0);
+  __builtin_amdgcn_sched_barrier(0);
+  // S's row state_row(m, g) + r is tile m's row 4 g + r.
+  f32x4 s[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) s[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (from >= 0 && from < b.n_slots) {
+    const float* p = a.states + ((int64_t)from * a.v_heads + head) * slot_size + col;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[m][r] = p[(state_row(m, g) + r) * v_dim];
+  }
+
+  put_kq();
+  for (int chunk = 0; chunk <= last; ++chunk) {
+    const int rows = min(n - chunk * kChunk, kChunk);
+    lds_barrier();
+    put_rest();
+    load_kq(min(chunk + 1, last));
+    if (chunk) {
+      // the outputs of the chunk before, which is a whole one
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = ((i * NW + wave) * 64 + lane) * 8, row = at / kCols;
+        const int64_t t = start + (chunk - 1) * kChunk + row;
+        *reinterpret_cast<uint4*>(a.out + (t * a.v_heads + head) * v_dim + cb * kCols + at % kCols) =
+            *reinterpret_cast<const uint4*>(&ob[row * kRowO + at % kCols]);
+      }
+    }
+    // K S and Q S, 16 rows a tile; towards the outputs two parts of S do
+    f32x4 pk[4], pq[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) pk[t] = pq[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int x = 0; x < KS; ++x) {
+      i32x4 sp[3];
+      split8(s[2 * x], s[2 * x + 1], sp);
+#pragma unroll
+      for (int i = BETA ? 0 : 1; i < 2; ++i) {
+        i32x4 rp[4][NP];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          i32x4 f = fragment((i ? kQ : kK) + t * KS + x);
+          if (rows < kChunk) f &= (t * 16 + r16 - rows) >> 31;  // rows behind the sequence's end are 0
+          Parts<H>::of(f, rp[t]);
+        }
+#pragma unroll
+        for (int j = i ? 1 : 2; j >= 0; --j)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            f32x4& p = i ? pq[t] : pk[t];
+            if (NP > 1 && j < (i ? 1 : 2)) p = mfma_bf16(rp[t][NP - 1], sp[j], p);
+            p = mfma_bf16(rp[t][0], sp[j], p);
+          }
+      }
+    }
+    settle(pq);
+    lds_barrier();
+    put_kq();
+
+    f32x4 d[4], u[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t v = *reinterpret_cast<const uint16_t*>(lds + kV * kFragment + ((t * 16 + r4 + r) * kCols + wave * 16 + r16) * 2);
+        d[t][r] = H::lo(v);
+      }
+      if (rows < kChunk)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) d[t][r] = t * 16 + r4 + r < rows ? d[t][r] : 0.0f;
+      if constexpr (BETA) {
+        const f32x4 from_k = factor(kFromK, t), beta = factor(kBeta, t);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) d[t][r] = __builtin_fmaf(-from_k[r], pk[t][r], beta[r] * d[t][r]);
+      }
+    }
+    const auto solve = [&]() {
+      if constexpr (BETA) {
+        i32x4 dp[2][3];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) split8(d[2 * x], d[2 * x + 1], dp[x]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) u[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+          for (int i = 2; i >= 0; --i) {
+            i32x4 tf[4];
+#pragma unroll
+            for (int t = 2 * x; t < 4; ++t) tf[t] = fragment(kT + fragment_of(t, x) * 3 + i);
+#pragma unroll
+            for (int j = 2 - i; j >= 0; --j)
+#pragma unroll
+              for (int t = 2 * x; t < 4; ++t) u[t] = mfma_bf16(tf[t], dp[x][j], u[t]);
+          }
+        }
+        settle(u);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) u[t] = d[t];
+      }
+    };
+    // a column's first row of x that is not finite
+    const auto first_bad = [&](const f32x4(&x)[4]) {
+      int first = kChunk;
+#pragma unroll
+      for (int t = 3; t >= 0; --t)
+#pragma unroll
+        for (int r = 3; r >= 0; --r)
+          if (!(__builtin_fabsf(x[t][r]) < __builtin_inff())) first = t * 16 + r4 + r;
+      first = min(first, __shfl_xor(first, 16));
+      return min(first, __shfl_xor(first, 32));
+    };
+    solve();
+    int bad = kChunk;
+    {
+      float z = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z = __builtin_fmaf(u[t][r], 0.0f, z);
+      if (__ballot(z != z)) {
+        bad = first_bad(d);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (t * 16 + r4 + r >= bad) d[t][r] = 0.0f;
+        solve();
+        bad = min(bad, first_bad(u));
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (t * 16 + r4 + r >= bad) u[t][r] = 0.0f;
+      }
+    }
+
+    load_rest(min(chunk + 1, last));
+
+    // the chunk's outputs
+    f32x4 o[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) o[t] = factor(kFromQ, t) * pq[t];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      i32x4 up[2];
+      split8(u[2 * x], u[2 * x + 1], up);
+#pragma unroll
+      for (int i = 1; i >= 0; --i) {
+        i32x4 mf[4];
+#pragma unroll
+        for (int t = 2 * x; t < 4; ++t) mf[t] = fragment(kM + fragment_of(t, x) * 2 + i);
+#pragma unroll
+        for (int j = 1 - i; j >= 0; --j)
+#pragma unroll
+          for (int t = 2 * x; t < 4; ++t) o[t] = mfma_bf16(mf[t], up[j], o[t]);
+      }
+    }
+    // the state behind the chunk
+    const float end = *reinterpret_cast<const float*>(lds + kF * kFragment + kEnd * kChunk * 4);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) u[t] *= factor(kToEnd, t);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) s[m] *= end;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      i32x4 up[3];
+      split8(u[2 * x], u[2 * x + 1], up);
+#pragma unroll
+      for (int m0 = 0; m0 < MT; m0 += 4) {
+        i32x4 kp[4][NP];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) Parts<H>::of(fragment(kKt + (m0 + m) * 2 + x), kp[m]);
+#pragma unroll
+        for (int i = 2; i >= 0; --i)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            if (NP > 1 && i < 2) s[m0 + m] = mfma_bf16(kp[m][NP - 1], up[i], s[m0 + m]);
+            s[m0 + m] = mfma_bf16(kp[m][0], up[i], s[m0 + m]);
+          }
+      }
+    }
+    settle(o);
+    settle(s);
+    if (__ballot(bad < kChunk)) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (t * 16 + r4 + r >= bad) o[t][r] = __builtin_nanf("");
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        if (bad < kChunk) s[m] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        const uint32_t p = H::pack(o[t][r], o[t][r + 1]);
+        ob[(t * 16 + r4 + r) * kRowO + wave * 16 + r16] = (uint16_t)p;
+        ob[(t * 16 + r4 + r + 1) * kRowO + wave * 16 + r16] = (uint16_t)(p >> 16);
+      }
+  }
+  lds_barrier();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int at = ((i * NW + wave) * 64 + lane) * 8, row = at / kCols;
+    const int64_t t = start + last * kChunk + row;
+    if (t < start + n)
+      *reinterpret_cast<uint4*>(a.out + (t * a.v_heads + head) * v_dim + cb * kCols + at % kCols) =
+          *reinterpret_cast<const uint4*>(&ob[row * kRowO + at % kCols]);
+  }
+  if (to >= 0 && to < b.n_slots) {
+    float* p = a.states + ((int64_t)to * a.v_heads + head) * slot_size + col;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[(state_row(m, g) + r) * v_dim] = s[m][r];
+  }
+}
+
+// The same with 16 or 32 columns a workgroup, for calls of few heads and
+// sequences, where scan_kernel would leave compute units without one: a chunk's
+// work is spread over eight waves, in three steps with an exchange through LDS behind each:
+//   the state in three parts                               -> sb, as the right operand of K S and Q S
+//   D = beta (V - e^G K S) in three parts                  -> db, as that of T D
+//   U = T D in two parts, e^(G_C - G) U in three           -> ub, as that of M U and of K^T U, which gives the state
+// Waves 0 to 3 go through them, wave w with a chunk's rows from 16 w on and the
+// state's from w DK / 4 on. Waves 4 to 7 have the rows' outputs e^G Q S + M U,
+// which no later chunk waits for. An operand is loaded for the next chunk once
+// this one has used it, so that a load has most of a chunk's time and no
+// register of its own.
+template <class H, int DK, int kCols, bool BETA>
+__global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_dim, uint32_t col_blocks) {
   constexpr int KS = DK / 32, MT = DK / 64, NT = kCols / 16, NP = Parts<H>::n;
   constexpr int kRowS = DK + 8, kRowU = kChunk + 8;
   __shared__ __attribute__((aligned(16))) uint16_t sb[3][kCols * kRowS];
   __shared__ __attribute__((aligned(16))) uint16_t db[BETA ? 3 : 1][kCols * kRowU];
-  __shared__ __attribute__((aligned(16))) uint16_t ub[5][kCols * kRowU];  // U in 2 parts, e^(G_C - G) U in 3
+  __shared__ __attribute__((aligned(16))) uint16_t ub[5][kCols * kRowU];
   __shared__ int first_d[kCols], first_us[2][kCols];  // a column's first row that is not finite; U's by turns
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t cb = blockIdx.x % col_blocks, rest = blockIdx.x / col_blocks;
-  const int head = (int)(rest % (uint32_t)a.v_heads), seq = (int)(rest / (uint32_t)a.v_heads), kh = head / a.group;
+  const int tid = threadIdx.x, lane = tid & 63, all_wave = __builtin_amdgcn_readfirstlane(tid >> 6), wave = all_wave & 3;
+  // The hardware hands consecutive workgroups to the 8 XCDs in turn: those of
+  // one sequence and key head, which read the same operands, come to one.
   const Batch& b = a.b;
+  const uint32_t unit_size = (uint32_t)a.group * col_blocks, round = blockIdx.x / (8 * unit_size), within = blockIdx.x % (8 * unit_size);
+  const uint32_t units = min((uint32_t)(b.batch * a.k_heads) - round * 8, 8u);
+  const uint32_t unit = round * 8 + within % units, inner = within / units, cb = inner % col_blocks;
+  const int kh = (int)(unit % (uint32_t)a.k_heads), seq = (int)(unit / (uint32_t)a.k_heads), head = kh * a.group + (int)(inner / col_blocks);
   const int start = clamp_to(uniform_at(b.starts, seq), b.tokens), n = clamp_to(uniform_at(b.starts, seq + 1), b.tokens) - start;
   if (n <= 0) return;
-  const int from = uniform_at(b.from, seq), to = uniform_at(b.slots, seq);
-  const int r16 = lane & 15, r4 = (lane >> 4) * 4, k8 = (lane >> 4) * 8, col0 = (int)cb * kCols + r16;
-  const int64_t slot_size = (int64_t)DK * v_dim;
-  const int chunk0 = start / kChunk + seq;
+  const int r16 = lane & 15, r4 = (lane >> 4) * 4, k8 = (lane >> 4) * 8, col0 = (int)cb * kCols + r16, row16 = wave * 16 + r16;
+  const int last = (n - 1) / kChunk, chunk0 = start / kChunk + seq;
+  const uint8_t* data = head_data(a, chunk0, head);
+  const int64_t data_step = (int64_t)a.v_heads * kBytesHead;
+  if (tid < kCols) first_d[tid] = first_us[chunk0 & 1][tid] = kChunk;
 
+  if (all_wave >= 4) {
+    i32x4 qf[KS], mf[2][2];
+    f32x4 from_q;
+    const uint16_t* q_next = a.q + (int64_t)(start + row16) * a.q_ts + kh * a.q_hs + k8;
+    const auto load_q = [&](int c) {
+      const int rows = n - c * kChunk;
+      const uint16_t* p = rows >= kChunk ? q_next : a.q + (int64_t)(start + c * kChunk + min(row16, rows - 1)) * a.q_ts + kh * a.q_hs + k8;
+#pragma unroll
+      for (int x = 0; x < KS; ++x) qf[x] = *reinterpret_cast<const i32x4*>(p + x * 32);
+      q_next += c < last ? kChunk * a.q_ts : 0;  // never past the last chunk, which is loaded again
+    };
+    const auto load_m = [&](const uint8_t* d) {
+      const i32x4* p = reinterpret_cast<const i32x4*>(d + kBytesT) + lane;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (x > (wave >> 1)) break;
+        mf[x][0] = p[fragment_of(wave, x) * 128], mf[x][1] = p[fragment_of(wave, x) * 128 + 64];
+      }
+      from_q = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(d + kBytesT + kBytesM) + kFromQ * kChunk + wave * 16 + r4);
+    };
+    load_q(0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_m(data);
+    __builtin_amdgcn_sched_barrier(0);
+    uint16_t* out = a.out + ((int64_t)(start + wave * 16 + r4) * a.v_heads + head) * v_dim + col0;
+    const int64_t out_ts = (int64_t)a.v_heads * v_dim;
+    for (int chunk = 0; chunk <= last; ++chunk) {
+      const int rows = n - chunk * kChunk;
+      lds_barrier();
+      f32x4 pq[NT][2];
+#pragma unroll
+      for (int c = 0; c < NT; ++c) pq[c][0] = pq[c][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int x = 0; x < KS; ++x) {
+        i32x4 qp[NP];
+        Parts<H>::of(qf[x], qp);
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+          i32x4 sp[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) sp[i] = *reinterpret_cast<const i32x4*>(&sb[i][(c * 16 + r16) * kRowS + x * 32 + k8]);
+          pq[c][0] = mfma_bf16(qp[0], sp[0], pq[c][0]), pq[c][1] = mfma_bf16(qp[0], sp[1], pq[c][1]);
+          if (NP > 1) pq[c][1] = mfma_bf16(qp[NP - 1], sp[0], pq[c][1]);
+        }
+      }
+      load_q(min(chunk + 1, last));
+      if constexpr (BETA) {
+        lds_barrier();
+        if (__ballot(first_d[lane & (kCols - 1)] < kChunk)) lds_barrier();
+      }
+      lds_barrier();
+      const int* first_u = first_us[(chunk0 + chunk) & 1];
+      const bool spoilt = __ballot(first_u[lane & (kCols - 1)] < kChunk) != 0;
+      if (spoilt) lds_barrier();
+      f32x4 o[NT][2];
+#pragma unroll
+      for (int c = 0; c < NT; ++c) o[c][0] = o[c][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (x > (wave >> 1)) break;
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+          const i32x4 u0 = *reinterpret_cast<const i32x4*>(&ub[0][(c * 16 + r16) * kRowU + x * 32 + k8]);
+          const i32x4 u1 = *reinterpret_cast<const i32x4*>(&ub[1][(c * 16 + r16) * kRowU + x * 32 + k8]);
+          o[c][1] = mfma_bf16(mf[x][1], u0, o[c][1]), o[c][0] = mfma_bf16(mf[x][0], u0, o[c][0]);
+          o[c][1] = mfma_bf16(mf[x][0], u1, o[c][1]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[c][0][r] = __builtin_fmaf(from_q[r], pq[c][0][r] + pq[c][1][r], o[c][0][r] + o[c][1][r]);
+        if (spoilt) {
+          const int bad = first_u[c * 16 + r16];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (wave * 16 + r4 + r >= bad) o[c][0][r] = __builtin_nanf("");
+        }
+      }
+      data += chunk < last ? data_step : 0;
+      load_m(data);
+      const int mine = rows - wave * 16 - r4;  // this lane's rows that are the sequence's
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        const uint32_t p[2] = {H::pack(o[c][0][0], o[c][0][1]), H::pack(o[c][0][2], o[c][0][3])};
+        const uint16_t p16[4] = {(uint16_t)p[0], (uint16_t)(p[0] >> 16), (uint16_t)p[1], (uint16_t)(p[1] >> 16)};
+        if (rows >= kChunk) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) out[r * out_ts + c * 16] = p16[r];
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (r < mine) out[r * out_ts + c * 16] = p16[r];
+        }
+      }
+      out += kChunk * out_ts;
+    }
+    return;
+  }
+
+  const int from = uniform_at(b.from, seq), to = uniform_at(b.slots, seq);
+  const int place4 = place_of(wave * 16 + r4);
+  const int64_t slot_size = (int64_t)DK * v_dim;
   f32x4 s[MT][NT];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int c = 0; c < NT; ++c) s[m][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   if (from >= 0 && from < b.n_slots) {
-    const float* p = a.states + ((int64_t)from * a.v_heads + head) * slot_size + (wave * (DK / 4) + r4) * v_dim + col0;
+    const float* p = a.states + ((int64_t)from * a.v_heads + head) * slot_size + col0;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int c = 0; c < NT; ++c)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[m][c][r] = p[(m * 16 + r) * v_dim + c * 16];
+        for (int r = 0; r < 4; ++r) s[m][c][r] = p[(state_row(wave * MT + m, lane >> 4) + r) * v_dim + c * 16];
   }
-  if (tid < kCols) first_d[tid] = first_us[chunk0 & 1][tid] = kChunk;
-
-  for (int t0 = 0; t0 < n; t0 += kChunk) {
-    const int rows = min(n - t0, kChunk), first = start + t0, place = chunk0 + t0 / kChunk;
-    const uint8_t* data = head_data(a, place, head);
-    // this chunk's operands
-    i32x4 kf[KS], qf[KS];
-    {
-      const int i = wave * 16 + r16;
-      const int64_t t = first + min(i, rows - 1);
+  i32x4 kf[KS], tf[BETA ? 2 : 1][3], kt[2][MT];
+  uint32_t v16[NT][4];
+  f32x4 from_k, beta, to_end;
+  float end;
+  const uint16_t* k_next = a.k + (int64_t)(start + row16) * a.k_ts + kh * a.k_hs + k8;
+  const uint16_t* v_next = a.v + (int64_t)(start + wave * 16 + r4) * a.v_ts + head * a.v_hs + col0;
+  const auto load_k = [&](int c) {
+    if constexpr (BETA) {
+      const int rows = n - c * kChunk;
+      const uint16_t* p = rows >= kChunk ? k_next : a.k + (int64_t)(start + c * kChunk + min(row16, rows - 1)) * a.k_ts + kh * a.k_hs + k8;
 #pragma unroll
-      for (int x = 0; x < KS; ++x) {
-        kf[x] = *reinterpret_cast<const i32x4*>(a.k + t * a.k_ts + kh * a.k_hs + x * 32 + k8);
-        qf[x] = *reinterpret_cast<const i32x4*>(a.q + t * a.q_ts + kh * a.q_hs + x * 32 + k8);
-      }
-#pragma unroll
-      for (int x = 0; x < KS; ++x) kf[x] &= (i - rows) >> 31, qf[x] &= (i - rows) >> 31;
+      for (int x = 0; x < KS; ++x) kf[x] = *reinterpret_cast<const i32x4*>(p + x * 32);
+      k_next += c < last ? kChunk * a.k_ts : 0;  // never past the last chunk, which is loaded again
     }
-    i32x4 tf[BETA ? 2 : 1][3], mf[2][2], kt[2][MT];
+  };
+  const auto load_v = [&](int c) {
+    const int rows = n - c * kChunk;
+    if (rows >= kChunk) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if constexpr (BETA) {
+      for (int x = 0; x < NT; ++x)
 #pragma unroll
-        for (int i = 0; i < 3; ++i) tf[x][i] = reinterpret_cast<const i32x4*>(data)[((wave * 2 + (x & (wave >> 1))) * 3 + i) * 64 + lane];
-      }
+        for (int r = 0; r < 4; ++r) v16[x][r] = v_next[r * a.v_ts + x * 16];
+    } else {
+      const uint16_t* p = a.v + (int64_t)(start + c * kChunk) * a.v_ts + head * a.v_hs + col0;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        mf[x][i] = reinterpret_cast<const i32x4*>(data + kBytesT)[((wave * 2 + (x & (wave >> 1))) * 2 + i) * 64 + lane];
+      for (int x = 0; x < NT; ++x)
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-        kt[x][m] = reinterpret_cast<const i32x4*>(key_data(a, place, kh, DK))[((wave * MT + m) * 2 + x) * 64 + lane];
+        for (int r = 0; r < 4; ++r) v16[x][r] = p[min(wave * 16 + r4 + r, rows - 1) * a.v_ts + x * 16];
     }
-    float v[NT][4];
+    v_next += c < last ? kChunk * a.v_ts : 0;  // never past the last chunk, which is loaded again
+  };
+  const auto load_t = [&](const uint8_t* d) {
+    if constexpr (BETA) {
+      const i32x4* p = reinterpret_cast<const i32x4*>(d) + lane;
 #pragma unroll
-    for (int c = 0; c < NT; ++c)
+      for (int x = 0; x < 2; ++x) {
+        if (x > (wave >> 1)) break;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = wave * 16 + r4 + r;
-        const uint16_t x = a.v[(int64_t)(first + min(i, rows - 1)) * a.v_ts + head * a.v_hs + col0 + c * 16];
-        v[c][r] = H::lo((uint32_t)x & (uint32_t)((i - rows) >> 31));  // 0 behind the sequence's end
+        for (int i = 0; i < 3; ++i) tf[x][i] = p[(fragment_of(wave, x) * 3 + i) * 64];
       }
+    }
+  };
+  const uint8_t* keys = key_data(a, chunk0, kh, DK);
+  const int64_t keys_step = (int64_t)a.k_heads * bytes_kt(DK);
+  const auto load_kt = [&]() {
+    const i32x4* p = reinterpret_cast<const i32x4*>(keys) + wave * MT * 2 * 64 + lane;
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) kt[x][m] = p[(m * 2 + x) * 64];
     const float* f = reinterpret_cast<const float*>(data + kBytesT + kBytesM) + wave * 16 + r4;
-    const f32x4 from_k = *reinterpret_cast<const f32x4*>(f + kFromK * kChunk), from_q = *reinterpret_cast<const f32x4*>(f + kFromQ * kChunk);
-    const f32x4 beta = *reinterpret_cast<const f32x4*>(f + kBeta * kChunk), to_end = *reinterpret_cast<const f32x4*>(f + kToEnd * kChunk);
-    const float end = f[kEnd * kChunk];
+    from_k = *reinterpret_cast<const f32x4*>(f + kFromK * kChunk), beta = *reinterpret_cast<const f32x4*>(f + kBeta * kChunk);
+    to_end = *reinterpret_cast<const f32x4*>(f + kToEnd * kChunk);
+    end = f[kEnd * kChunk];
+  };
+  // in the order of the loop, whose waits count the loads behind the one that is waited for
+  load_k(0);
+  __builtin_amdgcn_sched_barrier(0);
+  load_v(0);
+  __builtin_amdgcn_sched_barrier(0);
+  load_t(data);
+  __builtin_amdgcn_sched_barrier(0);
+  load_kt();
+  __builtin_amdgcn_sched_barrier(0);
 
+  for (int chunk = 0; chunk <= last; ++chunk) {
+    const int rows = n - chunk * kChunk, place = chunk0 + chunk, next = min(chunk + 1, last);
+    int* first_u = first_us[place & 1];
     // the state in three parts, columns as rows
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -436,68 +1053,79 @@ __global__ __launch_bounds__(256) void scan_kernel(LinearArgs a, int v_dim, uint
         split2<3>(s[m][c][0], s[m][c][1], p[0]), split2<3>(s[m][c][2], s[m][c][3], p[1]);
 #pragma unroll
         for (int i = 0; i < 3; ++i)
-          *reinterpret_cast<uint2*>(&sb[i][(c * 16 + r16) * kRowS + wave * (DK / 4) + m * 16 + r4]) = uint2{p[0][i], p[1][i]};
+          *reinterpret_cast<uint2*>(&sb[i][(c * 16 + r16) * kRowS + state_row(wave * MT + m, lane >> 4)]) = uint2{p[0][i], p[1][i]};
       }
-    __syncthreads();
-    int* first_u = first_us[place & 1];
+    lds_barrier();
     if (tid < kCols) first_us[(place + 1) & 1][tid] = kChunk;
-
-    f32x4 pk[NT], pq[NT];
+    float v[NT][4];
 #pragma unroll
-    for (int c = 0; c < NT; ++c) pk[c] = pq[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < NT; ++c)
 #pragma unroll
-    for (int x = 0; x < KS; ++x) {
-      i32x4 kp[NP], qp[NP];
-      Parts<H>::of(kf[x], kp), Parts<H>::of(qf[x], qp);
-#pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        i32x4 sp[3];
-#pragma unroll
-        for (int i = 0; i < 3; ++i) sp[i] = *reinterpret_cast<const i32x4*>(&sb[i][(c * 16 + r16) * kRowS + x * 32 + k8]);
-        if (BETA) {
-#pragma unroll
-          for (int i = 0; i < 3; ++i) pk[c] = mfma_bf16(kp[0], sp[i], pk[c]);
-          if (NP > 1) pk[c] = mfma_bf16(kp[NP - 1], sp[0], mfma_bf16(kp[NP - 1], sp[1], pk[c]));
-        }
-        pq[c] = mfma_bf16(qp[0], sp[0], mfma_bf16(qp[0], sp[1], pq[c]));
-        if (NP > 1) pq[c] = mfma_bf16(qp[NP - 1], sp[0], pq[c]);
-      }
-    }
+      for (int r = 0; r < 4; ++r) v[c][r] = H::lo(v16[c][r] & (uint32_t)((wave * 16 + r4 + r - rows) >> 31));  // 0 behind the end
+    load_v(next);
 
     f32x4 u[NT];
     if constexpr (BETA) {
-      uint32_t bad = 0;
+      if (rows < kChunk)
 #pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        float d[4];
+        for (int x = 0; x < KS; ++x) kf[x] &= (row16 - rows) >> 31;
+      f32x4 pk[NT][2];
+#pragma unroll
+      for (int c = 0; c < NT; ++c) pk[c][0] = pk[c][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int x = 0; x < KS; ++x) {
+        i32x4 kp[NP];
+        Parts<H>::of(kf[x], kp);
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+          i32x4 sp[3];
+#pragma unroll
+          for (int i = 0; i < 3; ++i) sp[i] = *reinterpret_cast<const i32x4*>(&sb[i][(c * 16 + r16) * kRowS + x * 32 + k8]);
+          pk[c][1] = mfma_bf16(kp[0], sp[2], pk[c][1]), pk[c][0] = mfma_bf16(kp[0], sp[0], pk[c][0]);
+          pk[c][1] = mfma_bf16(kp[0], sp[1], pk[c][1]);
+          if (NP > 1) pk[c][1] = mfma_bf16(kp[NP - 1], sp[1], pk[c][1]), pk[c][1] = mfma_bf16(kp[NP - 1], sp[0], pk[c][1]);
+        }
+      }
+      load_k(next);
+      uint32_t bad = 0;
+      float d[NT][4];
+#pragma unroll
+      for (int c = 0; c < NT; ++c)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          d[r] = beta[r] * (v[c][r] - from_k[r] * pk[c][r]);
-          if (!(__builtin_fabsf(d[r]) < __builtin_inff())) bad |= 1u << (c * 4 + r);
+          d[c][r] = __builtin_fmaf(-from_k[r], pk[c][0][r] + pk[c][1][r], beta[r] * v[c][r]);
+          if (!(__builtin_fabsf(d[c][r]) < __builtin_inff())) bad |= 1u << (c * 4 + r);
         }
-        uint32_t p[2][3];
-        split2<3>(d[0], d[1], p[0]), split2<3>(d[2], d[3], p[1]);
+      const auto hand_over_d = [&]() {
 #pragma unroll
-        for (int i = 0; i < 3; ++i)
-          *reinterpret_cast<uint2*>(&db[i][(c * 16 + r16) * kRowU + wave * 16 + r4]) = uint2{p[0][i], p[1][i]};
-      }
+        for (int c = 0; c < NT; ++c) {
+          uint32_t p[2][3];
+          split2<3>(d[c][0], d[c][1], p[0]), split2<3>(d[c][2], d[c][3], p[1]);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) *reinterpret_cast<uint2*>(&db[i][(c * 16 + r16) * kRowU + place4]) = uint2{p[0][i], p[1][i]};
+        }
+      };
+      hand_over_d();
       if (__ballot(bad != 0)) {
 #pragma unroll
         for (int c = 0; c < NT; ++c)
           if ((bad >> (4 * c)) & 15) atomicMin(&first_d[c * 16 + r16], wave * 16 + r4 + __builtin_ctz((bad >> (4 * c)) & 15));
       }
-      __syncthreads();
+      lds_barrier();
       const bool spoilt = __ballot(first_d[lane & (kCols - 1)] < kChunk) != 0;
       if (spoilt) {
         // rows behind a column's first one that is not finite must not reach those before it
-        for (int i = tid; i < kCols * kChunk; i += 256)
-          if ((i & (kChunk - 1)) >= first_d[i / kChunk])
-            db[0][i / kChunk * kRowU + (i & (kChunk - 1))] = db[1][i / kChunk * kRowU + (i & (kChunk - 1))] =
-                db[2][i / kChunk * kRowU + (i & (kChunk - 1))] = 0;
-        __syncthreads();
-      }
 #pragma unroll
-      for (int c = 0; c < NT; ++c) u[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < NT; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (wave * 16 + r4 + r >= first_d[c * 16 + r16]) d[c][r] = 0.0f;
+        hand_over_d();
+        lds_barrier();
+      }
+      f32x4 td[NT][3];
+#pragma unroll
+      for (int c = 0; c < NT; ++c) td[c][0] = td[c][1] = td[c][2] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         if (x > (wave >> 1)) break;
@@ -507,10 +1135,14 @@ __global__ __launch_bounds__(256) void scan_kernel(LinearArgs a, int v_dim, uint
           i32x4 d[3];
 #pragma unroll
           for (int i = 0; i < 3; ++i) d[i] = *reinterpret_cast<const i32x4*>(&db[i][(c * 16 + r16) * kRowU + x * 32 + k8]);
-          u[c] = mfma_bf16(t[0], d[2], u[c]), u[c] = mfma_bf16(t[2], d[0], u[c]), u[c] = mfma_bf16(t[1], d[1], u[c]);
-          u[c] = mfma_bf16(t[0], d[1], u[c]), u[c] = mfma_bf16(t[1], d[0], u[c]), u[c] = mfma_bf16(t[0], d[0], u[c]);
+          td[c][2] = mfma_bf16(t[0], d[2], td[c][2]), td[c][1] = mfma_bf16(t[0], d[1], td[c][1]);
+          td[c][0] = mfma_bf16(t[0], d[0], td[c][0]), td[c][2] = mfma_bf16(t[1], d[1], td[c][2]);
+          td[c][1] = mfma_bf16(t[1], d[0], td[c][1]), td[c][2] = mfma_bf16(t[2], d[0], td[c][2]);
         }
       }
+#pragma unroll
+      for (int c = 0; c < NT; ++c) u[c] = td[c][0] + (td[c][1] + td[c][2]);
+      load_t(data + (chunk < last ? data_step : 0));
       if (spoilt) {
 #pragma unroll
         for (int c = 0; c < NT; ++c)
@@ -523,56 +1155,46 @@ __global__ __launch_bounds__(256) void scan_kernel(LinearArgs a, int v_dim, uint
       for (int c = 0; c < NT; ++c) u[c] = f32x4{v[c][0], v[c][1], v[c][2], v[c][3]};
     }
 
-    {
-      uint32_t bad = 0;
+    const auto hand_over = [&]() {
 #pragma unroll
       for (int c = 0; c < NT; ++c) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (!(__builtin_fabsf(u[c][r]) < __builtin_inff())) bad |= 1u << (c * 4 + r);
         uint32_t p[2][2], w[2][3];
         split2<2>(u[c][0], u[c][1], p[0]), split2<2>(u[c][2], u[c][3], p[1]);
         split2<3>(u[c][0] * to_end[0], u[c][1] * to_end[1], w[0]), split2<3>(u[c][2] * to_end[2], u[c][3] * to_end[3], w[1]);
-        const int at = (c * 16 + r16) * kRowU + wave * 16 + r4;
+        const int at = (c * 16 + r16) * kRowU + place4;
 #pragma unroll
         for (int i = 0; i < 2; ++i) *reinterpret_cast<uint2*>(&ub[i][at]) = uint2{p[0][i], p[1][i]};
 #pragma unroll
         for (int i = 0; i < 3; ++i) *reinterpret_cast<uint2*>(&ub[2 + i][at]) = uint2{w[0][i], w[1][i]};
       }
+    };
+    {
+      uint32_t bad = 0;
+#pragma unroll
+      for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (!(__builtin_fabsf(u[c][r]) < __builtin_inff())) bad |= 1u << (c * 4 + r);
+      hand_over();
       if (__ballot(bad != 0)) {
 #pragma unroll
         for (int c = 0; c < NT; ++c)
           if ((bad >> (4 * c)) & 15) atomicMin(&first_u[c * 16 + r16], wave * 16 + r4 + __builtin_ctz((bad >> (4 * c)) & 15));
       }
     }
-    __syncthreads();
+    lds_barrier();
     const bool spoilt = __ballot(first_u[lane & (kCols - 1)] < kChunk) != 0;
     if (spoilt) {
-      for (int i = tid; i < kCols * kChunk; i += 256)
-        if ((i & (kChunk - 1)) >= first_u[i / kChunk])
 #pragma unroll
-          for (int p = 0; p < 5; ++p) ub[p][i / kChunk * kRowU + (i & (kChunk - 1))] = 0;
-      __syncthreads();
+      for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (wave * 16 + r4 + r >= first_u[c * 16 + r16]) u[c][r] = 0.0f;
+      hand_over();
+      lds_barrier();
     }
     if (tid < kCols) first_d[tid] = kChunk;
 
-    // the chunk's outputs
-    f32x4 o[NT];
-#pragma unroll
-    for (int c = 0; c < NT; ++c)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o[c][r] = from_q[r] * pq[c][r];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if (x > (wave >> 1)) break;
-      const i32x4* m = mf[x];
-#pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        const i32x4 u0 = *reinterpret_cast<const i32x4*>(&ub[0][(c * 16 + r16) * kRowU + x * 32 + k8]);
-        const i32x4 u1 = *reinterpret_cast<const i32x4*>(&ub[1][(c * 16 + r16) * kRowU + x * 32 + k8]);
-        o[c] = mfma_bf16(m[1], u0, o[c]), o[c] = mfma_bf16(m[0], u1, o[c]), o[c] = mfma_bf16(m[0], u0, o[c]);
-      }
-    }
     // the state behind the chunk
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -585,55 +1207,39 @@ __global__ __launch_bounds__(256) void scan_kernel(LinearArgs a, int v_dim, uint
         i32x4 up[3];
 #pragma unroll
         for (int i = 0; i < 3; ++i) up[i] = *reinterpret_cast<const i32x4*>(&ub[2 + i][(c * 16 + r16) * kRowU + x * 32 + k8]);
+        i32x4 kp[MT][NP];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          i32x4 kp[NP];
-          Parts<H>::of(kt[x][m], kp);
-          s[m][c] = mfma_bf16(kp[0], up[2], s[m][c]), s[m][c] = mfma_bf16(kp[0], up[1], s[m][c]);
-          if (NP > 1) s[m][c] = mfma_bf16(kp[NP - 1], up[1], s[m][c]), s[m][c] = mfma_bf16(kp[NP - 1], up[0], s[m][c]);
-          s[m][c] = mfma_bf16(kp[0], up[0], s[m][c]);
-        }
+        for (int m = 0; m < MT; ++m) Parts<H>::of(kt[x][m], kp[m]);
+#pragma unroll
+        for (int i = 2; i >= 0; --i)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            if (NP > 1 && i < 2) s[m][c] = mfma_bf16(kp[m][NP - 1], up[i], s[m][c]);
+            s[m][c] = mfma_bf16(kp[m][0], up[i], s[m][c]);
+          }
       }
     }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) settle(s[m]);
+    data += chunk < last ? data_step : 0, keys += chunk < last ? keys_step : 0;
+    load_kt();
     if (spoilt) {
 #pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        const int bad = first_u[c * 16 + r16];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (wave * 16 + r4 + r >= bad) o[c][r] = __builtin_nanf("");
-        if (bad < kChunk)
+      for (int c = 0; c < NT; ++c)
+        if (first_u[c * 16 + r16] < kChunk)
 #pragma unroll
           for (int m = 0; m < MT; ++m) s[m][c] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < NT; ++c) {
-      const uint32_t p[2] = {H::pack(o[c][0], o[c][1]), H::pack(o[c][2], o[c][3])};
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = wave * 16 + r4 + r;
-        if (i < rows) a.out[((int64_t)(first + i) * a.v_heads + head) * v_dim + col0 + c * 16] = (uint16_t)(p[r >> 1] >> (16 * (r & 1)));
-      }
     }
   }
   if (to >= 0 && to < b.n_slots) {
-    float* p = a.states + ((int64_t)to * a.v_heads + head) * slot_size;
+    float* p = a.states + ((int64_t)to * a.v_heads + head) * slot_size + col0;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int c = 0; c < NT; ++c)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[(int64_t)(wave * (DK / 4) + m * 16 + r4 + r) * v_dim + col0 + c * 16] = s[m][c][r];
+        for (int r = 0; r < 4; ++r) p[(state_row(wave * MT + m, lane >> 4) + r) * v_dim + c * 16] = s[m][c][r];
   }
-}
-
-// Tokens before the first sequence's and behind the last's come out as 0.
-__global__ __launch_bounds__(256) void clear_kernel(LinearArgs a, int64_t row_chunks) {
-  const int lo = clamp_to(a.b.starts[0], a.b.tokens), hi = clamp_to(a.b.starts[a.b.batch], a.b.tokens);
-  const int64_t before = lo * row_chunks, all = before + (a.b.tokens - hi) * row_chunks, skip = (hi - lo) * row_chunks;
-  uint4* out = reinterpret_cast<uint4*>(a.out);
-  for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < all; i += gridDim.x * 256) out[i < before ? i : i + skip] = uint4{0, 0, 0, 0};
 }
 
 template <class H>
@@ -651,12 +1257,17 @@ hipError_t linear_step(const LinearArgs& a, int k_dim, int v_dim, bool fp16, hip
 
 template <class H, int DK, bool BETA>
 static void launch_prompt(const LinearArgs& a, int v_dim, hipStream_t stream) {
-  const uint32_t cols = (uint32_t)v_dim / kCols;
   const uint32_t places = (uint32_t)linear_chunks(a.b.tokens, a.b.batch);
-  prepare_kernel<H, DK, BETA><<<places * (uint32_t)a.v_heads, 256, 0, stream>>>(a);
-  scan_kernel<H, DK, BETA><<<(uint32_t)a.b.batch * (uint32_t)a.v_heads * cols, 256, 0, stream>>>(a, v_dim, cols);
-  const int64_t row_chunks = (int64_t)a.v_heads * v_dim / 8;
-  clear_kernel<<<256, 256, 0, stream>>>(a, row_chunks);
+  prepare_kernel<H, DK, BETA><<<places * (uint32_t)a.v_heads, 256, 0, stream>>>(a, v_dim);
+  const uint32_t heads = (uint32_t)a.b.batch * (uint32_t)a.v_heads, cols = (uint32_t)v_dim;
+  if (heads * (cols / 16) <= 256)
+    scan_few_kernel<H, DK, 16, BETA><<<heads * (cols / 16), 512, 0, stream>>>(a, v_dim, cols / 16);
+  else if (DK < 256 && heads * (cols / 32) <= 256)
+    scan_few_kernel<H, DK < 256 ? DK : 128, 32, BETA><<<heads * (cols / 32), 512, 0, stream>>>(a, v_dim, cols / 32);
+  else if (DK == 256 || v_dim == 64)
+    scan_kernel<H, DK, 4, BETA><<<heads * (cols / 64), 256, 0, stream>>>(a, v_dim, cols / 64);
+  else
+    scan_kernel<H, DK < 256 ? DK : 128, 8, BETA><<<heads * (cols / 128), 512, 0, stream>>>(a, v_dim, cols / 128);
 }
 
 template <class H>
