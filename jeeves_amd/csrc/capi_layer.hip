@@ -101,7 +101,7 @@ int jv_causal_conv(const void* x, int64_t x_ts, const float* weight, const float
     return fail(JV_ERR_VALUE, "the convolution takes a multiple of 8 channels up to 65536, got %lld", (long long)channels);
   if (activation != JV_CONV_PLAIN && activation != JV_CONV_SILU) return fail(JV_ERR_VALUE, "unknown activation %d", activation);
   if (int rc = check_batch(tokens, batch, starts, slots, n_slots, states)) return rc;
-  if ((tokens + 1) * ((channels + 511) / 512) / 4 >= kMaxGrid)
+  if ((tokens + 1) * ((channels + 255) / 256) / 4 >= kMaxGrid)
     return fail(JV_ERR_VALUE, "too many rows for one call: %lld tokens of %lld channels", (long long)tokens, (long long)channels);
   if (tokens == 0) return JV_OK;
   if (int rc = check_rows("x", x, x_ts, 0)) return rc;

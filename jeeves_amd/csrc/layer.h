@@ -22,8 +22,16 @@ __device__ __forceinline__ float inv_sqrt(float m) {
 }
 
 // 1 / (1 + e^-x) and x / (1 + e^-x), in the steps of the elementary operations
-// (exponential, sum, IEEE division, product), each rounded.
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+// (exponential, sum, quotient, product), each rounded. The quotient is the
+// hardware's with one Newton step, which rounds as the division does; past
+// 2^126, where the hardware has no quotient, it is the division (five
+// instructions instead of ten: 16 prompts through the convolution 96 -> 84 us).
+__device__ __forceinline__ float sigmoid(float x) {
+  const float d = 1.0f + expf(-x);
+  if (d >= 0x1p126f) return 1.0f / d;
+  const float r = __builtin_amdgcn_rcpf(d);
+  return __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+}
 __device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
 
 // log(1 + e^x) = max(x, 0) + log1p(u), u = e^-|x| <= 1, with log1p(u) =

@@ -1259,11 +1259,12 @@ template <class H, int DK, bool BETA>
 static void launch_prompt(const LinearArgs& a, int v_dim, hipStream_t stream) {
   const uint32_t places = (uint32_t)linear_chunks(a.b.tokens, a.b.batch);
   prepare_kernel<H, DK, BETA><<<places * (uint32_t)a.v_heads, 256, 0, stream>>>(a, v_dim);
-  const uint32_t heads = (uint32_t)a.b.batch * (uint32_t)a.v_heads, cols = (uint32_t)v_dim;
-  if (heads * (cols / 16) <= 256)
-    scan_few_kernel<H, DK, 16, BETA><<<heads * (cols / 16), 512, 0, stream>>>(a, v_dim, cols / 16);
-  else if (DK < 256 && heads * (cols / 32) <= 256)
-    scan_few_kernel<H, DK < 256 ? DK : 128, 32, BETA><<<heads * (cols / 32), 512, 0, stream>>>(a, v_dim, cols / 32);
+  const uint32_t heads = (uint32_t)a.b.batch * (uint32_t)a.v_heads, cols = (uint32_t)v_dim, w16 = heads * (cols / 16);
+  const uint32_t cus = (uint32_t)max(cu_count_of(-1), 1);
+  if (w16 <= (DK == 128 ? cus : 2 * cus))
+    scan_few_kernel<H, DK, 16, BETA><<<w16, 512, 0, stream>>>(a, v_dim, cols / 16);
+  else if (DK == 128 && w16 / 2 <= cus)
+    scan_few_kernel<H, 128, 32, BETA><<<w16 / 2, 512, 0, stream>>>(a, v_dim, cols / 32);
   else if (DK == 256 || v_dim == 64)
     scan_kernel<H, DK, 4, BETA><<<heads * (cols / 64), 256, 0, stream>>>(a, v_dim, cols / 64);
   else

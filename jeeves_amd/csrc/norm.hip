@@ -153,11 +153,13 @@ __global__ __launch_bounds__(512) void block_norm_kernel(NormArgs a) {
   const float scale = scale_from_amax_f32(__uint_as_float(top));
   if (threadIdx.x == 0 && real) a.scales[row] = scale;
   const bool finite = top < 0x7F800000u;
+  const float inv = 1.0f / scale;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     float q[8];
+    // with the correctly rounded 1 / scale the corrected product is the IEEE quotient
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = f[i][e] / scale;
+    for (int e = 0; e < 8; ++e) q[e] = finite ? __builtin_copysignf(quotient(f[i][e], scale, inv), f[i][e]) : f[i][e] / scale;
     uint2 code = {0u, 0u};
     if (finite) {
       int lo = cvt_pk_fp8<false>(q[0], q[1], 0), hi = cvt_pk_fp8<false>(q[4], q[5], 0);
