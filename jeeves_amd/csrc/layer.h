@@ -21,18 +21,24 @@ __device__ __forceinline__ float inv_sqrt(float m) {
   return r * (tiny ? 0x1p30f : 1.0f);
 }
 
-// 1 / (1 + e^-x) and x / (1 + e^-x), in the steps of the elementary operations
-// (exponential, sum, quotient, product), each rounded. The quotient is the
-// hardware's with one Newton step, which rounds as the division does; past
-// 2^126, where the hardware has no quotient, it is the division (five
-// instructions instead of ten: 16 prompts through the convolution 96 -> 84 us).
-__device__ __forceinline__ float sigmoid(float x) {
-  const float d = 1.0f + expf(-x);
+// 1 / d, d at least 1: the hardware's with one Newton step, which rounds as the
+// division does; past 2^126, where the hardware has no quotient, the division
+// (five instructions instead of ten: 16 prompts through the convolution 96 ->
+// 84 us).
+__device__ __forceinline__ float inverse(float d) {
   if (d >= 0x1p126f) return 1.0f / d;
   const float r = __builtin_amdgcn_rcpf(d);
   return __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
 }
+
+// 1 / (1 + e^-x) and x / (1 + e^-x) in the steps of the elementary operations
+// (exponential, sum, quotient, product), each rounded.
+__device__ __forceinline__ float sigmoid(float x) { return inverse(1.0f + expf(-x)); }
 __device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
+
+// The first by the hardware's 2^x alone: the product's rounding puts |x| 2^-24
+// into the exponential, which counts where that is not small against 1.
+__device__ __forceinline__ float quick_sigmoid(float x) { return inverse(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e)); }
 
 // log(1 + e^x) = max(x, 0) + log1p(u), u = e^-|x| <= 1, with log1p(u) =
 // 2 atanh(s), s = u / (2 + u) <= 1/3, by the series s + s^3/3 + .. + s^15/15

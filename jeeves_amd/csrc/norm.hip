@@ -106,7 +106,10 @@ __global__ __launch_bounds__(512) void block_norm_kernel(NormArgs a) {
       float g[8];
       unpack(gv[i], g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[i][e] *= a.activation == 2 ? silu(g[e]) : a.activation == 1 ? sigmoid(g[e]) : g[e];
+      for (int e = 0; e < 8; ++e) {
+        const float s = a.activation ? quick_sigmoid(g[e]) : g[e];
+        f[i][e] *= a.activation == 2 ? g[e] * s : s;
+      }
     }
   }
 #pragma unroll
