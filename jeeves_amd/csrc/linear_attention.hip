@@ -239,8 +239,12 @@ __device__ __forceinline__ int fragment_of(int t, int x) { return x ? t + 2 : t;
 template <class H, int DK, bool BETA>
 __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
   constexpr int KS = DK / 32, kRow = 68, kRowK = DK + 8, kRowD = 20;
-  __shared__ __attribute__((aligned(16))) uint16_t krows[kChunk * kRowK];
-  __shared__ __attribute__((aligned(16))) float tri[BETA ? kChunk * kRow : 4];
+  // K's rows, and in their place A once they are read: five workgroups a CU
+  // instead of three (16384 tokens 120 -> 105 us).
+  constexpr int kShared = kChunk * (BETA && kRow * 4 > kRowK * 2 ? kRow * 4 : kRowK * 2);
+  __shared__ __attribute__((aligned(16))) uint8_t shared[kShared];
+  uint16_t* krows = reinterpret_cast<uint16_t*>(shared);
+  float* tri = reinterpret_cast<float*>(shared);
   __shared__ __attribute__((aligned(16))) float diagonal[BETA ? 4 : 1][16 * kRowD];
   __shared__ __attribute__((aligned(16))) double sum[kChunk];
   __shared__ __attribute__((aligned(16))) float rk[kChunk], rq[kChunk], betas[kChunk];
@@ -335,6 +339,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
   const double sum_i = sum[i];
   const float rk_i = rk[i], rq_i = rq[i], beta_i = betas[i];
   uint2 mp[4][2];
+  f32x4 pull[BETA ? 4 : 1];
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     mp[t][0] = mp[t][1] = uint2{0u, 0u};
@@ -346,16 +351,15 @@ __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
       kk = H::mfma16(kb, kf[s], kk), qk = H::mfma16(kb, qf[s], qk);
     }
     const f32x4 rk_j = *reinterpret_cast<const f32x4*>(&rk[t * 16 + g * 4]);
-    f32x4 pull;
     float m[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int j = t * 16 + g * 4 + r;
       const float e = __builtin_amdgcn_exp2f((float)(sum_i - sum[j])) * rk_j[r];
       const float x = kk[r] * e * rk_i * beta_i, y = qk[r] * e * rq_i;
-      pull[r] = j < i ? x : 0.0f, m[r] = j <= i ? y : 0.0f;
+      if constexpr (BETA) pull[t][r] = j < i ? x : 0.0f;
+      m[r] = j <= i ? y : 0.0f;
     }
-    if constexpr (BETA) *reinterpret_cast<f32x4*>(&tri[i * kRow + t * 16 + g * 4]) = pull;
     uint32_t p[2][2];
     split2<2>(m[0], m[1], p[0]), split2<2>(m[2], m[3], p[1]);
     mp[t][0] = uint2{p[0][0], p[1][0]}, mp[t][1] = uint2{p[0][1], p[1][1]};
@@ -391,6 +395,10 @@ __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
   }
 
   if constexpr (BETA) {
+    lds_barrier();
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      if (t <= wave) *reinterpret_cast<f32x4*>(&tri[i * kRow + t * 16 + g * 4]) = pull[t];
     lds_barrier();
     // T by blocks of 16 rows. Wave w inverts the diagonal block w by forward
     // substitution, a column a lane (every 16 lanes the same), then works out
@@ -832,7 +840,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void scan_kernel(LinearArgs a, int
 //   U = T D in two parts, e^(G_C - G) U in three           -> ub, as that of M U and of K^T U, which gives the state
 // Waves 0 to 3 go through them, wave w with a chunk's rows from 16 w on and the
 // state's from w DK / 4 on. Waves 4 to 7 have the rows' outputs e^G Q S + M U,
-// which no later chunk waits for. An operand is loaded for the next chunk once
+// which no later chunk waits for, and bring the factors and V to LDS (a load's
+// issue is a wait of 16 to 32 cycles). An operand is loaded for the next chunk once
 // this one has used it, so that a load has most of a chunk's time and no
 // register of its own.
 template <class H, int DK, int kCols, bool BETA>
@@ -842,6 +851,8 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
   __shared__ __attribute__((aligned(16))) uint16_t sb[3][kCols * kRowS];
   __shared__ __attribute__((aligned(16))) uint16_t db[BETA ? 3 : 1][kCols * kRowU];
   __shared__ __attribute__((aligned(16))) uint16_t ub[5][kCols * kRowU];
+  __shared__ __attribute__((aligned(16))) float fb[2][5 * kChunk];            // the rows' factors, by turns
+  __shared__ __attribute__((aligned(16))) uint16_t vb[2][kChunk * kCols];     // and V's rows
   __shared__ int first_d[kCols], first_us[2][kCols];  // a column's first row that is not finite; U's by turns
   const int tid = threadIdx.x, lane = tid & 63, all_wave = __builtin_amdgcn_readfirstlane(tid >> 6), wave = all_wave & 3;
   // The hardware hands consecutive workgroups to the 8 XCDs in turn: those of
@@ -861,7 +872,6 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
 
   if (all_wave >= 4) {
     i32x4 qf[KS], mf[2][2];
-    f32x4 from_q;
     const uint16_t* q_next = a.q + (int64_t)(start + row16) * a.q_ts + kh * a.q_hs + k8;
     const auto load_q = [&](int c) {
       const int rows = n - c * kChunk;
@@ -877,12 +887,36 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
         if (x > (wave >> 1)) break;
         mf[x][0] = p[fragment_of(wave, x) * 128], mf[x][1] = p[fragment_of(wave, x) * 128 + 64];
       }
-      from_q = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(d + kBytesT + kBytesM) + kFromQ * kChunk + wave * 16 + r4);
     };
+    // 80 times 16 bytes of factors and kCols / 8 of each row of V
+    constexpr int kItems = 80 + kChunk * kCols / 8, kMine = (kItems + 255) / 256;
+    const int item = (all_wave - 4) * 64 + lane;
+    i32x4 held[kMine];
+    const auto load_held = [&](int c) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int at = min(item + i * 256, kItems - 1), v_at = max(at - 80, 0) * 8, row = min(v_at / kCols, n - c * kChunk - 1);
+        const uint16_t* v = a.v + (int64_t)(start + c * kChunk + row) * a.v_ts + head * a.v_hs + cb * kCols + v_at % kCols;
+        const uint8_t* f = head_data(a, chunk0 + c, head) + kBytesT + kBytesM + at * 16;
+        held[i] = *reinterpret_cast<const i32x4*>(at < 80 ? f : reinterpret_cast<const uint8_t*>(v));
+      }
+    };
+    const auto put_held = [&](int c) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int at = item + i * 256;
+        if (at < 80) *reinterpret_cast<i32x4*>(&fb[c & 1][at * 4]) = held[i];
+        else if (at < kItems) *reinterpret_cast<i32x4*>(&vb[c & 1][(at - 80) * 8]) = held[i];
+      }
+    };
+    load_held(0);
+    __builtin_amdgcn_sched_barrier(0);
     load_q(0);
     __builtin_amdgcn_sched_barrier(0);
     load_m(data);
     __builtin_amdgcn_sched_barrier(0);
+    put_held(0);
+    load_held(min(1, last));
     uint16_t* out = a.out + ((int64_t)(start + wave * 16 + r4) * a.v_heads + head) * v_dim + col0;
     const int64_t out_ts = (int64_t)a.v_heads * v_dim;
     for (int chunk = 0; chunk <= last; ++chunk) {
@@ -905,6 +939,9 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
         }
       }
       load_q(min(chunk + 1, last));
+      const f32x4 from_q = *reinterpret_cast<const f32x4*>(&fb[chunk & 1][kFromQ * kChunk + wave * 16 + r4]);
+      put_held(chunk + 1);
+      load_held(min(chunk + 2, last));
       if constexpr (BETA) {
         lds_barrier();
         if (__ballot(first_d[lane & (kCols - 1)] < kChunk)) lds_barrier();
@@ -977,11 +1014,7 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
         for (int r = 0; r < 4; ++r) s[m][c][r] = p[(state_row(wave * MT + m, lane >> 4) + r) * v_dim + c * 16];
   }
   i32x4 kf[KS], tf[BETA ? 2 : 1][3], kt[2][MT];
-  uint32_t v16[NT][4];
-  f32x4 from_k, beta, to_end;
-  float end;
   const uint16_t* k_next = a.k + (int64_t)(start + row16) * a.k_ts + kh * a.k_hs + k8;
-  const uint16_t* v_next = a.v + (int64_t)(start + wave * 16 + r4) * a.v_ts + head * a.v_hs + col0;
   const auto load_k = [&](int c) {
     if constexpr (BETA) {
       const int rows = n - c * kChunk;
@@ -990,22 +1023,6 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
       for (int x = 0; x < KS; ++x) kf[x] = *reinterpret_cast<const i32x4*>(p + x * 32);
       k_next += c < last ? kChunk * a.k_ts : 0;  // never past the last chunk, which is loaded again
     }
-  };
-  const auto load_v = [&](int c) {
-    const int rows = n - c * kChunk;
-    if (rows >= kChunk) {
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v16[x][r] = v_next[r * a.v_ts + x * 16];
-    } else {
-      const uint16_t* p = a.v + (int64_t)(start + c * kChunk) * a.v_ts + head * a.v_hs + col0;
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v16[x][r] = p[min(wave * 16 + r4 + r, rows - 1) * a.v_ts + x * 16];
-    }
-    v_next += c < last ? kChunk * a.v_ts : 0;  // never past the last chunk, which is loaded again
   };
   const auto load_t = [&](const uint8_t* d) {
     if constexpr (BETA) {
@@ -1026,15 +1043,17 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
     for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int m = 0; m < MT; ++m) kt[x][m] = p[(m * 2 + x) * 64];
-    const float* f = reinterpret_cast<const float*>(data + kBytesT + kBytesM) + wave * 16 + r4;
-    from_k = *reinterpret_cast<const f32x4*>(f + kFromK * kChunk), beta = *reinterpret_cast<const f32x4*>(f + kBeta * kChunk);
-    to_end = *reinterpret_cast<const f32x4*>(f + kToEnd * kChunk);
-    end = f[kEnd * kChunk];
+  };
+  // what of a lane's rows is not finite
+  const auto mark = [&](int* first, const auto& x) {
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (!(__builtin_fabsf(x[c][r]) < __builtin_inff())) atomicMin(&first[c * 16 + r16], wave * 16 + r4 + r);
   };
   // in the order of the loop, whose waits count the loads behind the one that is waited for
   load_k(0);
-  __builtin_amdgcn_sched_barrier(0);
-  load_v(0);
   __builtin_amdgcn_sched_barrier(0);
   load_t(data);
   __builtin_amdgcn_sched_barrier(0);
@@ -1057,19 +1076,11 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
       }
     lds_barrier();
     if (tid < kCols) first_us[(place + 1) & 1][tid] = kChunk;
-    float v[NT][4];
-#pragma unroll
-    for (int c = 0; c < NT; ++c)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[c][r] = H::lo(v16[c][r] & (uint32_t)((wave * 16 + r4 + r - rows) >> 31));  // 0 behind the end
-    load_v(next);
-
-    f32x4 u[NT];
+    f32x4 u[NT], pk[NT][2];
     if constexpr (BETA) {
       if (rows < kChunk)
 #pragma unroll
         for (int x = 0; x < KS; ++x) kf[x] &= (row16 - rows) >> 31;
-      f32x4 pk[NT][2];
 #pragma unroll
       for (int c = 0; c < NT; ++c) pk[c][0] = pk[c][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -1087,14 +1098,27 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
         }
       }
       load_k(next);
-      uint32_t bad = 0;
-      float d[NT][4];
+    }
+    float v[NT][4];
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t x = vb[chunk & 1][(wave * 16 + r4 + r) * kCols + c * 16 + r16];
+        v[c][r] = H::lo(x & (uint32_t)((wave * 16 + r4 + r - rows) >> 31));  // 0 behind the end
+      }
+    const auto factor = [&](int which) { return *reinterpret_cast<const f32x4*>(&fb[chunk & 1][which * kChunk + wave * 16 + r4]); };
+    const f32x4 from_k = factor(kFromK), beta = factor(kBeta), to_end = factor(kToEnd);
+    const float end = fb[chunk & 1][kEnd * kChunk];
+
+    if constexpr (BETA) {
+      float d[NT][4], z = 0.0f;
 #pragma unroll
       for (int c = 0; c < NT; ++c)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           d[c][r] = __builtin_fmaf(-from_k[r], pk[c][0][r] + pk[c][1][r], beta[r] * v[c][r]);
-          if (!(__builtin_fabsf(d[c][r]) < __builtin_inff())) bad |= 1u << (c * 4 + r);
+          z = __builtin_fmaf(d[c][r], 0.0f, z);
         }
       const auto hand_over_d = [&]() {
 #pragma unroll
@@ -1106,11 +1130,7 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
         }
       };
       hand_over_d();
-      if (__ballot(bad != 0)) {
-#pragma unroll
-        for (int c = 0; c < NT; ++c)
-          if ((bad >> (4 * c)) & 15) atomicMin(&first_d[c * 16 + r16], wave * 16 + r4 + __builtin_ctz((bad >> (4 * c)) & 15));
-      }
+      if (__ballot(z != z)) mark(first_d, d);
       lds_barrier();
       const bool spoilt = __ballot(first_d[lane & (kCols - 1)] < kChunk) != 0;
       if (spoilt) {
@@ -1169,18 +1189,13 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
       }
     };
     {
-      uint32_t bad = 0;
+      float z = 0.0f;
 #pragma unroll
       for (int c = 0; c < NT; ++c)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (!(__builtin_fabsf(u[c][r]) < __builtin_inff())) bad |= 1u << (c * 4 + r);
+        for (int r = 0; r < 4; ++r) z = __builtin_fmaf(u[c][r], 0.0f, z);
       hand_over();
-      if (__ballot(bad != 0)) {
-#pragma unroll
-        for (int c = 0; c < NT; ++c)
-          if ((bad >> (4 * c)) & 15) atomicMin(&first_u[c * 16 + r16], wave * 16 + r4 + __builtin_ctz((bad >> (4 * c)) & 15));
-      }
+      if (__ballot(z != z)) mark(first_u, u);
     }
     lds_barrier();
     const bool spoilt = __ballot(first_u[lane & (kCols - 1)] < kChunk) != 0;
