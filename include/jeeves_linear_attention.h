@@ -45,17 +45,17 @@ int jv_causal_conv(const void* x, int64_t x_ts, const float* weight, const float
                    int64_t batch, void* out, int64_t tokens, int64_t channels, int fp16, void* stream);
 
 /* Bytes of workspace jv_linear_attention needs for these sizes (0: none); -1 if
- * the sizes are refused. ragged: whether starts are given; beta: whether betas are. */
+ * the sizes are refused. ragged: whether starts are given. */
 int64_t jv_linear_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t k_heads, int64_t v_heads, int64_t k_dim,
-                                            int64_t v_dim, int ragged, int beta);
+                                            int64_t v_dim, int ragged);
 
 /*
  * Linear attention with a state S [k_dim, v_dim] for each value head: token by
  * token of a sequence
  *   S = e^g S;  u = beta (v - S^T k)  (u = v where beta is NULL);  S = S + k u^T;  out = scale S^T q
  * in fp32, out rounded once. Value head h reads query and key head
- * h / (v_heads / k_heads). With norm_eps > 0 q and k are divided by
- * sqrt(sum(x^2) + norm_eps) first.
+ * h / (v_heads / k_heads). With norm_eps > 0 (a normal float32) q and k are
+ * divided by sqrt(sum(x^2) + norm_eps) first.
  * g and beta of a token and value head: decay and beta [tokens, v_heads] with
  * row strides, float32 (gates16 = 0) or of the tensors' 16-bit type (gates16 =
  * 1); with rate (float32 [v_heads]; NULL: none) g = -rate softplus(decay +

@@ -70,7 +70,7 @@ SIGNATURES: dict[str, tuple] = {
     # include/jeeves_linear_attention.h
     "jv_causal_conv": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
                                c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p]),
-    "jv_linear_attention_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int]),
+    "jv_linear_attention_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int]),
     "jv_linear_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
                                     c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_float, c_void_p, c_int64, c_void_p,
                                     c_void_p, c_void_p, c_int64, c_float, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,

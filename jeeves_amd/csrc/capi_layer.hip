@@ -1,6 +1,7 @@
 // C ABI of the norms around a block, the short convolution and the linear
 // attention (declared in include/jeeves_norm.h and
 // include/jeeves_linear_attention.h): argument validation and launches only.
+#include <cfloat>
 #include <cmath>
 
 #include "../../include/jeeves_fp8.h"
@@ -118,9 +119,9 @@ int jv_causal_conv(const void* x, int64_t x_ts, const float* weight, const float
 }
 
 int64_t jv_linear_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t k_heads, int64_t v_heads, int64_t k_dim,
-                                            int64_t v_dim, int ragged, int beta) {
+                                            int64_t v_dim, int ragged) {
   if (check_dims(tokens, batch, k_heads, v_heads, k_dim, v_dim)) return -1;
-  return ragged && tokens && batch ? jv::linear_workspace(tokens, batch, k_heads, v_heads, k_dim, beta != 0) : 0;
+  return ragged && tokens && batch ? jv::linear_workspace(tokens, batch, k_heads, v_heads, k_dim) : 0;
 }
 
 int jv_linear_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs, const void* v,
@@ -132,7 +133,8 @@ int jv_linear_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k
   if (int rc = check_dims(tokens, batch, k_heads, v_heads, k_dim, v_dim)) return rc;
   if (int rc = check_batch(tokens, batch, starts, slots, n_slots, states)) return rc;
   if (!std::isfinite(scale)) return fail(JV_ERR_VALUE, "the scale must be finite, got %g", scale);
-  if (!(norm_eps >= 0.0f) || !std::isfinite(norm_eps)) return fail(JV_ERR_VALUE, "norm_eps is finite and at least 0, got %g", norm_eps);
+  if (norm_eps != 0.0f && !(norm_eps >= FLT_MIN && std::isfinite(norm_eps)))
+    return fail(JV_ERR_VALUE, "norm_eps is 0 or a normal float32, got %g", norm_eps);
   if (decay_bias && !rate) return fail(JV_ERR_VALUE, "a decay bias goes with the heads' rates");
   if (tokens == 0) return JV_OK;
   if (int rc = check_rows("q", q, q_ts, q_hs)) return rc;
@@ -140,7 +142,7 @@ int jv_linear_attention(const void* q, int64_t q_ts, int64_t q_hs, const void* k
   if (int rc = check_rows("v", v, v_ts, v_hs)) return rc;
   if (int rc = check_rows("the output", out, 0, 0)) return rc;
   if (!decay) return fail(JV_ERR_VALUE, "the decays are missing");
-  const int64_t need = starts ? jv::linear_workspace(tokens, batch, k_heads, v_heads, k_dim, beta != nullptr) : 0;
+  const int64_t need = starts ? jv::linear_workspace(tokens, batch, k_heads, v_heads, k_dim) : 0;
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
     return fail(JV_ERR_VALUE, "workspace needs %lld bytes, 256-byte aligned", (long long)need);
   jv::LinearArgs a{};

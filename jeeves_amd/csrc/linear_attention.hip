@@ -11,9 +11,10 @@
 //   O = scale (e^G Q S + M U),       M_ij = e^(G_i - G_j) q_i.k_j         (j <= i)
 //   S' = e^(G_C) S + K^T (e^(G_C - G) U)
 // prepare_kernel works out for all chunks at a time what does not depend on S:
-// T = (I + A)^-1 by forward substitution in fp32, M, the rows' factors and K's
-// transpose, all in the order in which scan_kernel's products read them.
-// scan_kernel goes through a sequence's chunks with its part of S in registers.
+// T = (I + A)^-1 in fp32, M, the rows' factors and K's transpose, all in the
+// order in which the scans' products read them. scan_kernel and, for calls of
+// few heads and sequences, scan_few_kernel go through a sequence's chunks with
+// their part of S in registers.
 //
 // Rounding. States, sums, decays and norms are fp32 (the sums G fp64: their
 // differences are what counts). The products are MFMAs of bf16: K and Q are
@@ -44,7 +45,10 @@ __device__ __forceinline__ float beta_of(const LinearArgs& a, float z) { return 
 // One token for each sequence. A workgroup has kStepCols columns of a head's
 // state, a thread 4 columns of every 32nd row; S^T k and S^T q come from the
 // state before the token (o = e^g S^T q + (q.k) u), so that one exchange
-// between the waves serves both. Bound by the states' bytes.
+// between the waves serves both. Bound by the states' bytes: 64 sequences with
+// 32 heads of 128 x 128 read and write 268 MB in 57 us, 4.7 TB/s (a large copy
+// reaches 4.9). 32 columns a workgroup leave each thread 16 floats of state, all
+// of whose loads are under way at a time.
 // ---------------------------------------------------------------------------
 template <class H, int DK>
 __global__ __launch_bounds__(256) void step_kernel(LinearArgs a, int v_dim, uint32_t col_blocks) {
@@ -143,8 +147,14 @@ constexpr int kBytesHead = kBytesT + kBytesM + kFactors * kChunk * 4;
 // K's transpose for a key head: [DK / 16][32 tokens] fragments.
 constexpr int bytes_kt(int k_dim) { return k_dim * kChunk * 2; }
 
-int64_t linear_workspace(int64_t tokens, int64_t batch, int64_t k_heads, int64_t v_heads, int64_t k_dim, bool beta) {
-  return linear_chunks(tokens, batch) * (v_heads * kBytesHead + k_heads * bytes_kt((int)k_dim));
+// Batches up to this size go through scan_kernel longest sequence first: its
+// workgroups come to the compute units as these become free, and a long one that
+// starts late is what the call then waits for (16 sequences of 64 to 1105 tokens,
+// in 512 workgroups: ORDERED us). prepare_kernel ranks the sequences, each against all.
+constexpr int kOrdered = 1024;
+
+int64_t linear_workspace(int64_t tokens, int64_t batch, int64_t k_heads, int64_t v_heads, int64_t k_dim) {
+  return linear_chunks(tokens, batch) * (v_heads * kBytesHead + k_heads * bytes_kt((int)k_dim)) + kOrdered * (int64_t)sizeof(int32_t);
 }
 
 __device__ __forceinline__ uint8_t* head_data(const LinearArgs& a, int chunk, int head) {
@@ -153,6 +163,9 @@ __device__ __forceinline__ uint8_t* head_data(const LinearArgs& a, int chunk, in
 __device__ __forceinline__ uint8_t* key_data(const LinearArgs& a, int chunk, int kh, int k_dim) {
   return a.workspace + linear_chunks(a.b.tokens, a.b.batch) * a.v_heads * kBytesHead +
          ((int64_t)chunk * a.k_heads + kh) * bytes_kt(k_dim);
+}
+__device__ __forceinline__ int32_t* ordered(const LinearArgs& a, int k_dim) {
+  return reinterpret_cast<int32_t*>(key_data(a, (int)linear_chunks(a.b.tokens, a.b.batch), 0, k_dim));
 }
 
 // Two fp32 values as sums of bf16 ones: x = p0 + p1 + p2 to 24 bits. What a
@@ -236,6 +249,16 @@ __device__ __forceinline__ int state_row(int m, int g) { return 32 * (m >> 1) + 
 // The lower triangle's fragments: of row tile t the 32 columns x, x <= t / 2.
 __device__ __forceinline__ int fragment_of(int t, int x) { return x ? t + 2 : t; }
 
+// One workgroup for a chunk of a value head; a wave has 16 of the chunk's rows.
+//   A, M   K K^T and Q K^T by MFMAs (fp16 as it is), times the decays between
+//          the rows, e^(G_i - G_j) of fp64 differences
+//   T      A's diagonal blocks of 16 rows inverted by forward substitution, a
+//          column a lane; the blocks below from those, T_ij = -T_ii (sum of
+//          A_ik T_kj), as fp32 MFMAs whose results are the next one's operand
+// 16384 tokens of 32 heads (16 key heads) of 128: 105 us. It writes T in three
+// and M in two bf16 parts (32 KB a chunk and head, 269 MB) and K's transpose,
+// and reads K and Q for each value head: 3.5 TB/s. Substitution over the whole 64
+// rows instead of blocks made it 480 us: one chain of 64 dependent steps.
 template <class H, int DK, bool BETA>
 __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
   constexpr int KS = DK / 32, kRow = 68, kRowK = DK + 8, kRowD = 20;
@@ -262,6 +285,18 @@ __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
         if (t < lo || t >= hi)
           *reinterpret_cast<uint4*>(a.out + ((int64_t)t * a.v_heads + head) * v_dim + i % (v_dim / 8) * 8) = uint4{0, 0, 0, 0};
       }
+  }
+
+  // sequence `place` by its length: how many are longer, or as long and before it
+  if (head == 0 && wave == 0 && b.batch <= kOrdered && place < b.batch) {
+    const auto length = [&](int i) { return clamp_to(b.starts[i + 1], b.tokens) - clamp_to(b.starts[i], b.tokens); };
+    const int mine = length(place);
+    int rank = 0;
+    for (int b0 = 0; b0 < b.batch; b0 += 64) {
+      const int i = min(b0 + lane, b.batch - 1), n = length(i);
+      rank += __popcll(__ballot(b0 + lane < b.batch && (n > mine || (n == mine && i < place))));
+    }
+    if (lane == 0) ordered(a, DK)[rank] = place;
   }
 
   // the sequence whose chunk this is
@@ -514,8 +549,12 @@ __device__ __forceinline__ void settle(f32x4 (&r)[N]) {
 // chunk's time before (copies straight into LDS are not used: the compiler
 // waits for all of those in flight at any read of LDS).
 //
-// What bounds it: the 182 MFMAs of a wave's chunk (DK 128), 2900 cycles, beside
-// 450 VALU instructions.
+// What bounds it: LDS. Each of the 8 waves reads all of the left operands, 1.1
+// MB a chunk at 128 B a cycle, with 182 MFMAs and some 780 VALU instructions of a
+// wave beside it: 6.8 us a chunk (DK 128). A call takes as long as the chunks
+// of its longest sequence. 16 sequences of 16 to 1900 tokens, 32 heads of 128 x 128:
+// 200 us. 32 columns a wave, which would halve the reads, took 248: their sums
+// no longer fit the registers without moves to and from the accumulators.
 //
 // A chunk whose U is not finite is gone through again: what lies behind a
 // column's first row that is not finite is left out, where it would reach the
@@ -536,7 +575,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void scan_kernel(LinearArgs a, int
   const uint32_t unit_size = (uint32_t)a.group * col_blocks, round = blockIdx.x / (8 * unit_size), within = blockIdx.x % (8 * unit_size);
   const uint32_t units = min((uint32_t)(b.batch * a.k_heads) - round * 8, 8u);
   const uint32_t unit = round * 8 + within % units, inner = within / units, cb = inner % col_blocks;
-  const int kh = (int)(unit % (uint32_t)a.k_heads), seq = (int)(unit / (uint32_t)a.k_heads), head = kh * a.group + (int)(inner / col_blocks);
+  const int kh = (int)(unit % (uint32_t)a.k_heads), rank = (int)(unit / (uint32_t)a.k_heads), head = kh * a.group + (int)(inner / col_blocks);
+  const int seq = b.batch <= kOrdered ? __builtin_amdgcn_readfirstlane(uniform_at(ordered(a, DK), rank)) : rank;
   const int start = clamp_to(uniform_at(b.starts, seq), b.tokens), n = clamp_to(uniform_at(b.starts, seq + 1), b.tokens) - start;
   if (n <= 0) return;
   const int from = uniform_at(b.from, seq), to = uniform_at(b.slots, seq);
@@ -844,6 +884,12 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void scan_kernel(LinearArgs a, int
 // issue is a wait of 16 to 32 cycles). An operand is loaded for the next chunk once
 // this one has used it, so that a load has most of a chunk's time and no
 // register of its own.
+//
+// What bounds it: the chain of a chunk, 4600 cycles: the split of S 450, K S 750,
+// D 500, T D 360, U 590, K^T U 720, and the exchanges between them. One sequence
+// of 16384 tokens, 32 heads (16 key heads) of 128 x 128: 256 chunks in 530 us. With
+// waves 4 to 7 left out it is 690; K S as partial sums of the waves, exchanged
+// instead of the state's parts, 600; 16 columns a wave for all 64 rows 1290.
 template <class H, int DK, int kCols, bool BETA>
 __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_dim, uint32_t col_blocks) {
   constexpr int KS = DK / 32, MT = DK / 64, NT = kCols / 16, NP = Parts<H>::n;
@@ -1276,6 +1322,13 @@ static void launch_prompt(const LinearArgs& a, int v_dim, hipStream_t stream) {
   prepare_kernel<H, DK, BETA><<<places * (uint32_t)a.v_heads, 256, 0, stream>>>(a, v_dim);
   const uint32_t heads = (uint32_t)a.b.batch * (uint32_t)a.v_heads, cols = (uint32_t)v_dim, w16 = heads * (cols / 16);
   const uint32_t cus = (uint32_t)max(cu_count_of(-1), 1);
+  // Which scan: few columns a workgroup as long as that gives each compute unit
+  // one (two, where the state's parts in LDS are small or the wide one's workgroups
+  // few). Whole calls of 1024 tokens a sequence in us, 16 / 32 columns / scan_kernel:
+  //   16 key and 32 value heads of 128 x 128   1 sequence 54 / 72 / 119, 2 82 / 77 / 124, 3 123 / 130 / 133,
+  //                                            4 155 / 138 / 139, 8 304 / 271 / 197, 16 584 / 503 / 391
+  //   14 heads of 64 x 64                      up to 4 37-42 / - / 72-75, 8 63 / - / 85, 12 89 / - / 93, 16 120 / - / 117
+  //   5 heads of 256 x 256                     up to 3 69-71 / - / 144-146, 6 128 / - / 153, 8 180 / - / 156
   if (w16 <= (DK == 128 ? cus : 2 * cus))
     scan_few_kernel<H, DK, 16, BETA><<<w16, 512, 0, stream>>>(a, v_dim, cols / 16);
   else if (DK == 128 && w16 / 2 <= cus)

@@ -38,6 +38,7 @@ from .norms import _ptr, _weight, gated_norm
 CONV_WIDTHS = (2, 3, 4)
 CONV_MAX_CHANNELS = 65536
 _CONV_ACTIVATIONS = {None: 0, "silu": 1}
+_TINY = torch.finfo(torch.float32).tiny
 
 
 def _batch(slots: torch.Tensor, from_slots: torch.Tensor | None, query_starts: torch.Tensor | None, tokens: int, index: int) -> tuple:
@@ -111,8 +112,8 @@ def _gate(name: str, t: torch.Tensor, dtype: torch.dtype, tokens: int, heads: in
 
 
 @lru_cache(maxsize=4096)
-def _workspace(tokens: int, batch: int, k_heads: int, v_heads: int, k_dim: int, v_dim: int, ragged: bool, beta: bool) -> int:
-    size = _lib.lib().jv_linear_attention_workspace_bytes(tokens, batch, k_heads, v_heads, k_dim, v_dim, ragged, beta)
+def _workspace(tokens: int, batch: int, k_heads: int, v_heads: int, k_dim: int, v_dim: int, ragged: bool) -> int:
+    size = _lib.lib().jv_linear_attention_workspace_bytes(tokens, batch, k_heads, v_heads, k_dim, v_dim, ragged)
     if size < 0:
         _lib.check(_lib.JV_ERR_VALUE)
     return size
@@ -173,12 +174,12 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     if rate is None and decay_bias is not None:
         raise ValueError("a decay bias goes with the heads' rates")
     rate, decay_bias = _weight("rate", rate, v_heads, index), _weight("decay_bias", decay_bias, v_heads, index)
-    if norm_eps is not None and not norm_eps > 0:
-        raise ValueError(f"norm_eps is positive, got {norm_eps}")
+    if norm_eps is not None and not norm_eps >= _TINY:  # a smaller one would be none in 32 bits
+        raise ValueError(f"norm_eps is at least {_TINY}, got {norm_eps}")
     batch, slots, from_slots, query_starts = _batch(slots, from_slots, query_starts, tokens, index)
     out = torch.empty(tokens, v_heads, v_dim, dtype=dtype, device=q.device)
     if tokens:
-        size = _workspace(tokens, batch, k_heads, v_heads, k_dim, v_dim, query_starts is not None, beta is not None)
+        size = _workspace(tokens, batch, k_heads, v_heads, k_dim, v_dim, query_starts is not None)
         ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
         with _on(index):
             _lib.check(_lib.lib().jv_linear_attention(

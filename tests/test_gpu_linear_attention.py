@@ -238,6 +238,20 @@ def test_prompts_of_every_layout(heads, dims, beta, dtype):
     Case(3, [65, 130], heads, dims, dtype, beta, raw=not beta, norm=False).check()
 
 
+# Sequences without tokens that bring a batch of four value heads to each of the scans: 16 and 32 columns a workgroup, 64 and 128.
+SCANS = [((64, 64), 0), ((128, 128), 9), ((64, 64), 45), ((128, 128), 20)]
+
+
+@pytest.mark.parametrize("heads,dims", LAYOUTS + [((2, 4), (64, 128))])
+@pytest.mark.parametrize("beta", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("columns", [300, 700])
+def test_prompts_of_every_layout_in_large_batches(heads, dims, beta, dtype, columns):
+    """As above in the scans for more than 256 and 512 times 16 state columns, which batches of empty sequences reach too."""
+    empty = columns * 16 // (heads[1] * dims[1]) + 1
+    Case(5, [0] * (empty // 2) + [70, 3, 128, 65, 1] + [0] * (empty // 2), heads, dims, dtype, beta, raw=beta).check()
+
+
 @pytest.mark.parametrize("lengths", [[1], [2], [63], [64], [65], [0], [0, 0, 5, 0, 64, 0], [127, 128, 129], [1] * 70, [3, 61, 64, 0, 1, 191, 16]])
 @pytest.mark.parametrize("beta", [True, False])
 def test_prompt_lengths(lengths, beta):
@@ -348,12 +362,13 @@ def test_strides_and_scale():
 @pytest.mark.parametrize("beta", [True, False])
 @pytest.mark.parametrize("what", ["v", "k", "q", "decay", "beta"])
 @pytest.mark.parametrize("value", [math.nan, math.inf])
-def test_what_is_not_finite_reaches_later_tokens_alone(what, value, beta):
+@pytest.mark.parametrize("dims,empty", SCANS)
+def test_what_is_not_finite_reaches_later_tokens_alone(what, value, beta, dims, empty):
     """Of a token in the middle of a chunk: the tokens before it, and the other sequences, heads and (for a value) channels
     keep their bits; what sees it is not finite."""
     if what == "beta" and not beta:
         return
-    c = Case(29, [40, 150, 70], dims=(64, 64), beta=beta)
+    c = Case(29, [40, 150, 70] + [0] * empty, dims=dims, beta=beta)
     clean, clean_states = c.run()
     at = 40 + 64 + 21
     if what == "v":
@@ -378,9 +393,10 @@ def test_what_is_not_finite_reaches_later_tokens_alone(what, value, beta):
     assert torch.equal(states[same], clean_states[same])
 
 
-def test_a_state_that_is_not_finite_stays_in_its_column():
+@pytest.mark.parametrize("dims,empty", SCANS)
+def test_a_state_that_is_not_finite_stays_in_its_column(dims, empty):
     for single in (True, False):
-        c = Case(30, [1, 1, 1] if single else [10, 130, 5], dims=(64, 64), single=single)
+        c = Case(30, [1, 1, 1] if single else [10, 130, 5] + [0] * empty, dims=dims, single=single)
         clean, clean_states = c.run()
         c.states[c.source[1], 2, 5, 33] = math.nan
         c.states[c.source[2]] = math.inf
@@ -493,7 +509,7 @@ def test_refusals():
                 lambda: ok(h, h, h, f32, states.transpose(2, 3), slots), lambda: ok(h, h, h, f32, states, slots[:2]),
                 lambda: ok(h, h, h, f32, states, slots, beta=f32.bfloat16()), lambda: ok(h, h, h, f32, states, slots, beta=f32[:3]),
                 lambda: ok(h, h, h, f32, states, slots, decay_bias=f32[0]), lambda: ok(h, h, h, f32, states, slots, rate=f32[:, 0]),
-                lambda: ok(h, h, h, f32, states, slots, norm_eps=0.0), lambda: ok(h, h, h, f32, states, slots, scale=math.inf),
+                lambda: ok(h, h, h, f32, states, slots, norm_eps=0.0), lambda: ok(h, h, h, f32, states, slots, norm_eps=1e-60), lambda: ok(h, h, h, f32, states, slots, scale=math.inf),
                 lambda: ok(h, h, h, f32, states, slots, query_starts=ints([0, 4])), lambda: ok(x.view(4, 8, 32), h, h, f32, states, slots)):
         with pytest.raises(ValueError):
             bad()

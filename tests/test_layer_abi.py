@@ -55,7 +55,7 @@ def test_causal_conv_refuses(product_lib, bad):
     dict(k_dim=96), dict(v_dim=32), dict(k_heads=0), dict(v_heads=0), dict(v_heads=3), dict(v_heads=1 << 17), dict(tokens=-1),
     dict(tokens=1 << 24), dict(tokens=1 << 23, v_heads=64), dict(batch=-1), dict(batch=0), dict(batch=(1 << 20) + 1), dict(starts=None),
     dict(slots=None), dict(n_slots=-1), dict(states=None), dict(states=P + 8), dict(scale=float("nan")), dict(scale=float("inf")),
-    dict(norm_eps=-1.0), dict(norm_eps=float("nan")), dict(rate=None), dict(q=None), dict(q=P + 2), dict(q_ts=4), dict(q_hs=2), dict(k=None),
+    dict(norm_eps=-1.0), dict(norm_eps=1e-40), dict(norm_eps=float("nan")), dict(rate=None), dict(q=None), dict(q=P + 2), dict(q_ts=4), dict(q_hs=2), dict(k=None),
     dict(v=None), dict(decay=None), dict(out=None), dict(out=P + 8), dict(ws=None), dict(ws=P + 16), dict(ws_bytes=64),
 ])
 def test_linear_attention_refuses(product_lib, bad):
@@ -71,11 +71,11 @@ def test_empty_calls_need_no_device(product_lib):
 
 def test_linear_attention_workspace_is_host_logic(product_lib):
     size = product_lib.jv_linear_attention_workspace_bytes
-    assert size(64, 64, 16, 32, 128, 128, 0, 1) == 0 and size(0, 3, 16, 32, 128, 128, 1, 1) == 0
-    one, two = size(1, 1, 16, 32, 128, 128, 1, 1), size(64, 1, 16, 32, 128, 128, 1, 1)
-    assert 0 < one < two and size(640, 1, 16, 32, 128, 128, 1, 1) == 11 * one
-    assert size(1 << 23, 1, 16, 64, 128, 128, 1, 1) == -1 and size(4, 1, 3, 4, 128, 128, 1, 1) == -1
-    assert size(4, 1, 4, 4, 100, 128, 1, 1) == -1
+    assert size(64, 64, 16, 32, 128, 128, 0) == 0 and size(0, 3, 16, 32, 128, 128, 1) == 0
+    one, two = size(1, 1, 16, 32, 128, 128, 1), size(64, 1, 16, 32, 128, 128, 1)
+    assert 0 < one < two and size(640, 1, 16, 32, 128, 128, 1) - two == 9 * (two - one)
+    assert size(1 << 23, 1, 16, 64, 128, 128, 1) == -1 and size(4, 1, 3, 4, 128, 128, 1) == -1
+    assert size(4, 1, 4, 4, 100, 128, 1) == -1
 
 
 def test_python_refuses_host_tensors_and_bad_names():
