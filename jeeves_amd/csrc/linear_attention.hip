@@ -149,8 +149,9 @@ constexpr int bytes_kt(int k_dim) { return k_dim * kChunk * 2; }
 
 // Batches up to this size go through scan_kernel longest sequence first: its
 // workgroups come to the compute units as these become free, and a long one that
-// starts late is what the call then waits for (16 sequences of 64 to 1105 tokens,
-// in 512 workgroups: ORDERED us). prepare_kernel ranks the sequences, each against all.
+// starts late is what the call then waits for (16 sequences of 64 to 1105 tokens
+// in 512 workgroups: 200 -> 165 us). prepare_kernel ranks the sequences, each
+// against all, which past this size costs more than it can give.
 constexpr int kOrdered = 1024;
 
 int64_t linear_workspace(int64_t tokens, int64_t batch, int64_t k_heads, int64_t v_heads, int64_t k_dim) {
@@ -255,10 +256,10 @@ __device__ __forceinline__ int fragment_of(int t, int x) { return x ? t + 2 : t;
 //   T      A's diagonal blocks of 16 rows inverted by forward substitution, a
 //          column a lane; the blocks below from those, T_ij = -T_ii (sum of
 //          A_ik T_kj), as fp32 MFMAs whose results are the next one's operand
-// 16384 tokens of 32 heads (16 key heads) of 128: 105 us. It writes T in three
-// and M in two bf16 parts (32 KB a chunk and head, 269 MB) and K's transpose,
-// and reads K and Q for each value head: 3.5 TB/s. Substitution over the whole 64
-// rows instead of blocks made it 480 us: one chain of 64 dependent steps.
+// What bounds it: its own bytes. 16384 tokens of 32 heads (16 key heads) of 128:
+// 105 us, 331 MB written (T in three and M in two bf16 parts, 32 KB a chunk and
+// head, and K's transpose) and 285 fetched, 5.9 TB/s. Substitution over the whole
+// 64 rows instead of blocks of 16 took 324: one chain of 64 dependent steps.
 template <class H, int DK, bool BETA>
 __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
   constexpr int KS = DK / 32, kRow = 68, kRowK = DK + 8, kRowD = 20;
@@ -549,12 +550,13 @@ __device__ __forceinline__ void settle(f32x4 (&r)[N]) {
 // chunk's time before (copies straight into LDS are not used: the compiler
 // waits for all of those in flight at any read of LDS).
 //
-// What bounds it: LDS. Each of the 8 waves reads all of the left operands, 1.1
-// MB a chunk at 128 B a cycle, with 182 MFMAs and some 780 VALU instructions of a
-// wave beside it: 6.8 us a chunk (DK 128). A call takes as long as the chunks
-// of its longest sequence. 16 sequences of 16 to 1900 tokens, 32 heads of 128 x 128:
-// 200 us. 32 columns a wave, which would halve the reads, took 248: their sums
-// no longer fit the registers without moves to and from the accumulators.
+// What bounds it: a chunk's steps one after another, two waves a SIMD to fill
+// each other's gaps. 6.8 us a chunk (DK 128); of a call's time MFMA is busy 30%,
+// LDS, where every wave reads all of the left operands, 25%, VALU 25%. A call takes as long
+// as the chunks of its longest sequence, or all chunks over the compute units. 16
+// sequences of 64 to 1105 tokens (149 chunks), 32 heads of 128 x 128: 165 us. 32
+// columns a wave, which would halve the reads, took 248 for 200: their sums no
+// longer fit the registers without moves to and from the accumulators.
 //
 // A chunk whose U is not finite is gone through again: what lies behind a
 // column's first row that is not finite is left out, where it would reach the

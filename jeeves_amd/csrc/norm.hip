@@ -3,9 +3,9 @@
 // norm, and the e4m3 codes that the next FP8 projection multiplies).
 //
 // Bound by bytes, each read and written once: 8192 rows of 4096, with a gate, a
-// residual and both norms, in 65 us (336 MB, 5.1 TB/s); 4099 rows of 4096 with gate to packed codes
-// in 21 us (84 MB, 4.0 TB/s; a 4 us share of it is the sigmoid and the quotients). One row: 3.3 us, a launch
-// and the row's way through memory once.
+// residual and both norms, in 65 us (336 MB, 5.2 TB/s, VALU 62%); 4099 rows of
+// 4096 with a gate to packed codes in 21 us (84 MB, 4.1 TB/s, VALU 67%: the
+// sigmoids, and quotients for the codes). One row: 3.3 us, a launch and memory's latency.
 #include "kernels.h"
 #include "layer.h"
 
