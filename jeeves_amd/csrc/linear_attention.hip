@@ -263,8 +263,8 @@ __device__ __forceinline__ int fragment_of(int t, int x) { return x ? t + 2 : t;
 template <class H, int DK, bool BETA>
 __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
   constexpr int KS = DK / 32, kRow = 68, kRowK = DK + 8, kRowD = 20;
-  // K's rows, and in their place A once they are read: five workgroups a CU
-  // instead of three (16384 tokens 120 -> 105 us).
+  // K's rows, and in their place A once they are read: four workgroups a CU,
+  // by registers, instead of three (16384 tokens 120 -> 105 us).
   constexpr int kShared = kChunk * (BETA && kRow * 4 > kRowK * 2 ? kRow * 4 : kRowK * 2);
   __shared__ __attribute__((aligned(16))) uint8_t shared[kShared];
   uint16_t* krows = reinterpret_cast<uint16_t*>(shared);
@@ -273,8 +273,12 @@ __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
   __shared__ __attribute__((aligned(16))) double sum[kChunk];
   __shared__ __attribute__((aligned(16))) float rk[kChunk], rq[kChunk], betas[kChunk];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int place = (int)(blockIdx.x / (uint32_t)a.v_heads), head = (int)(blockIdx.x % (uint32_t)a.v_heads), kh = head / a.group;
   const Batch& b = a.b;
+  // The hardware hands consecutive workgroups to the 8 XCDs in turn: the value
+  // heads of one chunk and key head, which read the same rows, come to one.
+  const uint32_t round_size = 8 * (uint32_t)a.group, round = blockIdx.x / round_size, within = blockIdx.x % round_size;
+  const uint32_t units = min(gridDim.x / (uint32_t)a.group - round * 8, 8u), unit = round * 8 + within % units;
+  const int place = (int)(unit / (uint32_t)a.k_heads), kh = (int)(unit % (uint32_t)a.k_heads), head = kh * a.group + (int)(within / units);
 
   // Tokens before the first sequence's and behind the last's come out as 0: of the batch's 64 from `place` x 64 on.
   {
