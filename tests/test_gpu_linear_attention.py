@@ -434,6 +434,8 @@ def test_long_prompt():
 def test_many_sequences():
     c = Case(33, [i % 4 for i in range(150)], heads=(1, 1), dims=(64, 64), raw=True, before=2)
     c.check()
+    c = Case(37, [i % 7 == 3 for i in range(1500)], heads=(1, 1), dims=(64, 64), raw=True, behind=1)  # too many to be ranked by length
+    c.check()
 
 
 @pytest.mark.parametrize("single", [True, False])
