@@ -6,7 +6,7 @@ Public API mirrors the reference's ``inference/fp8.py`` and
 ``libjeeves_fp8.so`` behind the C ABI of ``include/jeeves_fp8.h``. What lies
 between a model's FP8 projections -- norms, rotation, the paged cache, the
 attention -- is ``jeeves_amd.attention`` (``include/jeeves_attention.h``), for
-layers with linear attention ``jeeves_amd.linear_attention``
+layers with linear attention ``jeeves_amd.recurrent``
 (``include/jeeves_linear_attention.h``), and around every block
 ``jeeves_amd.norms`` (``include/jeeves_norm.h``).
 """
@@ -18,8 +18,8 @@ from .fp8 import (BLOCK_K, DECODE_MAX_ROWS, TILE_COUNTER_SLOTS, TILE_COUNTERS, W
                   tile_weight, tileable, untile_weight, warm)
 from .fp8_weights import (FP8, FP8_MAX, FP8_MAX_RECIPROCAL, QUANTIZE_BLOCK_ROWS, SCALE_SUFFIX, quantizable, quantize_row_blocks_on_cpu,
                           quantize_rows, replace_linears)
-from .linear_attention import FP8LinearAttention, causal_conv, linear_attention
 from .norms import add_norm, gated_norm
+from .recurrent import FP8LinearAttention, causal_conv, linear_attention
 
 __all__ = [
     "FP8Attention", "PagedKVCache", "append_kv", "paged_attention", "qk_norm_rope", "rope_table",

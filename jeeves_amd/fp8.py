@@ -893,7 +893,7 @@ def warm(module: nn.Module) -> int:
     before graph capture; attention blocks run their own operators. Returns the
     number of distinct (N, K)."""
     from .attention import FP8Attention  # which import this module
-    from .linear_attention import FP8LinearAttention
+    from .recurrent import FP8LinearAttention
 
     seen = set()
     for m in module.modules():

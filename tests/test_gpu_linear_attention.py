@@ -524,8 +524,7 @@ def test_refusals():
 # a run of them, as a layer has them
 # ---------------------------------------------------------------------------
 def block_of(g, hidden=256, hk=2, hv=4, d=64):
-    from jeeves_amd import FP8Linear
-    from jeeves_amd.linear_attention import FP8LinearAttention
+    from jeeves_amd import FP8Linear, FP8LinearAttention
 
     channels = 2 * hk * d + hv * d
     qkvz, out = FP8Linear(hidden, channels + hv * d, device=DEV), FP8Linear(hv * d, hidden, device=DEV)

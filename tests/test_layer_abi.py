@@ -112,8 +112,7 @@ def test_forward_codes_needs_per_token_codes():
 
 
 def test_linear_attention_block_checks_its_parts():
-    from jeeves_amd import FP8Linear
-    from jeeves_amd.linear_attention import FP8LinearAttention
+    from jeeves_amd import FP8Linear, FP8LinearAttention
 
     def block(outputs=512, inputs=128, gates=(4, 256), conv=(384, 4), k_heads=1, dims=(64, 64)):
         return FP8LinearAttention(FP8Linear(256, outputs), torch.zeros(gates), FP8Linear(inputs, 256), k_heads, 2, *dims, torch.zeros(conv),
