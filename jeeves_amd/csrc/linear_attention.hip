@@ -256,10 +256,11 @@ __device__ __forceinline__ int fragment_of(int t, int x) { return x ? t + 2 : t;
 //   T      A's diagonal blocks of 16 rows inverted by forward substitution, a
 //          column a lane; the blocks below from those, T_ij = -T_ii (sum of
 //          A_ik T_kj), as fp32 MFMAs whose results are the next one's operand
-// What bounds it: its own bytes. 16384 tokens of 32 heads (16 key heads) of 128:
-// 105 us, 331 MB written (T in three and M in two bf16 parts, 32 KB a chunk and
-// head, and K's transpose) and 285 fetched, 5.9 TB/s. Substitution over the whole
-// 64 rows instead of blocks of 16 took 324: one chain of 64 dependent steps.
+// What bounds it: its own bytes, and a workgroup's steps one after another, 24000
+// cycles with four of them on a compute unit (VALU 42%). 16384 tokens of 32 heads
+// (16 key heads) of 128: 105 us, 331 MB written (T in three and M in two bf16 parts,
+// 32 KB a chunk and head, and K's transpose) and 152 fetched, 4.6 TB/s. Substitution
+// over the whole 64 rows instead of blocks of 16 took 324: a chain of 64 steps.
 template <class H, int DK, bool BETA>
 __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
   constexpr int KS = DK / 32, kRow = 68, kRowK = DK + 8, kRowD = 20;
