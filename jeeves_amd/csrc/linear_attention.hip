@@ -19,8 +19,11 @@
 // Rounding. States, sums, decays and norms are fp32 (the sums G fp64: their
 // differences are what counts). The products are MFMAs of bf16: K and Q are
 // exact (one bf16, or two for fp16), and what is fp32 goes in as the sum of
-// three bf16 values (24 bits) towards the state, of two (16 bits) towards the
-// outputs, which are rounded to 8 or 11 bits once.
+// three bf16 values (24 bits), towards the state and towards the outputs: with
+// two values (16 bits) there, a whole call of 16384 tokens takes 612 us instead of
+// 654 and one of 16 prompts 210 instead of 223, but outputs that are small
+// differences lose their bits, and one in 300 (bf16) or 50 (fp16) of the others
+// is rounded to the neighbouring value.
 #include "layer.h"
 
 namespace jv {
@@ -137,10 +140,10 @@ __global__ __launch_bounds__(256) void step_kernel(LinearArgs a, int v_dim, uint
 typedef short bits8 __attribute__((ext_vector_type(8)));
 
 // A chunk's data for a value head in the workspace, in fragments of 64 lanes
-// of 16 bytes: T [lower fragment][3 parts], M [lower fragment][2 parts], then
+// of 16 bytes: T [lower fragment][3 parts], M [lower fragment][3 parts], then
 // the rows' factors.
 constexpr int kFragment = 1024;
-constexpr int kBytesT = 6 * 3 * kFragment, kBytesM = 6 * 2 * kFragment;
+constexpr int kBytesT = 6 * 3 * kFragment, kBytesM = kBytesT;
 enum { kFromK, kFromQ, kBeta, kToEnd, kEnd, kFactors = 8 };  // [8][64] floats; kEnd: the whole chunk's decay
 constexpr int kBytesHead = kBytesT + kBytesM + kFactors * kChunk * 4;
 
@@ -379,11 +382,11 @@ __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
   const int i = wave * 16 + r16;
   const double sum_i = sum[i];
   const float rk_i = rk[i], rq_i = rq[i], beta_i = betas[i];
-  uint2 mp[4][2];
+  uint2 mp[4][3];
   f32x4 pull[BETA ? 4 : 1];
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    mp[t][0] = mp[t][1] = uint2{0u, 0u};
+    mp[t][0] = mp[t][1] = mp[t][2] = uint2{0u, 0u};
     if (t > wave) continue;
     f32x4 kk = {0.0f, 0.0f, 0.0f, 0.0f}, qk = kk;
 #pragma unroll
@@ -401,16 +404,17 @@ __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
       if constexpr (BETA) pull[t][r] = j < i ? x : 0.0f;
       m[r] = j <= i ? y : 0.0f;
     }
-    uint32_t p[2][2];
-    split2<2>(m[0], m[1], p[0]), split2<2>(m[2], m[3], p[1]);
-    mp[t][0] = uint2{p[0][0], p[1][0]}, mp[t][1] = uint2{p[0][1], p[1][1]};
+    uint32_t p[2][3];
+    split2<3>(m[0], m[1], p[0]), split2<3>(m[2], m[3], p[1]);
+#pragma unroll
+    for (int x = 0; x < 3; ++x) mp[t][x] = uint2{p[0][x], p[1][x]};
   }
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     if (s > wave >> 1) continue;
-    uint4* m = reinterpret_cast<uint4*>(out + kBytesT) + fragment_of(wave, s) * 2 * 64 + lane;
+    uint4* m = reinterpret_cast<uint4*>(out + kBytesT) + fragment_of(wave, s) * 3 * 64 + lane;
 #pragma unroll
-    for (int p = 0; p < 2; ++p) m[p * 64] = uint4{mp[2 * s][p].x, mp[2 * s][p].y, mp[2 * s + 1][p].x, mp[2 * s + 1][p].y};
+    for (int p = 0; p < 3; ++p) m[p * 64] = uint4{mp[2 * s][p].x, mp[2 * s][p].y, mp[2 * s + 1][p].x, mp[2 * s + 1][p].y};
   }
   if (wave == 0) {
     const double d = sum[lane], all = sum[kChunk - 1];
@@ -567,11 +571,11 @@ __device__ __forceinline__ void settle(f32x4 (&r)[N]) {
 // column's first row that is not finite is left out, where it would reach the
 // rows before it as 0 times infinity, and comes out as NaN.
 template <class H, int DK, int NW, bool BETA>
-__global__ __launch_bounds__(64 * NW, NW / 4) void scan_kernel(LinearArgs a, int v_dim, uint32_t col_blocks) {
+__global__ __launch_bounds__(64 * NW, DK == 64 ? 2 : NW / 4) void scan_kernel(LinearArgs a, int v_dim, uint32_t col_blocks) {
   constexpr int kCols = 16 * NW, kRowO = kCols + 8;
-  constexpr int KS = DK / 32, MT = DK / 16, NP = Parts<H>::n;
+  constexpr int KS = DK / 32, MT = DK / 16, NP = Parts<H>::n, NU = BETA ? 3 : NP;  // parts of U: without beta it is V
   // fragments of 1 KB: what the first half of a chunk reads, and the second
-  constexpr int kK = 0, kQ = BETA ? 4 * KS : 0, kKt = kQ + 4 * KS, kM = kKt + 2 * MT, kT = kM + 12, kF = kT + (BETA ? 18 : 0), kV = kF + 2;
+  constexpr int kK = 0, kQ = BETA ? 4 * KS : 0, kKt = kQ + 4 * KS, kM = kKt + 2 * MT, kT = kM + 18, kF = kT + (BETA ? 18 : 0), kV = kF + 2;
   constexpr int kVs = 2 * NW;  // V's fragments
   __shared__ __attribute__((aligned(1024))) uint8_t lds[(kV + kVs) * kFragment];
   __shared__ __attribute__((aligned(16))) uint16_t ob[kChunk * kRowO];
@@ -616,7 +620,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void scan_kernel(LinearArgs a, int
   };
   // Its other operands, every NW-th fragment of each kind a wave's (a kind's
   // last one again where it has none), and V's rows [64][kCols].
-  constexpr int kKts = 2 * MT, kMs = 12, kTs = BETA ? 20 : 2;  // T's 18 and the factors' 2, in the order of LDS
+  constexpr int kKts = 2 * MT, kMs = 18, kTs = BETA ? 20 : 2;  // T's 18 and the factors' 2, in the order of LDS
   constexpr int kNKt = (kKts + NW - 1) / NW, kNM = (kMs + NW - 1) / NW, kNT = (kTs + NW - 1) / NW;
   i32x4 kt[kNKt], mt[kNM], tail[kNT], v8[2];
   const auto load_rest = [&](int c) {
@@ -685,7 +689,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void scan_kernel(LinearArgs a, int
             *reinterpret_cast<const uint4*>(&ob[row * kRowO + at % kCols]);
       }
     }
-    // K S and Q S, 16 rows a tile; towards the outputs two parts of S do
+    // K S and Q S, 16 rows a tile
     f32x4 pk[4], pq[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) pk[t] = pq[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -697,17 +701,13 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void scan_kernel(LinearArgs a, int
       for (int i = BETA ? 0 : 1; i < 2; ++i) {
         i32x4 rp[4][NP];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          i32x4 f = fragment((i ? kQ : kK) + t * KS + x);
-          if (rows < kChunk) f &= (t * 16 + r16 - rows) >> 31;  // rows behind the sequence's end are 0
-          Parts<H>::of(f, rp[t]);
-        }
+        for (int t = 0; t < 4; ++t) Parts<H>::of(fragment((i ? kQ : kK) + t * KS + x), rp[t]);
 #pragma unroll
-        for (int j = i ? 1 : 2; j >= 0; --j)
+        for (int j = 2; j >= 0; --j)
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
             f32x4& p = i ? pq[t] : pk[t];
-            if (NP > 1 && j < (i ? 1 : 2)) p = mfma_bf16(rp[t][NP - 1], sp[j], p);
+            if (NP > 1 && j < 2) p = mfma_bf16(rp[t][NP - 1], sp[j], p);
             p = mfma_bf16(rp[t][0], sp[j], p);
           }
       }
@@ -724,14 +724,15 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void scan_kernel(LinearArgs a, int
         const uint32_t v = *reinterpret_cast<const uint16_t*>(lds + kV * kFragment + ((t * 16 + r4 + r) * kCols + wave * 16 + r16) * 2);
         d[t][r] = H::lo(v);
       }
-      if (rows < kChunk)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) d[t][r] = t * 16 + r4 + r < rows ? d[t][r] : 0.0f;
       if constexpr (BETA) {
         const f32x4 from_k = factor(kFromK, t), beta = factor(kBeta, t);
 #pragma unroll
         for (int r = 0; r < 4; ++r) d[t][r] = __builtin_fmaf(-from_k[r], pk[t][r], beta[r] * d[t][r]);
       }
+      // rows behind the sequence's end, whose K, Q and V are its last row's, count nothing
+      if (rows < kChunk)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) d[t][r] = t * 16 + r4 + r < rows ? d[t][r] : 0.0f;
     }
     const auto solve = [&]() {
       if constexpr (BETA) {
@@ -803,15 +804,15 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void scan_kernel(LinearArgs a, int
     for (int t = 0; t < 4; ++t) o[t] = factor(kFromQ, t) * pq[t];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      i32x4 up[2];
+      i32x4 up[NU];
       split8(u[2 * x], u[2 * x + 1], up);
 #pragma unroll
-      for (int i = 1; i >= 0; --i) {
+      for (int i = 2; i >= 0; --i) {
         i32x4 mf[4];
 #pragma unroll
-        for (int t = 2 * x; t < 4; ++t) mf[t] = fragment(kM + fragment_of(t, x) * 2 + i);
+        for (int t = 2 * x; t < 4; ++t) mf[t] = fragment(kM + fragment_of(t, x) * 3 + i);
 #pragma unroll
-        for (int j = 1 - i; j >= 0; --j)
+        for (int j = min(2 - i, NU - 1); j >= 0; --j)
 #pragma unroll
           for (int t = 2 * x; t < 4; ++t) o[t] = mfma_bf16(mf[t], up[j], o[t]);
       }
@@ -884,7 +885,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void scan_kernel(LinearArgs a, int
 // work is spread over eight waves, in three steps with an exchange through LDS behind each:
 //   the state in three parts                               -> sb, as the right operand of K S and Q S
 //   D = beta (V - e^G K S) in three parts                  -> db, as that of T D
-//   U = T D in two parts, e^(G_C - G) U in three           -> ub, as that of M U and of K^T U, which gives the state
+//   U = T D and e^(G_C - G) U, each in three parts         -> ub, as that of M U and of K^T U, which gives the state
 // Waves 0 to 3 go through them, wave w with a chunk's rows from 16 w on and the
 // state's from w DK / 4 on. Waves 4 to 7 have the rows' outputs e^G Q S + M U,
 // which no later chunk waits for, and bring the factors and V to LDS (a load's
@@ -899,11 +900,11 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void scan_kernel(LinearArgs a, int
 // instead of the state's parts, 600; 16 columns a wave for all 64 rows 1290.
 template <class H, int DK, int kCols, bool BETA>
 __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_dim, uint32_t col_blocks) {
-  constexpr int KS = DK / 32, MT = DK / 64, NT = kCols / 16, NP = Parts<H>::n;
+  constexpr int KS = DK / 32, MT = DK / 64, NT = kCols / 16, NP = Parts<H>::n, NU = BETA ? 3 : NP;  // parts of U: without beta it is V
   constexpr int kRowS = DK + 8, kRowU = kChunk + 8;
   __shared__ __attribute__((aligned(16))) uint16_t sb[3][kCols * kRowS];
   __shared__ __attribute__((aligned(16))) uint16_t db[BETA ? 3 : 1][kCols * kRowU];
-  __shared__ __attribute__((aligned(16))) uint16_t ub[5][kCols * kRowU];
+  __shared__ __attribute__((aligned(16))) uint16_t ub[NU + 3][kCols * kRowU];
   __shared__ __attribute__((aligned(16))) float fb[2][5 * kChunk];            // the rows' factors, by turns
   __shared__ __attribute__((aligned(16))) uint16_t vb[2][kChunk * kCols];     // and V's rows
   __shared__ int first_d[kCols], first_us[2][kCols];  // a column's first row that is not finite; U's by turns
@@ -924,7 +925,7 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
   if (tid < kCols) first_d[tid] = first_us[chunk0 & 1][tid] = kChunk;
 
   if (all_wave >= 4) {
-    i32x4 qf[KS], mf[2][2];
+    i32x4 qf[KS], mf[2][3];
     const uint16_t* q_next = a.q + (int64_t)(start + row16) * a.q_ts + kh * a.q_hs + k8;
     const auto load_q = [&](int c) {
       const int rows = n - c * kChunk;
@@ -938,7 +939,8 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         if (x > (wave >> 1)) break;
-        mf[x][0] = p[fragment_of(wave, x) * 128], mf[x][1] = p[fragment_of(wave, x) * 128 + 64];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) mf[x][i] = p[(fragment_of(wave, x) * 3 + i) * 64];
       }
     };
     // 80 times 16 bytes of factors and kCols / 8 of each row of V
@@ -984,11 +986,12 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
         Parts<H>::of(qf[x], qp);
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
-          i32x4 sp[2];
+          i32x4 sp[3];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) sp[i] = *reinterpret_cast<const i32x4*>(&sb[i][(c * 16 + r16) * kRowS + x * 32 + k8]);
-          pq[c][0] = mfma_bf16(qp[0], sp[0], pq[c][0]), pq[c][1] = mfma_bf16(qp[0], sp[1], pq[c][1]);
-          if (NP > 1) pq[c][1] = mfma_bf16(qp[NP - 1], sp[0], pq[c][1]);
+          for (int i = 0; i < 3; ++i) sp[i] = *reinterpret_cast<const i32x4*>(&sb[i][(c * 16 + r16) * kRowS + x * 32 + k8]);
+          pq[c][1] = mfma_bf16(qp[0], sp[2], pq[c][1]), pq[c][0] = mfma_bf16(qp[0], sp[0], pq[c][0]);
+          pq[c][1] = mfma_bf16(qp[0], sp[1], pq[c][1]);
+          if (NP > 1) pq[c][1] = mfma_bf16(qp[NP - 1], sp[1], pq[c][1]), pq[c][1] = mfma_bf16(qp[NP - 1], sp[0], pq[c][1]);
         }
       }
       load_q(min(chunk + 1, last));
@@ -1011,10 +1014,16 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
         if (x > (wave >> 1)) break;
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
-          const i32x4 u0 = *reinterpret_cast<const i32x4*>(&ub[0][(c * 16 + r16) * kRowU + x * 32 + k8]);
-          const i32x4 u1 = *reinterpret_cast<const i32x4*>(&ub[1][(c * 16 + r16) * kRowU + x * 32 + k8]);
-          o[c][1] = mfma_bf16(mf[x][1], u0, o[c][1]), o[c][0] = mfma_bf16(mf[x][0], u0, o[c][0]);
-          o[c][1] = mfma_bf16(mf[x][0], u1, o[c][1]);
+          i32x4 up[NU];
+#pragma unroll
+          for (int i = 0; i < NU; ++i) up[i] = *reinterpret_cast<const i32x4*>(&ub[i][(c * 16 + r16) * kRowU + x * 32 + k8]);
+#pragma unroll
+          for (int i = 2; i >= 0; --i)
+#pragma unroll
+            for (int j = min(2 - i, NU - 1); j >= 0; --j) {
+              f32x4& sum = o[c][i + j > 0];
+              sum = mfma_bf16(mf[x][i], up[j], sum);
+            }
         }
       }
 #pragma unroll
@@ -1231,14 +1240,14 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
     const auto hand_over = [&]() {
 #pragma unroll
       for (int c = 0; c < NT; ++c) {
-        uint32_t p[2][2], w[2][3];
-        split2<2>(u[c][0], u[c][1], p[0]), split2<2>(u[c][2], u[c][3], p[1]);
+        uint32_t p[2][NU], w[2][3];
+        split2<NU>(u[c][0], u[c][1], p[0]), split2<NU>(u[c][2], u[c][3], p[1]);
         split2<3>(u[c][0] * to_end[0], u[c][1] * to_end[1], w[0]), split2<3>(u[c][2] * to_end[2], u[c][3] * to_end[3], w[1]);
         const int at = (c * 16 + r16) * kRowU + place4;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) *reinterpret_cast<uint2*>(&ub[i][at]) = uint2{p[0][i], p[1][i]};
+        for (int i = 0; i < NU; ++i) *reinterpret_cast<uint2*>(&ub[i][at]) = uint2{p[0][i], p[1][i]};
 #pragma unroll
-        for (int i = 0; i < 3; ++i) *reinterpret_cast<uint2*>(&ub[2 + i][at]) = uint2{w[0][i], w[1][i]};
+        for (int i = 0; i < 3; ++i) *reinterpret_cast<uint2*>(&ub[NU + i][at]) = uint2{w[0][i], w[1][i]};
       }
     };
     {
@@ -1274,7 +1283,7 @@ __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_di
       for (int c = 0; c < NT; ++c) {
         i32x4 up[3];
 #pragma unroll
-        for (int i = 0; i < 3; ++i) up[i] = *reinterpret_cast<const i32x4*>(&ub[2 + i][(c * 16 + r16) * kRowU + x * 32 + k8]);
+        for (int i = 0; i < 3; ++i) up[i] = *reinterpret_cast<const i32x4*>(&ub[NU + i][(c * 16 + r16) * kRowU + x * 32 + k8]);
         i32x4 kp[MT][NP];
 #pragma unroll
         for (int m = 0; m < MT; ++m) Parts<H>::of(kt[x][m], kp[m]);

@@ -1,0 +1,62 @@
+"""What the kernels between the projections of a linear attention layer keep of
+their inputs' bits, and what they do with calls at the edge of what their
+callers may ask."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.test_gpu_linear_attention import DEV, SCANS, ints, rounding, starts_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dims,empty", SCANS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("what,beta", [("state", True), ("state", False), ("products", True), ("products", False), ("updates", True)])
+def test_outputs_keep_32_bits(what, beta, dims, empty, dtype):
+    """Outputs that are the difference of two terms below 2 which agree to 12 bits or more: the terms come from the state, from
+    the products q.k or from the updates beta v, each of 24 bits. Three parts keep a term to 2^-24 of it and sums of two such
+    terms take 6 roundings of fp32 at most, so the difference is off by 8 x 2^-24 x 2 = 2^-20 and its own rounding; terms of
+    16 bits would put it off by up to 2^-16."""
+    from jeeves_amd import linear_attention
+
+    (dk, dv), hk, hv = dims, 2, 4
+    g = torch.Generator(DEV).manual_seed(dk + empty)
+    lengths = [40, 150, 70] + [0] * empty
+    starts, n = starts_of(lengths), len(lengths)
+    tokens = starts[-1]
+    q, k = torch.zeros(tokens, hk, dk, device=DEV), torch.zeros(tokens, hk, dk, device=DEV)
+    v, betas = torch.zeros(tokens, hv, dv, device=DEV), torch.ones(tokens, hv, device=DEV)
+    states = torch.zeros(n, hv, dk, dv, device=DEV)
+    near = torch.zeros(tokens, hv, dv, dtype=torch.float64, device=DEV)
+    for b, length in enumerate(lengths):
+        at, end = starts[b], starts[b + 1]
+        if not length:
+            continue
+        if what == "state":
+            q[at:end, :, :2] = 1
+            states[b, :, 0] = 1 + torch.rand(hv, dv, generator=g, device=DEV)
+            states[b, :, 1] = -states[b, :, 0] + torch.rand(hv, dv, generator=g, device=DEV) * 2.0 ** -13
+            near[at:end] = states[b, :, 0].double() + states[b, :, 1].double()
+            continue
+        v[at], v[at + 1] = 1, -1
+        if what == "products":
+            # 1 + 2^-9 (1 + m / 128) + n 2^-23 of the first two tokens' keys, which have no channel in common
+            q[at:end, :, :6] = 1
+            for h in range(hk):
+                m, low = 17 + 31 * b + h, (100 - h, 60 + b)
+                for t in range(2):
+                    k[at + t, h, 3 * t:3 * t + 3] = torch.tensor([1, 2.0 ** -9 * (1 + m / 128), low[t] * 2.0 ** -23], device=DEV)
+                first = 1 + 2.0 ** -9 * (1 + m / 128) + low[0] * 2.0 ** -23
+                near[at, 2 * h:2 * h + 2], near[at + 1:end, 2 * h:2 * h + 2] = first, (low[0] - low[1]) * 2.0 ** -23
+        else:
+            q[at:end, :, :2] = 1
+            k[at, :, 0] = k[at + 1, :, 1] = 1
+            betas[at] = 0.5 + 0.5 * torch.rand(hv, generator=g, device=DEV)
+            betas[at + 1] = betas[at] - torch.rand(hv, generator=g, device=DEV) * 2.0 ** -13
+            near[at], near[at + 1:end] = betas[at, :, None].double(), (betas[at] - betas[at + 1])[:, None].double()
+    out = linear_attention(q.to(dtype), k.to(dtype), v.to(dtype), torch.zeros(tokens, hv, device=DEV), states, ints(list(range(n))),
+                           beta=betas if beta else None, query_starts=ints(starts), scale=1.0)
+    assert ((out.double() - near).abs() <= rounding(near, dtype) + 2.0 ** -20).all(), (out.double() - near).abs().max().item()
