@@ -129,6 +129,12 @@ constexpr int kChunk = 64;
 // Chunks of a batch: sequence b's take the places from floor(start_b / 64) + b
 // on, which never meet those of b + 1.
 __host__ __device__ inline int64_t linear_chunks(int64_t tokens, int64_t batch) { return tokens / kChunk + batch; }
+// Of the batch's 64 tokens from `place` x 64 on those that there are: batches of
+// many sequences have places past the last token, 2^20 of them and more.
+__host__ __device__ inline int rows_at(int place, int tokens) {
+  const int n = tokens - place * kChunk;
+  return n < 0 ? 0 : n < kChunk ? n : kChunk;
+}
 int64_t linear_workspace(int64_t tokens, int64_t batch, int64_t k_heads, int64_t v_heads, int64_t k_dim);
 hipError_t linear_step(const LinearArgs& a, int k_dim, int v_dim, bool fp16, hipStream_t stream);
 hipError_t linear_prompt(const LinearArgs& a, int k_dim, int v_dim, bool fp16, hipStream_t stream);

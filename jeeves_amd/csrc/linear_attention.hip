@@ -287,10 +287,10 @@ __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
   // Tokens before the first sequence's and behind the last's come out as 0: of the batch's 64 from `place` x 64 on.
   {
     const int lo = clamp_to(uniform_at(b.starts, 0), b.tokens), hi = clamp_to(uniform_at(b.starts, b.batch), b.tokens);
-    const int at = place * kChunk, to = min(at + kChunk, b.tokens);
-    if (at < lo || to > hi)
-      for (int i = at * (v_dim / 8) + tid; i < to * (v_dim / 8); i += 256) {
-        const int t = i / (v_dim / 8);
+    const int at = place * kChunk, n = rows_at(place, b.tokens);
+    if (n > 0 && (at < lo || at + n > hi))
+      for (int i = tid; i < n * (v_dim / 8); i += 256) {
+        const int t = at + i / (v_dim / 8);
         if (t < lo || t >= hi)
           *reinterpret_cast<uint4*>(a.out + ((int64_t)t * a.v_heads + head) * v_dim + i % (v_dim / 8) * 8) = uint4{0, 0, 0, 0};
       }

@@ -7,7 +7,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_gpu_linear_attention import DEV, SCANS, ints, rounding, starts_of
+from jeeves_amd import linear_attention
+from tests.test_gpu_linear_attention import DEV, SCANS, Case, ints, rounding, starts_of
 
 pytestmark = pytest.mark.gpu
 
@@ -20,8 +21,6 @@ def test_outputs_keep_32_bits(what, beta, dims, empty, dtype):
     the products q.k or from the updates beta v, each of 24 bits. Three parts keep a term to 2^-24 of it and sums of two such
     terms take 6 roundings of fp32 at most, so the difference is off by 8 x 2^-24 x 2 = 2^-20 and its own rounding; terms of
     16 bits would put it off by up to 2^-16."""
-    from jeeves_amd import linear_attention
-
     (dk, dv), hk, hv = dims, 2, 4
     g = torch.Generator(DEV).manual_seed(dk + empty)
     lengths = [40, 150, 70] + [0] * empty
@@ -60,3 +59,24 @@ def test_outputs_keep_32_bits(what, beta, dims, empty, dtype):
     out = linear_attention(q.to(dtype), k.to(dtype), v.to(dtype), torch.zeros(tokens, hv, device=DEV), states, ints(list(range(n))),
                            beta=betas if beta else None, query_starts=ints(starts), scale=1.0)
     assert ((out.double() - near).abs() <= rounding(near, dtype) + 2.0 ** -20).all(), (out.double() - near).abs().max().item()
+
+
+def test_as_many_sequences_as_a_call_may_have():
+    """2^20 sequences, two of them with tokens, and tokens behind the last: places past the last token clear nothing."""
+    c = Case(60, [70, 110], heads=(1, 1), dims=(64, 256), raw=True, behind=20)
+    n, tokens = 1 << 20, c.v.shape[0]
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("the workspace takes 50 GB")
+    starts = torch.zeros(n + 1, dtype=torch.int32, device=DEV)
+    starts[6:], starts[n - 1:] = 70, 180
+    slots, source = torch.full((n,), -1, dtype=torch.int32, device=DEV), torch.full((n,), -1, dtype=torch.int32, device=DEV)
+    for b, seq in enumerate((5, n - 2)):
+        slots[seq], source[seq] = c.to[b], c.source[b]
+    states = c.states.clone()
+    out = linear_attention(c.q, c.k, c.v, c.decay, states, slots, beta=c.beta, rate=c.rate, decay_bias=c.bias, from_slots=source,
+                           query_starts=starts, norm_eps=c.norm_eps)
+    exact, mag, far, want, spread = c.exact()
+    assert out.shape[0] == tokens and (out[180:] == 0).all()
+    assert ((out.double() - exact).abs() <= rounding(exact, out.dtype) + 2.0 ** -14 * mag + 2.0 ** -17 * far).all()
+    assert ((states.double() - want).norm(dim=2) <= 2.0 ** -17 * spread).all()
+    torch.cuda.empty_cache()

@@ -4,10 +4,14 @@ their Python callers before they load the library's kernels."""
 
 from __future__ import annotations
 
+import shutil
+import subprocess
+from pathlib import Path
+
 import pytest
 import torch
 
-from jeeves_amd import _lib
+from jeeves_amd import _lib, build
 
 P = 4096  # an aligned address that no refused call follows
 
@@ -125,3 +129,26 @@ def test_linear_attention_block_checks_its_parts():
                 dict(outputs=384, conv=(256, 4), inputs=256), dict(k_heads=3), dict(dims=(96, 64))):
         with pytest.raises(ValueError):
             block(**bad)
+
+
+AMDCLANG = shutil.which("amdclang++") or "/opt/rocm/bin/amdclang++"
+
+
+@pytest.fixture(scope="module")
+def layer_rows(tmp_path_factory):
+    if not Path(AMDCLANG).exists():
+        pytest.skip("amdclang++ not found")
+    exe = tmp_path_factory.mktemp("rows") / "layer_rows"
+    subprocess.run([AMDCLANG, "-x", "hip", "--offload-host-only", "-O1", "-std=c++17", f"-I{build.CSRC}", f"-I{build.ROOT / 'include'}",
+                    str(build.ROOT / "tests" / "csrc" / "layer_rows.cpp"), "-o", str(exe)], check=True, capture_output=True, timeout=600)
+    return exe
+
+
+@pytest.mark.parametrize("tokens,batch", [(1, 1), (64, 1), (65, 3), (64, 1 << 20), (200, 1 << 20), ((1 << 23) - 1, 7), ((1 << 20) - 5, (1 << 20) - 3)])
+def test_places_share_the_tokens(product_lib, layer_rows, tokens, batch):
+    """Each token is one place's to clear, and none is a place's that lies past the last one: sizes up to the largest that a
+    call may have (one head of 256 channels), where an index over all places' rows would not fit 32 bits."""
+    size = product_lib.jv_linear_attention_workspace_bytes(tokens, batch, 1, 1, 64, 256, 1)
+    assert size > 0
+    got = subprocess.run([str(layer_rows), str(tokens), str(batch)], capture_output=True, text=True, check=True, timeout=60).stdout.split()
+    assert got == [str(tokens), str(min(tokens, 64)), "-1"]
