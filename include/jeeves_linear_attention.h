@@ -66,8 +66,8 @@ int64_t jv_linear_attention_workspace_bytes(int64_t tokens, int64_t batch, int64
  * v_dim 64, 128 or 256. states: float32 [n_slots, v_heads, k_dim, v_dim],
  * 16-byte aligned. out [tokens, v_heads, v_dim], contiguous. workspace:
  * 256-byte aligned. A token has no effect on those before it. Values that are
- * not finite stay visible: from the first of a chunk of 64 tokens on that gives
- * a non-finite update of a value channel, that channel is NaN until the
+ * not finite stay visible: from the first token on that gives a non-finite update
+ * u of a value channel, in a prompt or by itself, that channel is NaN until the
  * sequence's end and in its state. The role of the gated delta rule and of its
  * in-place step (model/fla_inplace.py:17-60) with their gates (_delta_gates,
  * model/triton_kernels.py:78).

@@ -117,6 +117,8 @@ __global__ __launch_bounds__(256) void step_kernel(LinearArgs a, int v_dim, uint
     const float sk = (parts[0][0][cl + e] + parts[0][1][cl + e]) + (parts[0][2][cl + e] + parts[0][3][cl + e]);
     const float sq = (parts[1][0][cl + e] + parts[1][1][cl + e]) + (parts[1][2][cl + e] + parts[1][3][cl + e]);
     u[e] = a.beta ? beta * (v[e] - decay * rk * sk) : v[e];
+    // an update that is not finite makes its channel NaN, in the state as well, as a prompt's does
+    if (!(__builtin_fabsf(u[e]) < __builtin_inff())) u[e] = __builtin_nanf("");
     o[e] = rq * __builtin_fmaf(rk * qk, u[e], decay * sq);
   }
   if (tid < 8)

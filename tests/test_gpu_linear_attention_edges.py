@@ -4,6 +4,8 @@ callers may ask."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -80,3 +82,29 @@ def test_as_many_sequences_as_a_call_may_have():
     assert ((out.double() - exact).abs() <= rounding(exact, out.dtype) + 2.0 ** -14 * mag + 2.0 ** -17 * far).all()
     assert ((states.double() - want).norm(dim=2) <= 2.0 ** -17 * spread).all()
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("single", [True, False])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("what,beta", [("v", True), ("v", False), ("k", True), ("decay", True), ("beta", True)])
+@pytest.mark.parametrize("dims,empty", SCANS)
+def test_an_update_that_is_not_finite_leaves_nan(what, beta, value, dims, empty, single):
+    """The same for single tokens and for prompts: the value channels of such an update are NaN from its token on, and in the
+    state; what does not see it keeps its bits."""
+    if what == "decay" and value < 0:
+        return  # a state dropped whole
+    c = Case(61, [1, 1, 1] if single else [40, 150, 70] + [0] * empty, dims=dims, beta=beta, single=single)
+    at, end = (1, 2) if single else (40 + 64 + 21, 190)
+    clean, clean_states = c.run()
+    heads, channels = slice(0, 2) if what == "k" else slice(1, 2), 17 if what == "v" else slice(None)
+    t = getattr(c, what).clone()
+    if what in ("v", "k"):
+        t[at, 0 if what == "k" else 1, channels if what == "v" else 9] = value
+    else:
+        t[at, 1] = value
+    setattr(c, what, t)
+    out, states = c.run()
+    hit, left = torch.zeros(out.shape, dtype=torch.bool, device=DEV), torch.zeros(states.shape, dtype=torch.bool, device=DEV)
+    hit[at:end, heads, channels], left[c.to[1], heads, :, channels] = True, True
+    assert out[hit].isnan().all() and states[left].isnan().all()
+    assert torch.equal(out[~hit], clean[~hit]) and torch.equal(states[~left], clean_states[~left])
