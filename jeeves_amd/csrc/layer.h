@@ -21,10 +21,11 @@ __device__ __forceinline__ float inv_sqrt(float m) {
   return r * (tiny ? 0x1p30f : 1.0f);
 }
 
-// 1 / d, d at least 1: the hardware's with one Newton step, which rounds as the
-// division does; past 2^126, where the hardware has no quotient, the division
-// (five instructions instead of ten: 16 prompts through the convolution 96 ->
-// 84 us).
+// 1 / d, d at least 1: the hardware's with one Newton step, which on this chip
+// gives the division's bits for every float (the tests go through all of them:
+// from any reciprocal within one unit the step would miss some); past 2^126, where
+// the hardware has no quotient, the division (five instructions instead of ten:
+// 16 prompts through the convolution 96 -> 84 us).
 __device__ __forceinline__ float inverse(float d) {
   if (d >= 0x1p126f) return 1.0f / d;
   const float r = __builtin_amdgcn_rcpf(d);

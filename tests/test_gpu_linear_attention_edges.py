@@ -4,13 +4,14 @@ callers may ask."""
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
 import torch
 
-from jeeves_amd import linear_attention
-from tests.test_gpu_linear_attention import DEV, SCANS, Case, ints, rounding, starts_of
+from jeeves_amd import causal_conv, linear_attention
+from tests.test_gpu_linear_attention import DEV, SCANS, Case, gen, ints, randn, rounding, starts_of
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +109,36 @@ def test_an_update_that_is_not_finite_leaves_nan(what, beta, value, dims, empty,
     hit[at:end, heads, channels], left[c.to[1], heads, :, channels] = True, True
     assert out[hit].isnan().all() and states[left].isnan().all()
     assert torch.equal(out[~hit], clean[~hit]) and torch.equal(states[~left], clean_states[~left])
+
+
+def test_reciprocal_rounds_as_the_division_does(hooks_lib):
+    """Every float from 1 to infinity."""
+    hooks_lib.th_inverse_sweep.argtypes = [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p]
+    count = torch.zeros(1, dtype=torch.int64, device=DEV)
+    assert hooks_lib.th_inverse_sweep(0x3F800000, 0x7F800001 - 0x3F800000, count.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    assert count.item() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("width,bias", [(2, True), (3, False), (4, True), (4, False)])
+@pytest.mark.parametrize("single", [True, False])
+def test_conv_has_the_bits_of_the_elementary_operations(single, width, bias, dtype):
+    """Products, sums in the inputs' order, exponential, sum, quotient and product, each rounded to 32 bits."""
+    g = gen(62 + width)
+    tokens, channels = (300, 1024)
+    x, weight = randn(g, tokens, channels, dtype=dtype) * 3, randn(g, channels, width, dtype=torch.float32)
+    b = randn(g, channels, dtype=torch.float32) if bias else None
+    n = tokens if single else 1
+    states = randn(g, n, width - 1, channels, dtype=dtype)
+    before = states.clone()
+    out = causal_conv(x, weight, states, ints(list(range(n))), bias=b, query_starts=None if single else ints([0, tokens]))
+    if single:
+        rows = torch.cat([before, x[:, None]], 1).float()
+        taps = [rows[:, j] for j in range(width)]
+    else:
+        rows = torch.cat([before[0], x]).float()
+        taps = [rows[j:j + tokens] for j in range(width)]
+    y = torch.zeros(tokens, channels, device=DEV) if b is None else b.expand(tokens, channels)
+    for j in range(width):
+        y = y + taps[j] * weight[:, j]
+    assert torch.equal(out, (y * (1 / (1 + torch.exp(-y)))).to(dtype))
