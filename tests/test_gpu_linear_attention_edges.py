@@ -142,3 +142,20 @@ def test_conv_has_the_bits_of_the_elementary_operations(single, width, bias, dty
     for j in range(width):
         y = y + taps[j] * weight[:, j]
     assert torch.equal(out, (y * (1 / (1 + torch.exp(-y)))).to(dtype))
+
+
+@pytest.mark.parametrize("single", [True, False])
+def test_decays_of_raw_gates_keep_32_bits(single):
+    """States of 1 that nothing is added to, so that they become the decays, for gates down to -85 with rates that bring g to
+    -1. softplus takes at most 8 roundings of 2^-24 (the exponential two), the rate one, so e^g is off by 9 x 2^-24 |g|; its
+    own exponential and the product add 4: below 2^-20 of the state."""
+    n, hv, d = 86, 2, 64
+    z = -torch.arange(n, dtype=torch.float32, device=DEV)[:, None].expand(n, hv) - torch.tensor([0.0, 0.37], device=DEV)
+    zeros = torch.zeros(n, hv, d, dtype=torch.bfloat16, device=DEV)
+    for at in range(n):
+        rate = (1 / torch.logaddexp(z[at].double(), torch.zeros(hv, dtype=torch.float64, device=DEV))).float()
+        states = torch.ones(1, hv, d, d, device=DEV)
+        linear_attention(zeros[:1], zeros[:1], zeros[:1], z[at:at + 1], states, ints([0]), rate=rate,
+                         query_starts=None if single else ints([0, 1]))
+        want = (-rate.double() * torch.logaddexp(z[at].double(), torch.zeros(hv, dtype=torch.float64, device=DEV))).exp()
+        assert ((states.double() / want[None, :, None, None] - 1).abs() <= 2.0 ** -20).all(), at
