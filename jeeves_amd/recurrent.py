@@ -32,7 +32,8 @@ import torch.nn as nn
 
 from . import _lib
 from .attention import _FP16, HEAD_DIMS, _first, _heads, _int32, _on, _refuse
-from .fp8 import FP8Linear
+from .device import sm_count
+from .fp8 import WARM_ROWS, FP8Linear
 from .norms import _ptr, _weight, gated_norm
 
 CONV_WIDTHS = (2, 3, 4)
@@ -225,19 +226,34 @@ class FP8LinearAttention(nn.Module):
 
     @torch.no_grad()
     def warm(self) -> None:
-        """Runs the operators between the projections in each of their forms,
-        keeping nothing, so that their kernels load before graph capture."""
-        device = self.qkvz.weight.device
+        """Runs what the block does around its FP8 linears, keeping nothing, so
+        that kernels load and the library of the small projection is set up
+        before graph capture: that projection and the out projection of codes
+        at ``WARM_ROWS``, single tokens, and prompts in batches that reach
+        each form of the linear attention, with the norm's codes and without."""
+        device, columns = self.qkvz.weight.device, self.v_heads * self.v_dim // 16
         conv_states, states = self.allocate(1)
-        none = torch.full((1,), -1, dtype=torch.int32, device=device)
-        for tokens in (1, 2):
-            starts = torch.tensor([0, tokens], dtype=torch.int32, device=device) if tokens > 1 else None
+        for rows in WARM_ROWS:
+            nn.functional.linear(torch.zeros(rows, self.qkvz.in_features, dtype=torch.bfloat16, device=device), self.gates)
+            if self.out.takes_codes():
+                z = torch.zeros(rows, self.v_heads, self.v_dim, dtype=torch.bfloat16, device=device)
+                self.out.forward_codes(*gated_norm(z, z, self.norm_weight, eps=self.eps, quantize="packed"), packed_rows=rows)
+        # the form goes by the state columns of a batch, 16 a workgroup, to the compute units
+        units = sm_count(device)
+        for sequences in (0, 1, units // columns + 1, 2 * units // columns + 1):
+            tokens, starts = 1, None
+            if sequences:
+                tokens, starts = 2, torch.full((sequences + 1,), 2, dtype=torch.int32, device=device)
+                starts[0] = 0
+            none = torch.full((max(sequences, 1),), -1, dtype=torch.int32, device=device)
             proj = torch.zeros(tokens, self.qkvz.out_features, dtype=torch.bfloat16, device=device)
-            self._between(proj, torch.zeros(tokens, 2 * self.v_heads, dtype=torch.bfloat16, device=device), conv_states, states, none,
-                          none, starts)
+            gates = torch.zeros(tokens, 2 * self.v_heads, dtype=torch.bfloat16, device=device)
+            for codes in {False, self.out.takes_codes()}:
+                self._between(proj, gates, conv_states, states, none, none, starts, codes)
 
     def _between(self, proj: torch.Tensor, gates: torch.Tensor, conv_states: torch.Tensor, states: torch.Tensor, slots: torch.Tensor,
-                 from_slots: torch.Tensor | None, query_starts: torch.Tensor | None) -> tuple[torch.Tensor | None, tuple | None]:
+                 from_slots: torch.Tensor | None, query_starts: torch.Tensor | None,
+                 codes: bool) -> tuple[torch.Tensor | None, tuple | None]:
         """(the out projection's input, None), or (None, its packed codes and scales)."""
         tokens, hk, hv, dk, dv = proj.shape[0], self.k_heads, self.v_heads, self.k_dim, self.v_dim
         mixed = causal_conv(proj[:, :self.channels], self.conv_weight, conv_states, slots, from_slots=from_slots, query_starts=query_starts)
@@ -246,7 +262,7 @@ class FP8LinearAttention(nn.Module):
                              beta=gates[:, hv:], rate=self.rate, decay_bias=self.decay_bias, from_slots=from_slots,
                              query_starts=query_starts, norm_eps=self.eps)
         z = proj[:, self.channels:].view(tokens, hv, dv)
-        if self.out.takes_codes():
+        if codes:
             return None, gated_norm(y, z, self.norm_weight, eps=self.eps, quantize="packed")
         return gated_norm(y, z, self.norm_weight, eps=self.eps).view(tokens, hv * dv), None
 
@@ -258,5 +274,5 @@ class FP8LinearAttention(nn.Module):
         if not x.shape[0]:
             return self.out(x.new_zeros(0, self.out.in_features))
         gates = nn.functional.linear(x.to(torch.bfloat16), self.gates)
-        y, codes = self._between(self.qkvz(x), gates, conv_states, states, slots, from_slots, query_starts)
+        y, codes = self._between(self.qkvz(x), gates, conv_states, states, slots, from_slots, query_starts, self.out.takes_codes())
         return self.out(y) if codes is None else self.out.forward_codes(*codes, packed_rows=x.shape[0])
