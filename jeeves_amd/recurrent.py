@@ -198,7 +198,8 @@ class FP8LinearAttention(nn.Module):
     values, gates z), the small 16-bit projection of decays and betas
     (``gates`` [2 v_heads, hidden]: decay rows, then beta rows), the convolution
     of q, k and v, the linear attention with keys of length 1, the gated norm
-    straight to the out projection's codes, and the out projection."""
+    straight to the out projection's codes, and the out projection (called as a
+    module, with 16-bit input, where it has hooks)."""
 
     def __init__(self, qkvz: FP8Linear, gates: torch.Tensor, out: FP8Linear, k_heads: int, v_heads: int, k_dim: int, v_dim: int,
                  conv_weight: torch.Tensor, rate: torch.Tensor, decay_bias: torch.Tensor, norm_weight: torch.Tensor, eps: float = 1e-6):
@@ -251,6 +252,15 @@ class FP8LinearAttention(nn.Module):
             for codes in {False, self.out.takes_codes()}:
                 self._between(proj, gates, conv_states, states, none, none, starts, codes)
 
+    def _codes(self) -> bool:
+        """Whether the out projection is given codes: not where its call is more than
+        its forward, as with hooks, which see its 16-bit input."""
+        out, every = self.out, nn.modules.module
+        return out.takes_codes() and not (
+            out._forward_pre_hooks or out._forward_hooks or out._backward_pre_hooks or out._backward_hooks or every._global_forward_pre_hooks
+            or every._global_forward_hooks or every._global_backward_pre_hooks or every._global_backward_hooks
+            or getattr(out.forward, "__func__", None) is not FP8Linear.forward)
+
     def _between(self, proj: torch.Tensor, gates: torch.Tensor, conv_states: torch.Tensor, states: torch.Tensor, slots: torch.Tensor,
                  from_slots: torch.Tensor | None, query_starts: torch.Tensor | None,
                  codes: bool) -> tuple[torch.Tensor | None, tuple | None]:
@@ -274,5 +284,5 @@ class FP8LinearAttention(nn.Module):
         if not x.shape[0]:
             return self.out(x.new_zeros(0, self.out.in_features))
         gates = nn.functional.linear(x.to(torch.bfloat16), self.gates)
-        y, codes = self._between(self.qkvz(x), gates, conv_states, states, slots, from_slots, query_starts, self.out.takes_codes())
+        y, codes = self._between(self.qkvz(x), gates, conv_states, states, slots, from_slots, query_starts, self._codes())
         return self.out(y) if codes is None else self.out.forward_codes(*codes, packed_rows=x.shape[0])

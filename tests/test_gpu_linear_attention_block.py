@@ -55,3 +55,34 @@ def test_warm_reaches_every_form(monkeypatch, d):
         want = block(x, *eager, slots, query_starts=starts)
         torch.cuda.synchronize()
         assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(held, eager))
+
+
+def test_hooks_of_the_projections_run():
+    """Those of the out projection too, which then takes the 16-bit input that they see."""
+    block = block_of(gen(75))
+    x, slots, seen = randn(gen(76), 6, 256), ints(list(range(6))), []
+    plain = block(x, *block.allocate(6), slots)
+    block.out.set_lora(torch.zeros(16, 256, device=DEV), torch.zeros(256, 16, device=DEV), 1.0)
+    sixteen = block(x, *block.allocate(6), slots)  # from 16-bit input, by an adapter that adds nothing
+    block.out.lora = None
+    handles = [block.qkvz.register_forward_hook(lambda m, a, y: seen.append("qkvz")),
+               block.out.register_forward_pre_hook(lambda m, a: seen.append(a[0].shape)),
+               block.out.register_forward_hook(lambda m, a, y: y + 1)]
+    hooked = block(x, *block.allocate(6), slots)
+    assert seen == ["qkvz", (6, 256)] and torch.equal(hooked, sixteen + 1)
+    for h in handles:
+        h.remove()
+    assert torch.equal(block(x, *block.allocate(6), slots), plain)
+    handle = torch.nn.modules.module.register_module_forward_pre_hook(lambda m, a: seen.append(m))
+    try:
+        block(x, *block.allocate(6), slots)
+    finally:
+        handle.remove()
+    assert block.out in seen
+
+    class Doubled(type(block.out)):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    block.out.__class__ = Doubled
+    assert torch.equal(block(x, *block.allocate(6), slots), 2 * sixteen)
