@@ -33,7 +33,7 @@ import torch.nn as nn
 from . import _lib
 from .attention import _FP16, HEAD_DIMS, _first, _heads, _int32, _on, _refuse
 from .device import sm_count
-from .fp8 import WARM_ROWS, FP8Linear
+from .fp8 import QUANT_MAX_PACKED_COLS, WARM_ROWS, FP8Linear
 from .norms import _ptr, _weight, gated_norm
 
 CONV_WIDTHS = (2, 3, 4)
@@ -205,14 +205,24 @@ class FP8LinearAttention(nn.Module):
                  conv_weight: torch.Tensor, rate: torch.Tensor, decay_bias: torch.Tensor, norm_weight: torch.Tensor, eps: float = 1e-6):
         super().__init__()
         channels = 2 * k_heads * k_dim + v_heads * v_dim
-        if v_heads % k_heads or k_dim not in HEAD_DIMS or v_dim not in HEAD_DIMS:
+        # what a call would refuse is refused here
+        if k_heads < 1 or v_heads < 1 or v_heads % k_heads or k_dim not in HEAD_DIMS or v_dim not in HEAD_DIMS:
             raise ValueError(f"{v_heads} value heads of {v_dim} do not go with {k_heads} key heads of {k_dim}")
         if qkvz.out_features != channels + v_heads * v_dim or out.in_features != v_heads * v_dim:
             raise ValueError(f"the projections have {qkvz.out_features} outputs and {out.in_features} inputs, the heads "
                              f"{channels + v_heads * v_dim} and {v_heads * v_dim}")
-        if gates.shape != (2 * v_heads, qkvz.in_features) or conv_weight.dim() != 2 or conv_weight.shape[0] != channels:
-            raise ValueError(f"gates must be [{2 * v_heads}, {qkvz.in_features}] and conv_weight [{channels}, width], got "
-                             f"{tuple(gates.shape)} and {tuple(conv_weight.shape)}")
+        if gates.shape != (2 * v_heads, qkvz.in_features) or conv_weight.dim() != 2 or conv_weight.shape[0] != channels \
+                or conv_weight.shape[1] not in CONV_WIDTHS:
+            raise ValueError(f"gates must be [{2 * v_heads}, {qkvz.in_features}] and conv_weight [{channels}, a width of {CONV_WIDTHS}], "
+                             f"got {tuple(gates.shape)} and {tuple(conv_weight.shape)}")
+        if channels > CONV_MAX_CHANNELS or v_heads * v_dim > QUANT_MAX_PACKED_COLS:
+            raise ValueError(f"q, k and v may have {CONV_MAX_CHANNELS} channels and the output {QUANT_MAX_PACKED_COLS}, got {channels} "
+                             f"and {v_heads * v_dim}")
+        for name, w, n in (("rate", rate, v_heads), ("decay_bias", decay_bias, v_heads), ("norm_weight", norm_weight, v_dim)):
+            if w.shape != (n,):
+                raise ValueError(f"{name} must be [{n}], got {tuple(w.shape)}")
+        if not _TINY <= eps < float("inf"):
+            raise ValueError(f"eps is at least {_TINY}, got {eps}")
         self.qkvz, self.out = qkvz, out
         self.k_heads, self.v_heads, self.k_dim, self.v_dim, self.channels, self.eps = k_heads, v_heads, k_dim, v_dim, channels, eps
         self.register_buffer("gates", gates.detach().to(torch.bfloat16))

@@ -131,6 +131,26 @@ def test_linear_attention_block_checks_its_parts():
             block(**bad)
 
 
+def test_linear_attention_block_refuses_what_a_call_would():
+    """More output channels than a norm's row has, more than the convolution's, widths, weights' shapes and eps: when it is
+    built, not at its first call."""
+    from jeeves_amd import FP8Linear, FP8LinearAttention
+
+    def block(k_heads=1, v_heads=2, k_dim=64, v_dim=64, width=4, rate=None, bias=None, norm=None, eps=1e-6):
+        channels, outputs = 2 * k_heads * k_dim + v_heads * v_dim, v_heads * v_dim
+        return FP8LinearAttention(FP8Linear(128, channels + outputs, device="meta"), torch.zeros(2 * v_heads, 128),
+                                  FP8Linear(outputs, 128, device="meta"), k_heads, v_heads, k_dim, v_dim, torch.zeros(channels, width),
+                                  torch.ones(v_heads if rate is None else rate), torch.zeros(v_heads if bias is None else bias),
+                                  torch.ones(v_dim if norm is None else norm), eps)
+
+    assert block(v_heads=64, v_dim=256).v_heads == 64
+    for bad in (dict(v_heads=65, v_dim=256), dict(k_heads=128, v_heads=128, k_dim=256), dict(width=1), dict(width=5), dict(rate=1),
+                dict(bias=3), dict(norm=128), dict(eps=0.0), dict(eps=-1.0), dict(eps=1e-40), dict(eps=float("nan")),
+                dict(eps=float("inf")), dict(k_heads=0), dict(v_heads=0)):
+        with pytest.raises(ValueError):
+            block(**bad)
+
+
 AMDCLANG = shutil.which("amdclang++") or "/opt/rocm/bin/amdclang++"
 
 
