@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_gpu_linear_attention import DEV, block_of, gen, ints, randn
+from tests.test_gpu_linear_attention import DEV, Case, block_of, gen, ints, randn, rounding, starts_of
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +86,53 @@ def test_hooks_of_the_projections_run():
 
     block.out.__class__ = Doubled
     assert torch.equal(block(x, *block.allocate(6), slots), 2 * sixteen)
+
+
+@pytest.mark.parametrize("lengths", [None, [5, 90, 1]])
+def test_block_against_its_steps_in_64_bits(monkeypatch, lengths):
+    """From the FP8 projection's own output on: the convolution has the bits of the elementary operations, the linear attention
+    is within its bound d of the recurrence in 64 bits, and the norm of what it stored is off by that and its own rounding: with
+    r the root mean square of a head, |w act(z)| / r (d + |y| |d| / |y|) in the 2-norms over the head, and u of the result. The
+    16-bit input of the out projection is compared, and the block's output is that projection of its codes, bit for bit."""
+    from jeeves_amd import gated_norm, recurrent
+
+    g = gen(80)
+    block = block_of(g)
+    n = len(lengths) if lengths else 3
+    starts = starts_of(lengths) if lengths else list(range(n + 1))
+    tokens, hk, hv, d = starts[-1], block.k_heads, block.v_heads, block.k_dim
+    x, (conv_states, states) = randn(g, tokens, 256), block.allocate(2 * n)
+    conv_states.copy_(randn(g, *conv_states.shape))
+    states.copy_(randn(g, *states.shape, dtype=torch.float32) * 0.3)
+    c = Case.__new__(Case)
+    c.lengths, c.starts, c.single = lengths or [1] * n, starts, lengths is None
+    c.to, c.source, c.norm_eps, c.rate, c.bias = list(range(n)), list(range(n, 2 * n)), block.eps, block.rate, block.decay_bias
+    c.states = states.clone()
+
+    proj, gates = block.qkvz(x), torch.nn.functional.linear(x, block.gates)
+    rows = torch.zeros(tokens, block.channels, device=DEV)
+    for b in range(n):
+        inputs = torch.cat([conv_states[n + b], proj[starts[b]:starts[b + 1], :block.channels]]).float()
+        for j in range(4):
+            rows[starts[b]:starts[b + 1]] += inputs[j:j + c.lengths[b]] * block.conv_weight[:, j]
+    mixed = (rows * (1 / (1 + torch.exp(-rows)))).bfloat16()
+    q, k, v = mixed.split([hk * d, hk * d, hv * d], 1)
+    c.q, c.k, c.v, c.decay, c.beta = q.view(tokens, hk, d), k.view(tokens, hk, d), v.view(tokens, hv, d), gates[:, :hv], gates[:, hv:]
+    y, mag, far, want, spread = c.exact()
+    off = rounding(y, torch.bfloat16) + 2.0 ** -14 * mag + 2.0 ** -17 * far
+
+    stored = []
+    monkeypatch.setattr(recurrent, "gated_norm", lambda y, *a, **kw: (stored.append(y), gated_norm(y, *a, **kw))[1])
+    out = block(x, conv_states, states, ints(c.to), from_slots=ints(c.source), query_starts=ints(starts) if lengths else None)
+    (y_stored,) = stored
+    z = proj[:, block.channels:].view(tokens, hv, d)
+    assert ((y_stored.double() - y).abs() <= off).all()
+    assert ((states.double() - want).norm(dim=2) <= 2.0 ** -17 * spread).all()
+    root = (y.square().mean(-1, keepdim=True) + block.eps).sqrt()
+    factor = block.norm_weight.double() * z.double() * torch.sigmoid(z.double())
+    normed = gated_norm(y_stored, z, block.norm_weight, eps=block.eps)
+    exact = y / root * factor
+    bound = factor.abs() / root * (off + y.abs() * off.norm(dim=-1, keepdim=True) / y.norm(dim=-1, keepdim=True)) * (1 + 2.0 ** -6)
+    assert ((normed.double() - exact).abs() <= bound + rounding(exact, torch.bfloat16) * (1 + 2.0 ** -6) + 2.0 ** -18 * exact.abs()).all()
+    codes = gated_norm(y_stored, z, block.norm_weight, eps=block.eps, quantize="packed")
+    assert torch.equal(out, block.out.forward_codes(*codes, packed_rows=tokens))
