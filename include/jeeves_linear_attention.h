@@ -15,7 +15,7 @@
  * (int32; NULL: slots; below 0 or past n_slots: the sequence starts from
  * zeros), slots[b] written (below 0 or past n_slots: nothing is kept). Several
  * sequences may start from one slot. A slot that two sequences write, or that
- * one reads and another writes, holds or gives either's. A sequence without
+ * one reads and another writes, holds or gives either's, value by value. A sequence without
  * tokens reads and writes nothing. Tokens of no sequence come out as 0.
  */
 #ifndef JEEVES_LINEAR_ATTENTION_H
@@ -45,7 +45,9 @@ int jv_causal_conv(const void* x, int64_t x_ts, const float* weight, const float
                    int64_t batch, void* out, int64_t tokens, int64_t channels, int fp16, void* stream);
 
 /* Bytes of workspace jv_linear_attention needs for these sizes (0: none); -1 if
- * the sizes are refused. ragged: whether starts are given. */
+ * the sizes are refused. ragged: whether starts are given. For every 64 tokens, and
+ * for every sequence, 38 KB a value head and 128 k_dim bytes a key head: 386 MB for
+ * 16384 tokens of 32 value and 16 key heads of 128. */
 int64_t jv_linear_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t k_heads, int64_t v_heads, int64_t k_dim,
                                             int64_t v_dim, int ragged);
 

@@ -9,7 +9,7 @@
 // A lane has 4 channels and a wave 256, for a run of R tokens, so an input row
 // is read (R + W - 1) / R times and the weights once a run, all of a run's rows
 // under way at a time. Bound by bytes and, as near, by the sigmoids: 11417 tokens
-// of 8192 channels in 85 us, 4.4 TB/s with VALU busy 88%; 96 with the exact
+// of 8192 channels in 84 us, 4.4 TB/s with VALU busy 88%; 96 with the exact
 // division instead of a corrected reciprocal, 134 with runs of 8 tokens and 8 channels a lane.
 #include "layer.h"
 

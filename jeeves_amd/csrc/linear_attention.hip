@@ -155,7 +155,7 @@ constexpr int bytes_kt(int k_dim) { return k_dim * kChunk * 2; }
 // Batches up to this size go through scan_kernel longest sequence first: its
 // workgroups come to the compute units as these become free, and a long one that
 // starts late is what the call then waits for (16 sequences of 64 to 1105 tokens
-// in 512 workgroups: 200 -> 165 us). prepare_kernel ranks the sequences, each
+// in 512 workgroups: a sixth of that scan's time). prepare_kernel ranks the sequences, each
 // against all, which past this size costs more than it can give.
 constexpr int kOrdered = 1024;
 
@@ -261,16 +261,16 @@ __device__ __forceinline__ int fragment_of(int t, int x) { return x ? t + 2 : t;
 //   T      A's diagonal blocks of 16 rows inverted by forward substitution, a
 //          column a lane; the blocks below from those, T_ij = -T_ii (sum of
 //          A_ik T_kj), as fp32 MFMAs whose results are the next one's operand
-// What bounds it: its own bytes, and a workgroup's steps one after another, 24000
+// What bounds it: its own bytes, and a workgroup's steps one after another, 25000
 // cycles with four of them on a compute unit (VALU 42%). 16384 tokens of 32 heads
-// (16 key heads) of 128: 105 us, 331 MB written (T in three and M in two bf16 parts,
-// 32 KB a chunk and head, and K's transpose) and 152 fetched, 4.6 TB/s. Substitution
+// (16 key heads) of 128: 109 us, 382 MB written (T and M in three bf16 parts, 38 KB a
+// chunk and head, and K's transpose) and 151 fetched, 4.9 TB/s. Substitution
 // over the whole 64 rows instead of blocks of 16 took 324: a chain of 64 steps.
 template <class H, int DK, bool BETA>
 __global__ __launch_bounds__(256) void prepare_kernel(LinearArgs a, int v_dim) {
   constexpr int KS = DK / 32, kRow = 68, kRowK = DK + 8, kRowD = 20;
   // K's rows, and in their place A once they are read: four workgroups a CU,
-  // by registers, instead of three (16384 tokens 120 -> 105 us).
+  // by registers, instead of three (an eighth of this kernel's time).
   constexpr int kShared = kChunk * (BETA && kRow * 4 > kRowK * 2 ? kRow * 4 : kRowK * 2);
   __shared__ __attribute__((aligned(16))) uint8_t shared[kShared];
   uint16_t* krows = reinterpret_cast<uint16_t*>(shared);
@@ -562,12 +562,12 @@ __device__ __forceinline__ void settle(f32x4 (&r)[N]) {
 // waits for all of those in flight at any read of LDS).
 //
 // What bounds it: a chunk's steps one after another, two waves a SIMD to fill
-// each other's gaps. 6.8 us a chunk (DK 128); of a call's time MFMA is busy 30%,
-// LDS, where every wave reads all of the left operands, 25%, VALU 25%. A call takes as long
+// each other's gaps. 6.8 us a chunk (DK 128); of a call's time MFMA is busy 34%,
+// LDS, where every wave reads all of the left operands, 25%, VALU 24%. A call takes as long
 // as the chunks of its longest sequence, or all chunks over the compute units. 16
-// sequences of 64 to 1105 tokens (149 chunks), 32 heads of 128 x 128: 165 us. 32
-// columns a wave, which would halve the reads, took 248 for 200: their sums no
-// longer fit the registers without moves to and from the accumulators.
+// sequences of 64 to 1105 tokens (149 chunks), 32 heads of 128 x 128: 166 to 174
+// us. 32 columns a wave, which would halve the reads, took a quarter more: their
+// sums no longer fit the registers without moves to and from the accumulators.
 //
 // A chunk whose U is not finite is gone through again: what lies behind a
 // column's first row that is not finite is left out, where it would reach the
@@ -895,11 +895,13 @@ __global__ __launch_bounds__(64 * NW, DK == 64 ? 2 : NW / 4) void scan_kernel(Li
 // this one has used it, so that a load has most of a chunk's time and no
 // register of its own.
 //
-// What bounds it: the chain of a chunk, 4600 cycles: the split of S 450, K S 750,
-// D 500, T D 360, U 590, K^T U 720, and the exchanges between them. One sequence
-// of 16384 tokens, 32 heads (16 key heads) of 128 x 128: 256 chunks in 530 us. With
-// waves 4 to 7 left out it is 690; K S as partial sums of the waves, exchanged
-// instead of the state's parts, 600; 16 columns a wave for all 64 rows 1290.
+// What bounds it: the chain of a chunk, 4850 cycles; taken apart when U went to the
+// outputs in two parts and it was 4600: the split of S 450, K S 750, D 500, T D 360,
+// U 590, K^T U 720, and the exchanges between them. One sequence of 16384 tokens, 32
+// heads (16 key heads) of 128 x 128: 256 chunks in 553 to 563 us. For the 525 of
+// those two parts it was 690 with waves 4 to 7 left out, 600 with K S as partial sums
+// of the waves, exchanged instead of the state's parts, and 1290 with 16 columns a
+// wave for all 64 rows.
 template <class H, int DK, int kCols, bool BETA>
 __global__ __launch_bounds__(512, 1) void scan_few_kernel(LinearArgs a, int v_dim, uint32_t col_blocks) {
   constexpr int KS = DK / 32, MT = DK / 64, NT = kCols / 16, NP = Parts<H>::n, NU = BETA ? 3 : NP;  // parts of U: without beta it is V
@@ -1343,10 +1345,11 @@ static void launch_prompt(const LinearArgs& a, int v_dim, hipStream_t stream) {
   // Which scan: few columns a workgroup as long as that gives each compute unit
   // one (two, where the state's parts in LDS are small or the wide one's workgroups
   // few). Whole calls of 1024 tokens a sequence in us, 16 / 32 columns / scan_kernel:
-  //   16 key and 32 value heads of 128 x 128   1 sequence 54 / 72 / 119, 2 82 / 77 / 124, 3 123 / 130 / 133,
-  //                                            4 155 / 138 / 139, 8 304 / 271 / 197, 16 584 / 503 / 391
-  //   14 heads of 64 x 64                      up to 4 37-42 / - / 72-75, 8 63 / - / 85, 12 89 / - / 93, 16 120 / - / 117
-  //   5 heads of 256 x 256                     up to 3 69-71 / - / 144-146, 6 128 / - / 153, 8 180 / - / 156
+  //   16 key and 32 value heads of 128 x 128   1 sequence 50 / 63 / 120, 2 82 / 69 / 126, 3 116 / 121 / 133,
+  //                                            4 145 / 127 / 138, 8 313 / 271 / 194, 16 612 / 528 / 388
+  //   14 heads of 64 x 64                      up to 4 39-45 / - / 68-74, 8 69 / - / 82, 12 94 / - / 92, 16 137 / - / 119
+  //   5 heads of 256 x 256                     up to 3 71-76 / - / 150, 6 132 / - / 154, 8 188 / - / 158
+  // All sequences here are of one length; a long one among short ones goes by their number all the same.
   if (w16 <= (DK == 128 ? cus : 2 * cus))
     scan_few_kernel<H, DK, 16, BETA><<<w16, 512, 0, stream>>>(a, v_dim, cols / 16);
   else if (DK == 128 && w16 / 2 <= cus)

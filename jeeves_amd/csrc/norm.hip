@@ -4,8 +4,9 @@
 //
 // Bound by bytes, each read and written once: 8192 rows of 4096, with a gate, a
 // residual and both norms, in 65 us (336 MB, 5.2 TB/s, VALU 62%); 4099 rows of
-// 4096 with a gate to packed codes in 21 us (84 MB, 4.1 TB/s, VALU 67%: the
-// sigmoids, and quotients for the codes). One row: 3.3 us, a launch and memory's latency.
+// 4096 with a gate to codes in 21 us as a call among others (84 MB, 4.0 TB/s, VALU
+// 67%: the sigmoids, and quotients for the codes), 28 by itself under a tracer, start
+// and end included. One row by itself: 3.3 us, a launch and memory's latency.
 #include "kernels.h"
 #include "layer.h"
 

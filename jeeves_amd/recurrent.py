@@ -13,7 +13,8 @@ A sequence carries its state in a slot: it is read from ``from_slots[b]`` and
 written to ``slots[b]``. ``from_slots`` defaults to ``slots``; a negative one
 starts a sequence from zeros, one slot may start several sequences (a shared
 prompt), and a negative entry of ``slots`` keeps nothing (padding). Slots
-written by one call are meant to differ, and not to be others' ``from_slots``.
+written by one call are meant to differ, and not to be others' ``from_slots``:
+each value of one that two write is either's.
 
 Tensors are bf16 or fp16, states of the linear attention float32. As in
 ``jeeves_amd.attention``, everything is enqueued on
@@ -149,7 +150,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
 
     States, sums and norms are in 32 bits, the output is rounded once; prompts
     go in chunks of 64 tokens, so a prompt's last bits differ from those of its
-    tokens one at a time. A token has no effect on those before it, whatever its
+    tokens one at a time, and take a workspace of 38 KB a value head and 128
+    k_dim bytes a key head for each 64 tokens and each sequence. A token has no effect on those before it, whatever its
     values; an update that is not finite makes its value channel NaN from that
     token on, and in the state.
     """
